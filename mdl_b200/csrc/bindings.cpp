@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <stdexcept>
@@ -948,6 +949,148 @@ void attn_simt_bwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Te
   g_launches += 3;
 }
 
+// ------------------------------------------------------------------ 4-bit key/value cache
+mdl::KvCache kv_cache_of(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table,
+                         const at::Tensor& lengths, const at::Tensor& err) {
+  require_cuda(codes, "codes");
+  TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 5 && codes.size(2) == 2 && codes.is_contiguous(),
+              "codes must be contiguous uint8 [pages, G, 2, page, hd / 2]");
+  TORCH_CHECK(scales.scalar_type() == at::kBFloat16 && scales.is_contiguous() && scales.dim() == 4 &&
+                  scales.numel() * (codes.size(4)) == codes.numel() && scales.size(0) == codes.size(0) &&
+                  scales.size(1) == codes.size(1),
+              "scales must be contiguous bf16 [pages, G, 2, page]");
+  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous(), "table must be int32 [R, n]");
+  TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.numel() == table.size(0),
+              "lengths must be int32 [R]");
+  TORCH_CHECK(codes.device() == scales.device() && codes.device() == table.device() &&
+                  codes.device() == lengths.device() && codes.device() == err.device(),
+              "the cache lies on one device");
+  mdl::KvCache c;
+  const int64_t page = codes.size(3);
+  TORCH_CHECK(page >= 16 && (page & (page - 1)) == 0, "page must be a power of two of at least 16");
+  while ((int64_t{1} << c.page_shift) < page) ++c.page_shift;
+  c.hd = static_cast<int>(codes.size(4) * 2);
+  TORCH_CHECK(c.hd == 32 || c.hd == 64, "head width must be 32 or 64");
+  TORCH_CHECK(codes.size(0) >= 1 && table.size(1) >= 1 && table.size(1) * page < (int64_t{1} << 31), "cache sizes");
+  c.codes = codes.data_ptr<uint8_t>();
+  c.scales = reinterpret_cast<__nv_bfloat16*>(scales.data_ptr());
+  c.table = table.data_ptr<int>();
+  c.lengths = lengths.data_ptr<int>();
+  c.R = static_cast<int>(table.size(0));
+  c.G = static_cast<int>(codes.size(1));
+  c.max_pages = static_cast<int>(table.size(1));
+  c.num_pages = static_cast<int>(codes.size(0));
+  c.err = err.data_ptr<int>();
+  return c;
+}
+
+// [n, T, width] bf16 whose rows are read in 16-byte pieces
+const __nv_bfloat16* kv_rows(const at::Tensor& t, int64_t n, int64_t T, int64_t width, const mdl::KvCache&,
+                             const at::Device& dev, const char* name, long long* sb, long long* st) {
+  TORCH_CHECK(t.device() == dev && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == n &&
+                  t.size(1) == T && t.size(2) == width && t.stride(2) == 1 && t.stride(0) % 8 == 0 &&
+                  t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be bf16 [", n, ", ", T, ", ", width, "] with 16-byte aligned rows");
+  *sb = t.stride(0);
+  *st = t.stride(1);
+  return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
+}
+
+const int* kv_index(const std::optional<at::Tensor>& t, int64_t n, const at::Device& dev, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == n, name,
+              " must be contiguous int32 [", n, "]");
+  return t->data_ptr<int>();
+}
+
+void kv_write(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
+              const at::Tensor& err, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& rows,
+              const std::optional<at::Tensor>& start, const std::optional<at::Tensor>& kstart) {
+  c10::cuda::CUDAGuard guard(codes.device());
+  mdl::KvWriteArgs a;
+  a.c = kv_cache_of(codes, scales, table, lengths, err);
+  TORCH_CHECK(k.dim() == 3, "k must be [n, T, G * hd]");
+  const int64_t n = k.size(0), T = k.size(1), width = static_cast<int64_t>(a.c.G) * a.c.hd;
+  TORCH_CHECK(T < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_write: sizes");
+  a.k = kv_rows(k, n, T, width, a.c, codes.device(), "k", &a.k_sb, &a.k_st);
+  a.v = kv_rows(v, n, T, width, a.c, codes.device(), "v", &a.v_sb, &a.v_st);
+  a.rows = kv_index(rows, n, codes.device(), "rows");
+  a.start = kv_index(start, n, codes.device(), "start");
+  a.kstart = kv_index(kstart, n, codes.device(), "kstart");
+  TORCH_CHECK(a.rows != nullptr || n <= a.c.R, "kv_write: more source rows than cache rows");
+  a.n = static_cast<int>(n);
+  a.T = static_cast<int>(T);
+  int launches = 0;
+  check(mdl::kv_write(a, stream_of(codes), &launches), "kv_write");
+  g_launches += launches;
+}
+
+void kv_read(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
+             const at::Tensor& err, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& rows,
+             const std::optional<at::Tensor>& start) {
+  c10::cuda::CUDAGuard guard(codes.device());
+  mdl::KvReadArgs a;
+  a.c = kv_cache_of(codes, scales, table, lengths, err);
+  TORCH_CHECK(k.device() == codes.device() && v.device() == codes.device() && k.is_contiguous() && v.is_contiguous() &&
+                  k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() &&
+                  k.size(2) == static_cast<int64_t>(a.c.G) * a.c.hd &&
+                  (k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat),
+              "kv_read: k and v must be contiguous bf16 or fp32 [n, count, G * hd]");
+  const int64_t n = k.size(0);
+  TORCH_CHECK(k.size(1) < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_read: sizes");
+  a.out_k = k.data_ptr();
+  a.out_v = v.data_ptr();
+  a.fp32 = k.scalar_type() == at::kFloat;
+  a.rows = kv_index(rows, n, codes.device(), "rows");
+  a.start = kv_index(start, n, codes.device(), "start");
+  TORCH_CHECK(a.rows != nullptr || n <= a.c.R, "kv_read: more rows than the cache has");
+  a.n = static_cast<int>(n);
+  a.count = static_cast<int>(k.size(1));
+  check(mdl::kv_read(a, stream_of(codes)), "kv_read");
+  g_launches += 1;
+}
+
+void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
+               const at::Tensor& err, const at::Tensor& q, const std::optional<at::Tensor>& k_new,
+               const std::optional<at::Tensor>& v_new, const std::optional<at::Tensor>& rows, const at::Tensor& out,
+               int64_t window, int64_t sinks, double scale) {
+  c10::cuda::CUDAGuard guard(codes.device());
+  mdl::KvAttendArgs a;
+  a.c = kv_cache_of(codes, scales, table, lengths, err);
+  TORCH_CHECK(q.dim() == 3 && q.size(2) % (static_cast<int64_t>(a.c.G) * a.c.hd) == 0 && q.size(2) > 0,
+              "q must be [B, N, H * hd] with H a multiple of the key heads");
+  const int64_t B = q.size(0), N = q.size(1), width = q.size(2), kw = static_cast<int64_t>(a.c.G) * a.c.hd;
+  TORCH_CHECK(B < (int64_t{1} << 30) && N * width / a.c.hd < (int64_t{1} << 30), "kv_attend: sizes");
+  a.q = kv_rows(q, B, N, width, a.c, codes.device(), "q", &a.q_sb, &a.q_sn);
+  TORCH_CHECK(k_new.has_value() == v_new.has_value(), "k_new and v_new come together");
+  if (k_new.has_value()) {
+    a.kn = kv_rows(*k_new, B, N, kw, a.c, codes.device(), "k_new", &a.kn_sb, &a.kn_sn);
+    a.vn = kv_rows(*v_new, B, N, kw, a.c, codes.device(), "v_new", &a.vn_sb, &a.vn_sn);
+  }
+  a.rows = kv_index(rows, B, codes.device(), "rows");
+  TORCH_CHECK(a.rows != nullptr || B <= a.c.R, "kv_attend: more batch rows than cache rows");
+  TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                  out.sizes() == q.sizes(), "out must be contiguous bf16 like q");
+  TORCH_CHECK(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.B = static_cast<int>(B);
+  a.N = static_cast<int>(N);
+  a.H = static_cast<int>(width / a.c.hd);
+  // positions stay below 2^31: larger ones would see the same
+  a.window = static_cast<int>(std::min<int64_t>(window, int64_t{1} << 30));
+  a.sinks = static_cast<int>(std::min<int64_t>(sinks, int64_t{1} << 30));
+  a.scale = static_cast<float>(scale);
+  at::Tensor ws;
+  const long long need = mdl::kv_attend_workspace(a);
+  if (need > 0) {
+    ws = at::empty({need}, q.options().dtype(at::kFloat));
+    a.partial = ws.data_ptr<float>();
+  }
+  int launches = 0;
+  check(mdl::kv_attend(a, stream_of(codes), &launches), "kv_attend");
+  g_launches += launches;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1013,6 +1156,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("Lq"), py::arg("causal"), py::arg("scale"), py::arg("err") = py::none(), py::arg("ktail") = 0,
         py::arg("kexcl") = 0);
   m.def("position_add", &position_add);
+  m.def("kv_write", &kv_write);
+  m.def("kv_read", &kv_read);
+  m.def("kv_attend", &kv_attend);
   m.def("position_grad", &position_grad);
   m.def("sqa_fwd", &sqa_fwd);
   m.def("sqa_shared_fwd", &sqa_shared_fwd);

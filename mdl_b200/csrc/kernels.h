@@ -7,6 +7,7 @@
 #include "embedding.h"
 #include "fmha.h"
 #include "gemm.h"
+#include "kv_cache.h"
 #include "misc.h"
 #include "norm.h"
 #include "sqa.h"

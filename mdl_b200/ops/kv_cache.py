@@ -1,0 +1,336 @@
+"""Key/value cache held in 4 bits: written as tokens arrive, read back, attended to.
+
+A request cache holds the keys and values of a history's tokens. In bf16 it costs
+``4 * head_dim`` bytes a token and head; here a head's row of a token is one bf16
+scale and ``head_dim`` 4-bit codes, ``head_dim + 4`` bytes for its key and value:
+
+* ``s = bf16(max |x| / 7)``, ``c = clamp(round(x / s), -7, 7)`` (ties to even), value
+  ``s * c``; a row of zeros (or one whose ``s`` underflows) has ``s = 0`` and ``c = 0``,
+  a row that holds an infinity or a NaN reads back as NaN;
+* tokens lie in pages of ``page`` positions, found through a table per cache row, so
+  rows of very different lengths share one pool.
+
+``kv_cache_write`` appends (or writes from a given position), ``kv_cache_read`` gives
+the values of a run of positions, ``cached_attention`` attends to a row: a single new
+token whose key is in the cache already, or candidates that bring fresh keys of their
+own (OneTrans NS tokens over their request's history), with an optional sliding
+window and always-visible first tokens. None of them has a gradient.
+
+CUDA: the kernels of ``csrc/kv_cache.cu`` (bf16, head widths 32 and 64); rows, pages
+and positions outside the cache are skipped and recorded in the device error word
+(``check_error_word``). CPU: the same contract in fp32 PyTorch.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ..utils.trace import trace_range
+from ._ext import error_word, ext
+
+HEAD_DIMS = (32, 64)
+MAX_CODE = 7
+
+
+class QuantizedKVCache:
+    """``rows`` histories of up to ``max_tokens`` tokens of ``kv_heads`` heads.
+
+    ``table [rows, ceil(max_tokens / page)]`` (int32) names the page of each run of
+    ``page`` positions; by default row ``r`` owns pages ``r * per_row ..``. A table with
+    fewer pages than that (``num_pages``) is the caller's to fill before it writes. A page
+    may be shared between rows that only read it."""
+
+    def __init__(self, rows: int, max_tokens: int, kv_heads: int, head_dim: int, page: int = 64,
+                 table: torch.Tensor | None = None, num_pages: int | None = None, device=None) -> None:
+        if rows < 1 or max_tokens < 1 or kv_heads < 1:
+            raise ValueError(f"key/value cache: rows {rows}, max_tokens {max_tokens} and kv_heads {kv_heads} must be "
+                             "positive")
+        if head_dim not in HEAD_DIMS:
+            raise NotImplementedError(f"key/value cache: head width {head_dim}, the cache takes {HEAD_DIMS}")
+        if page < 16 or page & (page - 1):
+            raise ValueError(f"key/value cache: page {page} must be a power of two of at least 16")
+        per_row = -(-max_tokens // page)
+        if per_row * page >= 2 ** 31:
+            raise ValueError(f"key/value cache: {max_tokens} tokens a row")
+        device = torch.device(device) if device is not None else torch.device("cpu")
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if num_pages is None:
+            num_pages = rows * per_row
+        if num_pages < 1:
+            raise ValueError(f"key/value cache: num_pages {num_pages}")
+        if table is None:
+            if num_pages < rows * per_row:
+                raise ValueError(f"key/value cache: {rows} rows of {per_row} pages need a table to share {num_pages}")
+            table = torch.arange(rows * per_row, dtype=torch.int32, device=device).view(rows, per_row)
+        else:
+            if table.shape != (rows, per_row):
+                raise ValueError(f"key/value cache: table {tuple(table.shape)}, expected {(rows, per_row)}")
+            if table.is_floating_point():
+                raise TypeError("key/value cache: the page table holds whole numbers")
+            table = table.to(device=device, dtype=torch.int32).contiguous()
+        self.rows, self.kv_heads, self.head_dim, self.page = rows, kv_heads, head_dim, page
+        self.num_pages, self.device = num_pages, device
+        self.table = table
+        self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.codes = torch.empty(num_pages, kv_heads, 2, page, head_dim // 2, dtype=torch.uint8, device=device)
+        self.scales = torch.empty(num_pages, kv_heads, 2, page, dtype=torch.bfloat16, device=device)
+
+    @property
+    def capacity(self) -> int:
+        """Positions a row can hold."""
+
+        return self.table.shape[1] * self.page
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + 2 * self.scales.numel()
+
+    def reset(self, rows: torch.Tensor | None = None) -> None:
+        """Empties the cache, or only ``rows``."""
+
+        if rows is None:
+            self.lengths.zero_()
+        else:
+            self.lengths[rows.long()] = 0
+
+    # ------------------------------------------------------------------ definition in PyTorch
+    def _slots(self, rows: torch.Tensor, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Page and slot of positions ``pos`` of ``rows`` (broadcast together)."""
+
+        pg = self.table[rows, pos // self.page].long()
+        if bool(((pg < 0) | (pg >= self.num_pages)).any()):
+            raise ValueError("key/value cache: page outside the cache")
+        return pg, pos % self.page
+
+    def values(self, rows: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+        """fp32 ``[..., kv_heads, 2, head_dim]`` at ``pos`` of ``rows``."""
+
+        pg, slot = self._slots(rows, pos)
+        n = self.codes[pg, :, :, slot]
+        c = torch.stack([n & 15, n >> 4], -1).flatten(-2).float() - 8.0
+        return c * self.scales[pg, :, :, slot].float().unsqueeze(-1)
+
+
+# ----------------------------------------------------------------------------- checks
+def _index(t: torch.Tensor | None, n: int, cache: QuantizedKVCache, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32:
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
+        t = t.to(torch.int32)
+    if t.shape != (n,):
+        raise ValueError(f"{name} {tuple(t.shape)}, expected ({n},)")
+    if t.device != cache.device:
+        raise ValueError(f"{name} on {t.device}, the cache on {cache.device}")
+    return t.contiguous()
+
+
+def _tokens(t: torch.Tensor, width: int, cache: QuantizedKVCache, name: str) -> torch.Tensor:
+    """``[n, T, width]`` with a dense last dimension, 16-byte aligned rows on CUDA."""
+
+    if t.dim() != 3 or t.shape[2] != width:
+        raise ValueError(f"{name} {tuple(t.shape)}, expected [rows, tokens, {width}]")
+    if t.device != cache.device:
+        raise ValueError(f"{name} on {t.device}, the cache on {cache.device}")
+    if t.device.type == "cuda":
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bf16, not {t.dtype}")
+        s0, s1, s2 = t.stride()
+        if s2 != 1 or s1 % 8 or s0 % 8 or s1 < 0 or s0 < 0 or t.data_ptr() % 16:
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+    elif not t.is_floating_point():
+        raise TypeError(f"{name} must be a floating type, not {t.dtype}")
+    return t
+
+
+def _no_grad(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the key/value cache has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+# ----------------------------------------------------------------------------- write
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes ``-7 .. 7`` (int8) and bf16 scales of the rows (last dimension) of ``x``."""
+
+    x = x.float()
+    top = x.abs().amax(-1)
+    finite = torch.isfinite(top)
+    s = torch.where(finite, top / float(MAX_CODE), torch.nan).to(torch.bfloat16)
+    sf = s.float().unsqueeze(-1)
+    ok = finite.unsqueeze(-1) & (sf > 0)
+    c = torch.where(ok, torch.round(x / torch.where(ok, sf, torch.ones_like(sf))), torch.zeros_like(x))
+    return c.clamp(-MAX_CODE, MAX_CODE).to(torch.int8), s
+
+
+def kv_cache_write_reference(cache: QuantizedKVCache, k, v, start=None, kstart=None, rows=None) -> None:
+    """PyTorch definition of ``kv_cache_write``."""
+
+    n, T, _ = k.shape
+    dev = cache.device
+    r = (torch.arange(n, device=dev) if rows is None else rows.long())
+    first = (torch.zeros(n, device=dev, dtype=torch.long) if kstart is None else kstart.long().clamp(0, T))
+    begin = cache.lengths[r].long() if start is None else start.long()
+    if bool(((begin < 0) | (begin > cache.capacity)).any()):
+        raise ValueError("key/value cache: start outside the row")
+    x = torch.stack([k, v], 2).view(n, T, 2, cache.kv_heads, cache.head_dim).to(torch.bfloat16)
+    c, s = quantize_rows(x)
+    u = (c + 8).to(torch.uint8)
+    packed = (u[..., 0::2] | (u[..., 1::2] << 4)).transpose(2, 3)
+    t = torch.arange(T, device=dev)
+    pos = begin.view(-1, 1) + t - first.view(-1, 1)
+    live = t >= first.view(-1, 1)
+    if bool((live & (pos >= cache.capacity)).any()):
+        raise ValueError("key/value cache: a row is full")
+    i, ti = live.nonzero(as_tuple=True)
+    pg, slot = cache._slots(r[i], pos[i, ti])
+    cache.codes[pg, :, :, slot] = packed[i, ti]
+    cache.scales[pg, :, :, slot] = s.transpose(2, 3)[i, ti]
+    cache.lengths[r] = (begin + T - first).to(torch.int32)
+
+
+def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor | None = None,
+                   kstart: torch.Tensor | None = None, rows: torch.Tensor | None = None) -> None:
+    """Quantises ``k, v [n, T, kv_heads * head_dim]`` into cache rows ``rows [n]`` (distinct;
+    default all rows in order). Source row ``i``'s tokens ``kstart[i] ..`` (default 0: none is
+    padding) go to positions ``start[i] ..`` (default: append), and the row's length becomes
+    the end of what was written."""
+
+    with trace_range("mdl.kv_cache.write"):
+        width = cache.kv_heads * cache.head_dim
+        _no_grad(k, v)
+        k, v = _tokens(k, width, cache, "k"), _tokens(v, width, cache, "v")
+        n = k.shape[0]
+        if v.shape != k.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        if rows is None and n != cache.rows:
+            raise ValueError(f"{n} source rows for {cache.rows} cache rows: give rows")
+        rows = _index(rows, n, cache, "rows")
+        kstart = _index(kstart, n, cache, "kstart")
+        start = _index(start, n, cache, "start")
+        if cache.device.type != "cuda":
+            kv_cache_write_reference(cache, k, v, start, kstart, rows)
+            return
+        if start is not None and start.untyped_storage().data_ptr() == cache.lengths.untyped_storage().data_ptr():
+            start = start.clone()  # the kernel writes the lengths
+        ext().kv_write(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), k, v, rows,
+                       start, kstart)
+
+
+# ----------------------------------------------------------------------------- read
+def kv_cache_read(cache: QuantizedKVCache, count: int, start: torch.Tensor | None = None,
+                  rows: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(k, v)``, each ``[n, count, kv_heads * head_dim]``: the values at positions ``start[i]
+    .. start[i] + count`` (default from 0) of rows ``rows [n]`` (default all); zero past a row's
+    length. fp32 holds them exactly; bf16 rounds once."""
+
+    with trace_range("mdl.kv_cache.read"):
+        if count < 0:
+            raise ValueError(f"count {count}")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"the cache reads back bf16 or fp32, not {dtype}")
+        n = cache.rows if rows is None else rows.shape[0]
+        rows = _index(rows, n, cache, "rows")
+        start = _index(start, n, cache, "start")
+        width = cache.kv_heads * cache.head_dim
+        if cache.device.type != "cuda":
+            r = (torch.arange(n) if rows is None else rows.long()).view(-1, 1)
+            pos = (0 if start is None else start.long().view(-1, 1)) + torch.arange(count)
+            if bool((pos < 0).any()):
+                raise ValueError("key/value cache: start outside the row")
+            live = pos < cache.lengths[r].long()
+            x = torch.zeros(n, count, cache.kv_heads, 2, cache.head_dim)
+            i, ti = live.expand(n, count).nonzero(as_tuple=True)
+            x[i, ti] = cache.values(r.expand(n, count)[i, ti], pos.expand(n, count)[i, ti])
+            x = x.to(dtype)
+            return x[..., 0, :].reshape(n, count, width), x[..., 1, :].reshape(n, count, width)
+        k = torch.empty(n, count, width, dtype=dtype, device=cache.device)
+        v = torch.empty_like(k)
+        ext().kv_read(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), k, v, rows,
+                      start)
+        return k, v
+
+
+# ----------------------------------------------------------------------------- attend
+def cached_attention_reference(q, cache: QuantizedKVCache, rows=None, k_new=None, v_new=None, window: int = 0,
+                               sinks: int = 0, scale: float | None = None) -> torch.Tensor:
+    """fp32 PyTorch definition of ``cached_attention``."""
+
+    B, N, W = q.shape
+    G, hd = cache.kv_heads, cache.head_dim
+    H = W // hd
+    scale = scale if scale else 1.0 / math.sqrt(hd)
+    dev = q.device
+    r = (torch.arange(B, device=dev) if rows is None else rows.long())
+    ln = cache.lengths[r].long()
+    T = int(ln.max()) if B else 0
+    kpos = torch.arange(T, device=dev)
+    pos = torch.minimum(kpos.view(1, -1), (ln.view(-1, 1) - 1).clamp(min=0))
+    kv = cache.values(r.view(-1, 1).expand(B, T), pos) if T else torch.zeros(B, 0, G, 2, hd, device=dev)
+    kv = kv.permute(3, 0, 2, 1, 4).repeat_interleave(H // G, 2)                   # [2, B, H, T, hd]
+    n = torch.arange(N, device=dev)
+    ln = ln.view(-1, 1, 1)
+    qpos = (ln if k_new is not None else ln - N) + n.view(1, -1, 1)
+
+    def visible(at):
+        ok = at <= qpos
+        return ok & ((qpos - at < window) | (at < sinks)) if window else ok
+
+    allowed = (kpos < ln) & visible(kpos)
+    k, v = kv[0], kv[1]
+    if k_new is not None:
+        kn = k_new.float().view(B, N, G, hd).transpose(1, 2).repeat_interleave(H // G, 1)
+        vn = v_new.float().view(B, N, G, hd).transpose(1, 2).repeat_interleave(H // G, 1)
+        k, v = torch.cat([k, kn], 2), torch.cat([v, vn], 2)
+        allowed = torch.cat([allowed, visible(ln + n.view(1, 1, -1))], 2)
+    qh = q.float().view(B, N, H, hd).transpose(1, 2)
+    s = (qh @ k.transpose(-1, -2)) * scale
+    allowed = allowed.unsqueeze(1)
+    p = torch.softmax(s.masked_fill(~allowed, float("-inf")), -1)
+    p = torch.where(allowed, p, torch.zeros_like(p))                              # rows that see nothing
+    v = torch.where(allowed.any(2).unsqueeze(-1), v, torch.zeros_like(v))         # keys that nobody sees
+    return (p @ v).transpose(1, 2).reshape(B, N, W)
+
+
+def cached_attention(q: torch.Tensor, cache: QuantizedKVCache, rows: torch.Tensor | None = None,
+                     k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None, window: int = 0,
+                     sinks: int = 0, scale: float | None = None) -> torch.Tensor:
+    """``q [B, N, heads * head_dim]`` over cache row ``rows[b]`` (default row ``b``) ->
+    ``[B, N, heads * head_dim]``.
+
+    Query ``n`` of batch row ``b`` sits at position ``length - N + n`` (its token is in the
+    cache), or, with fresh keys ``k_new, v_new [B, N, kv_heads * head_dim]`` that are not in the
+    cache, at ``length + n``. It sees the positions up to its own: all of them (``window`` 0),
+    or the last ``window`` and the first ``sinks``; a query that sees none gives zero. Heads
+    ``g * heads / kv_heads ..`` share key head ``g``. ``scale`` defaults to ``head_dim ** -0.5``."""
+
+    with trace_range("mdl.attention.cached"):
+        G, hd = cache.kv_heads, cache.head_dim
+        if q.dim() != 3 or q.shape[2] % (G * hd) or q.shape[2] == 0:
+            raise ValueError(f"q {tuple(q.shape)}: the width must be a multiple of {G} key heads of {hd}")
+        _no_grad(q, k_new, v_new)
+        if window < 0 or sinks < 0:
+            raise ValueError(f"window {window} and sinks {sinks} must not be negative")
+        if (k_new is None) != (v_new is None):
+            raise ValueError("k_new and v_new come together")
+        B, N, width = q.shape
+        q = _tokens(q, width, cache, "q")
+        if rows is None and B != cache.rows:
+            raise ValueError(f"{B} batch rows for {cache.rows} cache rows: give rows")
+        rows = _index(rows, B, cache, "rows")
+        if k_new is not None:
+            k_new, v_new = _tokens(k_new, G * hd, cache, "k_new"), _tokens(v_new, G * hd, cache, "v_new")
+            if k_new.shape[:2] != (B, N) or v_new.shape[:2] != (B, N):
+                raise ValueError(f"k_new {tuple(k_new.shape)} and v_new {tuple(v_new.shape)} for {B} x {N} queries")
+        if cache.device.type != "cuda":
+            return cached_attention_reference(q, cache, rows, k_new, v_new, window, sinks, scale).to(q.dtype)
+        out = torch.empty(B, N, width, dtype=torch.bfloat16, device=q.device)
+        ext().kv_attend(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), q, k_new,
+                        v_new, rows, out, int(window), int(sinks), float(scale) if scale else 1.0 / math.sqrt(hd))
+        return out
