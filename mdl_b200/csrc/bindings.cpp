@@ -1091,6 +1091,73 @@ void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tens
   g_launches += launches;
 }
 
+// ------------------------------------------------------------------ windowed attention
+mdl::WindowAttnArgs window_args(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out,
+                                const at::Tensor& lse, int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks,
+                                double scale, const at::Tensor& err) {
+  require_cuda(qkv, "qkv");
+  const at::Device dev = qkv.device();
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 3 && qkv.stride(2) == 1 && qkv.stride(1) % 8 == 0 &&
+                  qkv.stride(0) % 8 == 0 && H > 0 && G > 0 && H % G == 0 && qkv.size(2) % (H + 2 * G) == 0,
+              "qkv must be bf16 [B, Lk, (H + 2 G) * hd] with 16-byte aligned rows");
+  TORCH_CHECK(kstart.device() == dev && kstart.scalar_type() == at::kInt && kstart.is_contiguous() &&
+                  kstart.numel() == qkv.size(0), "kstart must be int32 [B]");
+  mdl::WindowAttnArgs a;
+  const int64_t B = qkv.size(0), Lk = qkv.size(1), hd = qkv.size(2) / (H + 2 * G);
+  TORCH_CHECK(B > 0 && B < (int64_t{1} << 30) && Lk < (int64_t{1} << 30) && Lq > 0 && Lq <= Lk && window > 0 &&
+                  sinks >= 0, "windowed attention: sizes");
+  TORCH_CHECK(out.device() == dev && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
+                  out.numel() == B * Lq * H * hd, "out must be contiguous bf16 [B, Lq, H * hd]");
+  TORCH_CHECK(lse.device() == dev && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == B * H * Lq, "lse must be fp32 [B, H, Lq]");
+  TORCH_CHECK(err.device() == dev && err.scalar_type() == at::kInt, "err must be int32");
+  a.qkv = qkv.data_ptr();
+  // strides of dimensions of one entry are anything; the tensor map wants real ones
+  a.ld = Lk > 1 ? qkv.stride(1) : qkv.size(2);
+  a.sb = B > 1 ? qkv.stride(0) : a.ld * Lk;
+  a.kstart = kstart.data_ptr<int>();
+  a.out = out.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  a.B = static_cast<int>(B);
+  a.H = static_cast<int>(H);
+  a.G = static_cast<int>(G);
+  a.Lk = static_cast<int>(Lk);
+  a.Lq = static_cast<int>(Lq);
+  a.hd = static_cast<int>(hd);
+  a.window = static_cast<int>(std::min<int64_t>(window, Lk));
+  a.sinks = static_cast<int>(std::min<int64_t>(sinks, Lk));
+  a.scale = scale > 0 ? static_cast<float>(scale) : 1.f / std::sqrt(static_cast<float>(hd));
+  a.err = err.data_ptr<int>();
+  return a;
+}
+
+void window_attn_fwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
+                     int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale,
+                     const at::Tensor& err) {
+  c10::cuda::CUDAGuard guard(qkv.device());
+  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err);
+  check(mdl::window_attn_fwd(a, stream_of(qkv)), "window_attn_fwd");
+  g_launches += 1;
+}
+
+void window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
+                     const at::Tensor& dout, const at::Tensor& dqkv, const at::Tensor& dsum, int64_t H, int64_t G,
+                     int64_t Lq, int64_t window, int64_t sinks, double scale, const at::Tensor& err) {
+  c10::cuda::CUDAGuard guard(qkv.device());
+  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err);
+  TORCH_CHECK(dout.device() == qkv.device() && dout.scalar_type() == at::kBFloat16 && dout.is_contiguous() &&
+                  dout.numel() == out.numel(), "dout must be contiguous bf16 like out");
+  TORCH_CHECK(dqkv.device() == qkv.device() && dqkv.scalar_type() == at::kBFloat16 && dqkv.is_contiguous() &&
+                  dqkv.sizes() == qkv.sizes(), "dqkv must be contiguous bf16 like qkv");
+  TORCH_CHECK(dsum.device() == qkv.device() && dsum.scalar_type() == at::kFloat && dsum.is_contiguous() &&
+                  dsum.numel() == lse.numel(), "dsum must be fp32 [B, H, Lq]");
+  a.dout = dout.data_ptr();
+  a.dqkv = dqkv.data_ptr();
+  a.dsum = dsum.data_ptr<float>();
+  check(mdl::window_attn_bwd(a, stream_of(qkv)), "window_attn_bwd");
+  g_launches += 2;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1156,6 +1223,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("Lq"), py::arg("causal"), py::arg("scale"), py::arg("err") = py::none(), py::arg("ktail") = 0,
         py::arg("kexcl") = 0);
   m.def("position_add", &position_add);
+  m.def("window_attn_fwd", &window_attn_fwd);
+  m.def("window_attn_bwd", &window_attn_bwd);
   m.def("kv_write", &kv_write);
   m.def("kv_read", &kv_read);
   m.def("kv_attend", &kv_attend);

@@ -11,3 +11,4 @@
 #include "misc.h"
 #include "norm.h"
 #include "sqa.h"
+#include "window_attn.h"
