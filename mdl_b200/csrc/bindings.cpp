@@ -1094,7 +1094,7 @@ void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tens
 // ------------------------------------------------------------------ windowed attention
 mdl::WindowAttnArgs window_args(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out,
                                 const at::Tensor& lse, int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks,
-                                double scale, const at::Tensor& err) {
+                                double scale, const at::Tensor& err, const std::optional<at::Tensor>& out_lo) {
   require_cuda(qkv, "qkv");
   const at::Device dev = qkv.device();
   TORCH_CHECK(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 3 && qkv.stride(2) == 1 && qkv.stride(1) % 8 == 0 &&
@@ -1117,6 +1117,11 @@ mdl::WindowAttnArgs window_args(const at::Tensor& qkv, const at::Tensor& kstart,
   a.sb = B > 1 ? qkv.stride(0) : a.ld * Lk;
   a.kstart = kstart.data_ptr<int>();
   a.out = out.data_ptr();
+  if (out_lo.has_value() && out_lo->defined()) {
+    TORCH_CHECK(out_lo->device() == dev && out_lo->scalar_type() == at::kBFloat16 && out_lo->is_contiguous() &&
+                    out_lo->numel() == out.numel(), "out_lo must be contiguous bf16 like out");
+    a.out_lo = out_lo->data_ptr();
+  }
   a.lse = lse.data_ptr<float>();
   a.B = static_cast<int>(B);
   a.H = static_cast<int>(H);
@@ -1133,18 +1138,19 @@ mdl::WindowAttnArgs window_args(const at::Tensor& qkv, const at::Tensor& kstart,
 
 void window_attn_fwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
                      int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale,
-                     const at::Tensor& err) {
+                     const at::Tensor& err, const std::optional<at::Tensor>& out_lo) {
   c10::cuda::CUDAGuard guard(qkv.device());
-  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err);
+  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err, out_lo);
   check(mdl::window_attn_fwd(a, stream_of(qkv)), "window_attn_fwd");
   g_launches += 1;
 }
 
 void window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
                      const at::Tensor& dout, const at::Tensor& dqkv, const at::Tensor& dsum, int64_t H, int64_t G,
-                     int64_t Lq, int64_t window, int64_t sinks, double scale, const at::Tensor& err) {
+                     int64_t Lq, int64_t window, int64_t sinks, double scale, const at::Tensor& err,
+                     const at::Tensor& out_lo) {
   c10::cuda::CUDAGuard guard(qkv.device());
-  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err);
+  auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err, out_lo);
   TORCH_CHECK(dout.device() == qkv.device() && dout.scalar_type() == at::kBFloat16 && dout.is_contiguous() &&
                   dout.numel() == out.numel(), "dout must be contiguous bf16 like out");
   TORCH_CHECK(dqkv.device() == qkv.device() && dqkv.scalar_type() == at::kBFloat16 && dqkv.is_contiguous() &&

@@ -34,6 +34,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "common.cuh"
@@ -47,23 +48,31 @@ constexpr int TILE_BYTES = TILE * 128;  // 128-byte rows: 64 columns, the head's
 constexpr int HALF_BYTES = HALF * 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
-constexpr int F_THREADS = 192, F_TMEM = 256;
-constexpr int F_SMEM = 1024 + 5 * TILE_BYTES + 256;
-constexpr int B_THREADS = 320, B_TMEM = 512;
+constexpr int F_THREADS = 320, F_TMEM = 256;
+constexpr int RECS = 4;                         // item records in flight
+constexpr int TAIL = 512;                       // barriers and item records
+// Q[2] | K[2] | V[2] | row maxima and sums of the column halves, [2][2][128] each | references [2][128]
+constexpr int F_SMEM = 1024 + 6 * TILE_BYTES + 10 * TILE * 4 + TAIL;
+constexpr int B_THREADS = 576, B_TMEM = 512;
 constexpr int B_STAGES = 4;
-// stationary pair [2] | streamed pair [4] | lse, D of the streamed rows [4][64] | barriers
-constexpr int B_SMEM = 1024 + 4 * TILE_BYTES + 2 * B_STAGES * HALF_BYTES + B_STAGES * 2 * HALF * 4 + 256;
-static_assert(2 * F_SMEM <= 227 * 1024 && B_SMEM <= 227 * 1024, "shared memory budget");
+// stationary pair [2] | queries stationary: O and its remainder [2] | streamed pair [4] |
+// lse, D of the streamed rows [4][64], or lse of the stationary rows [2][128] | barriers
+constexpr int b_smem(bool keys) {
+  return 1024 + (keys ? 4 : 8) * TILE_BYTES + 2 * B_STAGES * HALF_BYTES + B_STAGES * 2 * HALF * 4 + TAIL;
+}
+static_assert(2 * F_SMEM <= 227 * 1024 && b_smem(false) <= 227 * 1024, "shared memory budget");
 
 struct Params {
   __nv_bfloat16* out;
+  __nv_bfloat16* out_lo;
   float* lse;
   const int* kstart;
   const __nv_bfloat16* dout;
   __nv_bfloat16* dqkv;
   float* dsum;
   int B, H, G, Lk, Lq, hd, window, sinks;
-  int tiles;  // work items a (sample, head): query tiles or key tiles
+  int heads, tiles;  // work items = (head, sample, tile index): heads x B x tiles
+  int dh, db, di;    // gridDim.x items further on, in these digits
   float scale, scale2;
   int* err;
 };
@@ -115,6 +124,36 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -128,17 +167,89 @@ __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a,
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
-// K-major operand, 128-byte swizzle: 16-element K step ks inside the row.
-__device__ __forceinline__ uint64_t desc_k(uint32_t base, int ks) { return make_smem_desc(base + ks * 32, 16, 1024); }
-// MN-major operand (rows = K, 64 contiguous MN elements a 128-byte row): K step ks = 16 rows.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int ks) {
-  return make_smem_desc(base + ks * 2048, TILE_BYTES, 1024);
+// Operand descriptors are a base plus 16-byte units: 2 a K step (16 elements) of a K-major
+// operand, 128 a K step (16 rows of 128 bytes) of an MN-major one with 64 columns.
+__device__ __forceinline__ uint64_t desc_of(const void* base) { return make_smem_desc(smem_u32(base), 16, 1024); }
+__device__ __forceinline__ uint64_t desc_mn_of(const void* base) {
+  return make_smem_desc(smem_u32(base), TILE_BYTES, 1024);
+}
+constexpr uint32_t K_STEP = 2, MN_STEP = 128, TILE_UNITS = TILE_BYTES / 16, HALF_UNITS = HALF_BYTES / 16;
+
+// True on one lane of a converged warp, always the same one. The compiler knows that a single
+// lane runs what follows and keeps the operands of the tensor instructions in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
 }
 
-// A wait whose outcome is the same on every lane of the warp (.sync.aligned code follows).
+// Barrier of the two warps that hold the column halves of the same 32 rows.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// A wait of the whole warp, with one outcome for all lanes (.sync.aligned code follows). The
+// loop of a wait that is not over at once stays out of line: the issuing warp shares its
+// scheduler with the computing ones, so that each instruction between two issues counts.
+__device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  const uint64_t start = globaltimer_ns();
+  for (uint32_t spins = 1;; ++spins) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((spins & 255u) == 0) {
+      const bool late = globaltimer_ns() - start > kWaitLimitNs;
+      if (__any_sync(0xffffffffu, late || *abort_flag)) {
+        if (late) record_error(err, MDL_ERR_MBAR_TIMEOUT);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
-  const bool ok = mbar_wait(bar, parity, err, abort_flag);
-  return __all_sync(0xffffffffu, ok);
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return warp_wait_slow(bar, parity, err, abort_flag);
+}
+
+// Pairs of fp32: one instruction for two columns.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 pair_of(const uint32_t* r) { return {__uint_as_float(r[0]), __uint_as_float(r[1])}; }
+
+// 4-byte asynchronous copy into shared memory; zero when !real (the source is not read then).
+__device__ __forceinline__ void copy4(const void* dst, const float* src, bool real) {
+  const int n = real ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+// Arrives on `bar` (as one of its expected arrivals) once this thread's copies have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Bits [l, h] (inclusive, clipped) of 32-column word w.
@@ -148,96 +259,138 @@ __device__ __forceinline__ uint32_t range_bits(int l, int h, int w) {
   return (0xFFFFFFFFu >> (31 - b)) & (0xFFFFFFFFu << a);
 }
 
+// 128 rows as two boxes of 64 (one tensor map serves both tile heights).
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int b) {
+  tma_load_3d(dst, tm, bar, x, y, b);
+  tma_load_3d(dst + HALF_BYTES, tm, bar, x, y + HALF, b);
+}
+
 // One row of hd zeros (bf16).
 __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int hd) {
   for (int c = 0; c < hd / 8; ++c) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0, 0, 0, 0);
 }
 
 // ============================================================================ work items
-// Positions below are relative to the sample's first valid token.
-struct Item {
-  int b, h, i;      // sample, head (query head, or key head), index within the pair
-  int kst, len, qf; // first valid token, valid tokens, first query
-  int t;            // tile
-  int cs, k0, n;    // steps: cs from 0, then from k0 on; n in all (0: nothing to do)
+// FORWARD and QUERIES: query tiles, key steps of 128 or 64 rows; KEYS: key tiles, query steps
+// of 64 rows of each query head of the group. Positions are relative to the first valid token.
+enum class Kind { FORWARD, QUERIES, KEYS };
+
+struct alignas(16) Item {
+  int h, b, kst, n;    // head, sample, first valid token, steps (-1: no more items)
+  int t, cs, k0, qf;   // tile; steps: cs from 0, then from k0 on (KEYS: cs a head, from k0); first query
+  int len, pad[3];     // valid tokens
 };
 
-__device__ __forceinline__ Item item_base(const Params& p, int w, int heads) {
+// First row of step j (KEYS: of step s of a query head).
+template <Kind K>
+__device__ __forceinline__ int step_row(int j, int cs, int k0) {
+  constexpr int ROWS = K == Kind::FORWARD ? TILE : HALF;
+  if constexpr (K == Kind::KEYS) return ROWS * (k0 + j);
+  return ROWS * (j < cs ? j : k0 + j - cs);
+}
+
+// A block's items one after another (every gridDim.x-th). Only the loading warp walks them; it
+// hands the others a record an item in shared memory, so that they carry neither the walk nor
+// its registers (kept beside 64 scores a thread they spilled, and the spills set the pace).
+// kstart of the next item is loaded an item ahead, and the digits are carried along.
+template <Kind K>
+struct Walk {
   Item it;
-  it.h = w % heads;
-  const int rest = w / heads;
-  it.b = rest % p.B;
-  it.i = rest / p.B;
-  it.kst = min(max(p.kstart[it.b], 0), p.Lk);
-  it.len = p.Lk - it.kst;
-  it.qf = max(0, p.Lk - p.Lq - it.kst);
-  it.cs = it.k0 = it.n = 0;
-  return it;
-}
+  int i;                // index within the pair (head, sample)
+  int nh, nb, ni, nks;  // next item
 
-// Query tile i, counted from the last; key steps of `rows` rows.
-__device__ __forceinline__ Item query_item(const Params& p, int w, int rows) {
-  Item it = item_base(p, w, p.H);
-  it.t = (it.len + TILE - 1) / TILE - 1 - it.i;
-  if (it.t < 0 || TILE * (it.t + 1) <= it.qf) return it;
-  const int end = (min(TILE * (it.t + 1), it.len) + rows - 1) / rows;
-  it.k0 = max(0, max(TILE * it.t, it.qf) - p.window + 1) / rows;
-  it.cs = min((min(p.sinks, it.len) + rows - 1) / rows, it.k0);
-  it.n = it.cs + end - it.k0;
-  return it;
-}
-
-// Key tile i (the sinks' first: every query sees it); query steps of 64 rows, per query head
-// of the group.
-__device__ __forceinline__ Item key_item(const Params& p, int w) {
-  Item it = item_base(p, w, p.G);
-  it.t = it.i;
-  if (TILE * it.t >= it.len) return it;
-  const int qs = max(TILE * it.t, it.qf);
-  const int qe = TILE * it.t < p.sinks ? it.len : min(it.len, TILE * it.t + TILE - 1 + p.window);
-  it.k0 = qs / HALF;
-  it.cs = qe > qs ? (qe + HALF - 1) / HALF - it.k0 : 0;  // steps a query head
-  it.n = it.cs * (p.H / p.G);
-  return it;
-}
+  __device__ __forceinline__ explicit Walk(const Params& p) {
+    nh = blockIdx.x % p.heads;
+    const int rest = blockIdx.x / p.heads;
+    nb = rest % p.B;
+    ni = rest / p.B;
+    nks = ni < p.tiles ? __ldg(p.kstart + nb) : 0;
+  }
+  // To the next item, with work or without (then n is 0); false: none left.
+  __device__ __forceinline__ bool next(const Params& p) {
+    if (ni >= p.tiles) return false;
+    it.h = nh;
+    it.b = nb;
+    i = ni;
+    const int ks = __reduce_max_sync(0xffffffffu, nks);  // the warp runs as one: uniform registers
+    nh += p.dh;
+    int carry = nh >= p.heads ? 1 : 0;
+    nh -= carry ? p.heads : 0;
+    nb += p.db + carry;
+    carry = nb >= p.B ? 1 : 0;
+    nb -= carry ? p.B : 0;
+    ni += p.di + carry;
+    nks = ni < p.tiles ? __ldg(p.kstart + nb) : 0;
+    it.kst = min(max(ks, 0), p.Lk);
+    it.len = p.Lk - it.kst;
+    it.qf = max(0, p.Lk - p.Lq - it.kst);
+    it.n = it.cs = it.k0 = 0;
+    if constexpr (K == Kind::KEYS) {
+      // the sinks' tile comes first: every query sees it
+      it.t = i;
+      if (TILE * it.t >= it.len) return true;
+      const int qs = max(TILE * it.t, it.qf);
+      const int qe = TILE * it.t < p.sinks ? it.len : min(it.len, TILE * it.t + TILE - 1 + p.window);
+      it.k0 = qs / HALF;
+      it.cs = qe > qs ? (qe + HALF - 1) / HALF - it.k0 : 0;
+      it.n = it.cs * (p.H / p.G);
+    } else {
+      constexpr int ROWS = K == Kind::FORWARD ? TILE : HALF;
+      it.t = (it.len + TILE - 1) / TILE - 1 - i;  // the last tile first
+      if (it.t < 0 || TILE * (it.t + 1) <= it.qf) return true;
+      const int end = (min(TILE * (it.t + 1), it.len) + ROWS - 1) / ROWS;
+      it.k0 = max(0, max(TILE * it.t, it.qf) - p.window + 1) / ROWS;
+      it.cs = min((min(p.sinks, it.len) + ROWS - 1) / ROWS, it.k0);
+      it.n = it.cs + end - it.k0;
+    }
+    return true;
+  }
+};
 
 // ============================================================================ forward
 template <int HD>
 __global__ void __launch_bounds__(F_THREADS, 2)
     window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv,
-                      const Params p, int num_items) {
+                      const Params p) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* sQ = align1024(smem_raw);
-  uint8_t* sK = sQ + TILE_BYTES;      // [2]
+  uint8_t* sQ = align1024(smem_raw);  // [2]
+  uint8_t* sK = sQ + 2 * TILE_BYTES;  // [2]
   uint8_t* sV = sK + 2 * TILE_BYTES;  // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + 2 * TILE_BYTES);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;   // [2]
-  uint64_t* k_empty = bars + 4;  // [2]
-  uint64_t* v_full = bars + 6;   // [2]
-  uint64_t* v_empty = bars + 8;  // [2]
-  uint64_t* s_full = bars + 10;
-  uint64_t* s_empty = bars + 11;
-  uint64_t* p_full = bars + 12;
-  uint64_t* pv_done = bars + 13;
-  uint64_t* done = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  float* sMax = reinterpret_cast<float*>(sV + 2 * TILE_BYTES);  // [2 steps][2 halves][128]
+  float* sSum = sMax + 4 * TILE;                                // [2 items][2 halves][128]
+  float* sRef = sSum + 4 * TILE;                                // [2 items][128]
+  Item* recs = reinterpret_cast<Item*>(sRef + 2 * TILE);        // [RECS]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(recs + RECS);
+  uint64_t* q_full = bars;        // [2]
+  uint64_t* q_empty = bars + 2;   // [2]
+  uint64_t* kv_full = bars + 4;   // [2]
+  uint64_t* kv_empty = bars + 6;  // [2]
+  uint64_t* s_full = bars + 12;
+  uint64_t* s_empty = bars + 13;
+  uint64_t* p_full = bars + 14;
+  uint64_t* pv_done = bars + 15;
+  uint64_t* done = bars + 16;
+  uint64_t* rec_full = bars + 17;   // [RECS]
+  uint64_t* rec_empty = bars + 21;  // [RECS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(RECS * sizeof(Item) + 26 * 8 <= TAIL, "records and barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < RECS; ++s) {
+      mbar_init(&rec_full[s], 1);
+      mbar_init(&rec_empty[s], 9);  // the issuing warp and the softmax warps
     }
     mbar_init(s_full, 1);
-    mbar_init(s_empty, 4);
-    mbar_init(p_full, 4);
+    mbar_init(s_empty, 8);
+    mbar_init(p_full, 8);
     mbar_init(pv_done, 1);
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -252,150 +405,253 @@ __global__ void __launch_bounds__(F_THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tS = tmem, tP = tmem + 128, tO = tmem + 192;
-  auto tile_of = [](const Item& it, int j) { return j < it.cs ? j : it.k0 + j - it.cs; };
 
   if (warp == 0) {
+    // ------------------------------------------------------------ walk and load
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_kv);
-      const int q0 = p.Lk - p.Lq;
-      int items = 0, g = 0, k_issued = 0, v_issued = 0;
-      bool ok = true;
-      for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-        const Item it = query_item(p, w, TILE);
-        if (it.n == 0) continue;
-        const int kvh = it.h / (p.H / p.G);
-        if (items >= 1 && !mbar_wait(q_empty, (items - 1) & 1, p.err, abort_flag)) break;
-        mbar_arrive_expect_tx(q_full, TILE_BYTES);
-        tma_load_3d(sQ, &tm_q, q_full, it.h * HD, it.kst + TILE * it.t - q0, it.b);
-        ++items;
-        for (int j = 0; j < it.n; ++j, ++g) {
-          const int st = g & 1;
-          const int y = it.kst + TILE * tile_of(it, j);
-          if (g >= 2 && !mbar_wait(&k_empty[st], ((g >> 1) - 1) & 1, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&k_full[st], TILE_BYTES);
-          tma_load_3d(sK + st * TILE_BYTES, &tm_kv, &k_full[st], (p.H + kvh) * HD, y, it.b);
-          k_issued = g + 1;
-          if (g >= 2 && !mbar_wait(&v_empty[st], ((g >> 1) - 1) & 1, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&v_full[st], TILE_BYTES);
-          tma_load_3d(sV + st * TILE_BYTES, &tm_kv, &v_full[st], (p.H + p.G + kvh) * HD, y, it.b);
-          v_issued = g + 1;
-        }
-      }
-      // every copy into this CTA's smem has landed before the CTA may exit
-      if (items > 0) mbar_wait(q_full, (items - 1) & 1, nullptr, nullptr);
-      for (int j = max(0, k_issued - 2); j < k_issued; ++j) mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
-      for (int j = max(0, v_issued - 2); j < v_issued; ++j) mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
     }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc_bf16(TILE, TILE, false, false);
-      constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, 64, false, true);
-      const uint32_t q_base = smem_u32(sQ), k_base = smem_u32(sK), v_base = smem_u32(sV);
-      bool ok = true;
-      int items = 0, g0 = 0;
-      auto issue_s = [&](int g, bool last) -> bool {
-        if (!mbar_wait(&k_full[g & 1], (g >> 1) & 1, p.err, abort_flag) ||
-            (g > 0 && !mbar_wait(s_empty, (g - 1) & 1, p.err, abort_flag)))
-          return false;
-        tc_fence_after();
-        const uint32_t kb = k_base + (g & 1) * TILE_BYTES;
-        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS, desc_k(q_base, ks), desc_k(kb, ks), idesc_s, ks);
-        tc_commit(&k_empty[g & 1]);
-        tc_commit(s_full);
-        if (last) tc_commit(q_empty);
-        return true;
-      };
-      for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-        const Item it = query_item(p, w, TILE);
-        if (it.n == 0) continue;
-        if (!mbar_wait(q_full, items & 1, p.err, abort_flag) || !issue_s(g0, it.n == 1)) break;
-        ++items;
-        for (int j = 0; j < it.n; ++j) {
-          const int g = g0 + j;
-          if (j + 1 < it.n && !issue_s(g + 1, j + 2 == it.n)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(p_full, g & 1, p.err, abort_flag) ||
-              !mbar_wait(&v_full[g & 1], (g >> 1) & 1, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          for (int ks = 0; ks < 8; ++ks)
-            tc_mma_bf16_ts(tO, tP + ks * 8, desc_mn(v_base + (g & 1) * TILE_BYTES, ks), idesc_pv,
-                           (j > 0 || ks > 0) ? 1u : 0u);
-          tc_commit(pv_done);
-          tc_commit(&v_empty[g & 1]);
-        }
-        g0 += it.n;
+    const int q0 = p.Lk - p.Lq;
+    int items = 0, g = 0;
+    bool ok = true;
+    Walk<Kind::FORWARD> w(p);
+    while (ok && w.next(p)) {
+      const Item& it = w.it;
+      // queries before the first valid token (a share of them per item)
+      const int pad = min(p.Lq, it.kst - q0);
+      for (int q = w.i * 32 + lane; q < pad; q += p.tiles * 32) {
+        const long long row = static_cast<long long>(it.b) * p.Lq + q;
+        zero_row(p.out + (row * p.H + it.h) * HD, HD);
+        if (p.out_lo != nullptr) zero_row(p.out_lo + (row * p.H + it.h) * HD, HD);
+        p.lse[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + q] = CUDART_INF_F;
       }
-      // all MMAs have finished before TMEM is released
+      if (it.n == 0) continue;
+      const int slot = items % RECS, sq = items & 1;
+      // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
+      if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
+      if (lane == 0) {
+        recs[slot] = it;
+        mbar_arrive(&rec_full[slot]);
+      }
+      __syncwarp();
+      const int kvh = it.h / (p.H / p.G);
+      if (!warp_wait(&q_empty[sq], ((items >> 1) + 1) & 1, p.err, abort_flag)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&q_full[sq], TILE_BYTES);
+        load_tile(sQ + sq * TILE_BYTES, &tm_q, &q_full[sq], it.h * HD, it.kst + TILE * it.t - q0, it.b);
+      }
+      __syncwarp();
+      ++items;
+      for (int j = 0; j < it.n; ++j, ++g) {
+        const int st = g & 1, y = it.kst + step_row<Kind::FORWARD>(j, it.cs, it.k0);
+        if (!warp_wait(&kv_empty[st], ((g >> 1) + 1) & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&kv_full[st], 2 * TILE_BYTES);
+          load_tile(sK + st * TILE_BYTES, &tm_kv, &kv_full[st], (p.H + kvh) * HD, y, it.b);
+          load_tile(sV + st * TILE_BYTES, &tm_kv, &kv_full[st], (p.H + p.G + kvh) * HD, y, it.b);
+        }
+        __syncwarp();
+      }
+    }
+    const int slot = items % RECS;
+    if (ok && warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag) && lane == 0) {
+      recs[slot].n = -1;
+      mbar_arrive(&rec_full[slot]);
+    }
+    __syncwarp();
+    // every copy into this CTA's smem has landed before the CTA may exit
+    if (lane == 0) {
+      for (int j = max(0, items - 2); j < items; ++j) mbar_wait(&q_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
+      for (int j = max(0, g - 2); j < g; ++j) mbar_wait(&kv_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ issue
+    // The whole warp waits (uniform registers hold its counters and descriptors); lane 0
+    // issues. Scores run one step ahead of the products, across items.
+    constexpr uint32_t idesc_s = make_idesc_bf16(TILE, TILE, false, false);
+    constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, 64, false, true);
+    const uint64_t dQ = desc_of(sQ), dK = desc_of(sK), dV = desc_mn_of(sV);
+    int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the block
+    bool ok = true;
+    // steps of item `i`, -1 after the last
+    auto steps_of = [&](int i) -> int {
+      if (!warp_wait(&rec_full[i % RECS], (i / RECS) & 1, p.err, abort_flag)) {
+        ok = false;
+        return -1;
+      }
+      return __reduce_max_sync(0xffffffffu, recs[i % RECS].n);
+    };
+    auto issue_s = [&]() -> bool {
+      const int st = a_g & 1, sq = a_items & 1;
+      if ((a_j == 0 && !warp_wait(&q_full[sq], (a_items >> 1) & 1, p.err, abort_flag)) ||
+          !warp_wait(&kv_full[st], (a_g >> 1) & 1, p.err, abort_flag) ||
+          (a_g > 0 && !warp_wait(s_empty, (a_g - 1) & 1, p.err, abort_flag)))
+        return false;
+      tc_fence_after();
+      const uint64_t a = dQ + sq * TILE_UNITS, b = dK + st * TILE_UNITS;
+      const bool last = a_j + 1 == a_n;
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS, a + ks * K_STEP, b + ks * K_STEP, idesc_s, ks);
+        tc_commit(s_full);
+        if (last) tc_commit(&q_empty[sq]);
+      }
+      __syncwarp();
+      ++a_g;
+      ++a_j;
+      if (last) {
+        a_j = 0;
+        a_n = steps_of(++a_items);
+      }
+      return ok;
+    };
+    a_n = steps_of(0);
+    int n = a_n, g = 0;
+    if (ok && a_n > 0) ok = issue_s();
+    for (int items = 0; ok && n > 0; ++items) {
+      for (int j = 0; j < n; ++j, ++g) {
+        const int st = g & 1;
+        if ((a_n > 0 && !issue_s()) || !warp_wait(p_full, g & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t b = dV + st * TILE_UNITS;
+        const uint32_t acc = j > 0 ? 1u : 0u;
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            tc_mma_bf16_ts(tO, tP + ks * 8, b + ks * MN_STEP, idesc_pv, ks > 0 ? 1u : acc);
+          tc_commit(pv_done);
+          tc_commit(&kv_empty[st]);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      n = steps_of(items + 1);
+      if (elect_one()) mbar_arrive(&rec_empty[items % RECS]);
+      __syncwarp();
+    }
+    // all MMAs have finished before TMEM is released
+    if (elect_one()) {
       tc_commit(done);
       mbar_wait(done, 0, nullptr, nullptr);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
-    const int quarter = warp & 3;
+    // Two warps share 32 query rows, a half of the columns (of S and of O) each.
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
     const int r = quarter * 32 + lane;
-    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    constexpr int OC = HD / 2;
+    const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t tS_own = base + half * 64, tP_own = base + 128 + half * 32, tO_own = base + 192 + half * OC;
     bool ok = true;
-    int g0 = 0;
-    for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-      const Item it = query_item(p, w, TILE);
-      const long long orow0 = static_cast<long long>(it.b) * p.Lq;
-      float* lse = p.lse + (static_cast<long long>(it.b) * p.H + it.h) * p.Lq;
-      // queries before the first valid token (a share of them per item)
-      for (int q = it.i * TILE + r; q < min(p.Lq, it.kst - (p.Lk - p.Lq)); q += p.tiles * TILE) {
-        zero_row(p.out + (orow0 + q) * p.H * HD + it.h * HD, HD);
-        lse[q] = CUDART_INF_F;
+    int g = 0, items = 0;
+    // The output of item `items - 1`: written while the next item's first scores are
+    // exponentiated, when its last product has long finished.
+    auto write_out = [&]() {
+      const int k = items - 1, slot = k % RECS;
+      const Item& it = recs[slot];
+      const float l = sSum[((k & 1) * 2) * TILE + r] + sSum[((k & 1) * 2 + 1) * TILE + r];
+      const int qi = it.kst + TILE * it.t + r - (p.Lk - p.Lq);
+      const bool real = qi >= 0 && qi < p.Lq;
+      const long long row = static_cast<long long>(it.b) * p.Lq + qi;
+      const long long o = (row * p.H + it.h) * HD + half * OC;
+      if (real && half == 0)
+        p.lse[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + qi] = sRef[(k & 1) * TILE + r] + lg2(l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rec_empty[slot]);
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int c = 0; c < OC / 16; ++c) {
+        uint32_t ov[16];
+        tmem_ld16(tO_own + c * 16, ov);
+        tmem_wait_ld();
+        if (!real) continue;
+        uint32_t hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __uint_as_float(ov[2 * e]) * inv, y = __uint_as_float(ov[2 * e + 1]) * inv;
+          hi[e] = pack2(x, y);
+          ov[e] = pack2(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xFFFF0000u));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          reinterpret_cast<uint4*>(p.out + o + c * 16)[e] =
+              make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+          if (p.out_lo != nullptr)
+            reinterpret_cast<uint4*>(p.out_lo + o + c * 16)[e] =
+                make_uint4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
+        }
       }
-      if (it.n == 0) continue;
-      const int qp = TILE * it.t + r;
+    };
+    for (;; ++items) {
+      const int slot = items % RECS;
+      if (!warp_wait(&rec_full[slot], (items / RECS) & 1, p.err, abort_flag)) {
+        ok = false;
+        break;
+      }
+      const int n = recs[slot].n;
+      if (n < 0) break;
+      const int t = recs[slot].t, cs = recs[slot].cs, k0 = recs[slot].k0;
       float m = -CUDART_INF_F, l = 0.f;
-      for (int j = 0; j < it.n; ++j) {
-        const int g = g0 + j;
-        const int kt = tile_of(it, j);
+      for (int j = 0; j < n; ++j, ++g) {
         if (!warp_wait(s_full, g & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t sr[TILE];
+        uint32_t sr[64];
+        tmem_ld32(tS_own, sr);
+        tmem_ld32(tS_own + 32, sr + 32);
+        // Visible columns as two 32-column words: the diagonal, and what the window's lower edge
+        // cuts of tiles that are not all sinks. A word that is empty for the whole warp is not
+        // exponentiated; a full one needs no mask.
+        uint32_t vm[2] = {~0u, ~0u};
+        bool live[2] = {true, true}, part[2] = {false, false};
+        const int key0 = step_row<Kind::FORWARD>(j, cs, k0);
+        if (key0 == TILE * t || (TILE * t - key0 + TILE > p.window && key0 + TILE > p.sinks)) {
+          const int d = TILE * t + r - key0 - 64 * half;  // columns up to d are not in the future
+          const int lo = d - p.window + 1, sk = min(d, p.sinks - 1 - key0 - 64 * half);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + lane_off + c * 32, sr + c * 32);
+          for (int c = 0; c < 2; ++c) {
+            vm[c] = range_bits(lo, d, c) | range_bits(0, sk, c);
+            live[c] = __any_sync(0xffffffffu, vm[c] != 0u);
+            part[c] = __any_sync(0xffffffffu, vm[c] != ~0u);
+          }
+        }
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_empty);
-        // the diagonal, and what the window's lower edge cuts of tiles that are not all sinks
-        if (kt == it.t || (TILE * (it.t - kt) + TILE > p.window && TILE * (kt + 1) > p.sinks)) {
-          const int d = qp - TILE * kt;  // columns up to d are not in the future
-          const int lo = d - p.window + 1, sk = min(d, p.sinks - 1 - TILE * kt);
+        float mx = -CUDART_INF_F;
 #pragma unroll
-          for (int w4 = 0; w4 < 4; ++w4) {
-            const uint32_t vm = range_bits(lo, d, w4) | range_bits(0, sk, w4);
+        for (int c = 0; c < 2; ++c) {
+          if (!live[c]) continue;
+          if (part[c]) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!((vm >> c) & 1u)) sr[32 * w4 + c] = __float_as_uint(-CUDART_INF_F);
+            for (int k = 0; k < 32; ++k)
+              if (!((vm[c] >> k) & 1u)) sr[32 * c + k] = __float_as_uint(-CUDART_INF_F);
           }
+          float m4[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) m4[k] = __uint_as_float(sr[32 * c + k]);
+#pragma unroll
+          for (int k = 4; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(sr[32 * c + k]));
+          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
         }
-        float mx8[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = __uint_as_float(sr[k]);
-#pragma unroll
-        for (int c = 8; c < TILE; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], __uint_as_float(sr[c]));
-        const float mx = p.scale2 * fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                          fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-        const bool grow = mx > m + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
+        mx *= p.scale2;
+        float* row_max = sMax + (g & 1) * 2 * TILE;
+        row_max[half * TILE + r] = mx;
+        pair_sync(1 + quarter);
+        mx = fmaxf(mx, row_max[(half ^ 1) * TILE + r]);
+        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float m_new = fmaxf(m, mx);
           const float alpha = m_new == -CUDART_INF_F ? 1.f : ex2(m - m_new);
           m = m_new;
@@ -407,66 +663,58 @@ __global__ void __launch_bounds__(F_THREADS, 2)
             }
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t ov[32];
-              tmem_ld32(tO + lane_off + c * 32, ov);
+            for (int c = 0; c < OC / 8; ++c) {  // few registers at a time: the scores are held
+              uint32_t ov[8];
+              tmem_ld8(tO_own + c * 8, ov);
               tmem_wait_ld();
 #pragma unroll
-              for (int d = 0; d < 32; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha);
-              tmem_st32(tO + lane_off + c * 32, ov);
+              for (int d = 0; d < 8; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha);
+              tmem_st8(tO_own + c * 8, ov);
             }
           }
         }
-        const float m_use = m == -CUDART_INF_F ? 0.f : m;
-        float sum8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < TILE; c += 2) {
-          const float e0 = ex2(fmaf(__uint_as_float(sr[c]), p.scale2, -m_use));
-          const float e1 = ex2(fmaf(__uint_as_float(sr[c + 1]), p.scale2, -m_use));
-          sum8[c & 7] += e0;
-          sum8[(c + 1) & 7] += e1;
-          sr[c / 2] = pack2(e0, e1);
-        }
-        l += ((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7]));
         if (g > 0 && !warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {  // the last P was consumed
           ok = false;
           break;
         }
         tc_fence_after();
-        tmem_st32(tP + lane_off, sr);
-        tmem_st32(tP + lane_off + 32, sr + 32);
+        if (j == 0 && items > 0) write_out();
+        const float m_use = m == -CUDART_INF_F ? 0.f : m;
+        const F2 sc = {-p.scale2, -p.scale2}, mm = {m_use, m_use};
+        F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[16];
+          if (live[c]) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              const F2 x = fma2(pair_of(sr + 32 * c + k), sc, mm);  // m - score; the sign is free in ex2
+              const F2 e = {ex2(-x.x), ex2(-x.y)};
+              sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
+              pk[k / 2] = pack2(e.x, e.y);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[k] = 0u;
+          }
+          tmem_st16(tP_own + 16 * c, pk);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
       }
       if (!ok) break;
-      g0 += it.n;
-      if (!warp_wait(pv_done, (g0 - 1) & 1, p.err, abort_flag)) {
-        ok = false;
-        break;
-      }
+      // Read by the other half after the pair's next barrier, which it passes only once it has
+      // read the item's before: two buffers do.
+      sSum[((items & 1) * 2 + half) * TILE + r] = l;
+      if (half == 0) sRef[(items & 1) * TILE + r] = m;
+    }
+    if (ok && items > 0 && warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {
+      pair_sync(1 + quarter);
       tc_fence_after();
-      const int qi = it.kst + qp - (p.Lk - p.Lq);
-      const bool real = qi >= 0 && qi < p.Lq;
-      const float inv = 1.f / l;
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t ov[32];
-        tmem_ld32(tO + lane_off + c * 32, ov);
-        tmem_wait_ld();
-        if (real) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + (orow0 + qi) * p.H * HD + it.h * HD + c * 32);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dst[e] = make_uint4(pack2(__uint_as_float(ov[8 * e]) * inv, __uint_as_float(ov[8 * e + 1]) * inv),
-                                pack2(__uint_as_float(ov[8 * e + 2]) * inv, __uint_as_float(ov[8 * e + 3]) * inv),
-                                pack2(__uint_as_float(ov[8 * e + 4]) * inv, __uint_as_float(ov[8 * e + 5]) * inv),
-                                pack2(__uint_as_float(ov[8 * e + 6]) * inv, __uint_as_float(ov[8 * e + 7]) * inv));
-        }
-      }
-      tc_fence_before();
-      if (real) lse[qi] = m + lg2(l);
+      write_out();
     }
   }
   tc_fence_before();
@@ -481,48 +729,55 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 // KEYS: the stationary tile holds keys (dK, dV), else queries (dQ and D).
 template <int HD, bool KEYS>
 __global__ void __launch_bounds__(B_THREADS, 1)
-    window_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
-                      const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2,
-                      const Params p, int num_items) {
+    window_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv,
+                      const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_o,
+                      const __grid_constant__ CUtensorMap tm_olo, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint8_t* sA1 = smem;                                // [2]
   uint8_t* sA2 = sA1 + 2 * TILE_BYTES;                // [2]
-  uint8_t* sB1 = sA2 + 2 * TILE_BYTES;                // [4]
+  uint8_t* sO = sA2 + 2 * TILE_BYTES;                 // queries stationary: O | remainder, [2]
+  uint8_t* sB1 = sO + (KEYS ? 0 : 4) * TILE_BYTES;    // [4]
   uint8_t* sB2 = sB1 + B_STAGES * HALF_BYTES;         // [4]
-  float* sLse = reinterpret_cast<float*>(sB2 + B_STAGES * HALF_BYTES);  // [4][64]
+  float* sLse = reinterpret_cast<float*>(sB2 + B_STAGES * HALF_BYTES);  // [4][64], or [2][128]
   float* sD = sLse + B_STAGES * HALF;                                  // [4][64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + B_STAGES * HALF);
+  Item* recs = reinterpret_cast<Item*>(sD + B_STAGES * HALF);          // [RECS]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(recs + RECS);
   uint64_t* a_full = bars;        // [2]
   uint64_t* a_empty = bars + 2;   // [2]
   uint64_t* b_full = bars + 4;    // [4]
   uint64_t* b_empty = bars + 8;   // [4]
   uint64_t* s_full = bars + 12;   // [2]
-  uint64_t* s_empty = bars + 14;  // [2]
   uint64_t* p_full = bars + 16;   // [2]
   uint64_t* p_empty = bars + 18;  // [2]
   uint64_t* acc_full = bars + 20;
   uint64_t* acc_empty = bars + 21;
   uint64_t* done = bars + 22;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  uint64_t* rec_full = bars + 23;   // [RECS]
+  uint64_t* rec_empty = bars + 27;  // [RECS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(RECS * sizeof(Item) + 32 * 8 <= TAIL, "records and barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&a_full[s], 1);
-      mbar_init(&a_empty[s], 1);
+      mbar_init(&a_full[s], KEYS ? 1 : 33);   // TMA bytes (+ the 32 lanes that copy lse, D)
+      mbar_init(&a_empty[s], KEYS ? 1 : 17);  // the products (+ the warps that read O and dO)
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], 4);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[s], 8);
       mbar_init(&p_empty[s], 1);
     }
+    for (int s = 0; s < RECS; ++s) {
+      mbar_init(&rec_full[s], 1);
+      mbar_init(&rec_empty[s], 17);  // the issuing warp and the computing warps
+    }
     for (int s = 0; s < B_STAGES; ++s) {
-      mbar_init(&b_full[s], KEYS ? 33 : 1);  // TMA bytes (+ the 32 lanes that stage lse and D)
+      mbar_init(&b_full[s], KEYS ? 33 : 1);
       mbar_init(&b_empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
+    mbar_init(acc_empty, 16);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -539,287 +794,388 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   auto tS = [&](int s) { return tmem + s * 128; };
   auto tP = [&](int s) { return tmem + 256 + s * 64; };
   const uint32_t tAcc0 = tmem + 384, tAcc1 = tmem + 448;
-  const int group = p.H / p.G, q0 = p.Lk - p.Lq;
-  auto item_of = [&](int w) { return KEYS ? key_item(p, w) : query_item(p, w, HALF); };
-  // first row (relative) of step j, and the query head of it
-  auto step_row = [&](const Item& it, int j) {
-    return KEYS ? HALF * (it.k0 + j % it.cs) : HALF * (j < it.cs ? j : it.k0 + j - it.cs);
-  };
-  auto step_head = [&](const Item& it, int j) { return KEYS ? it.h * group + j / it.cs : it.h; };
+  constexpr Kind KIND = KEYS ? Kind::KEYS : Kind::QUERIES;
+  const int q0 = p.Lk - p.Lq;
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tm_a1);
-      tma_prefetch_desc(&tm_a2);
-      tma_prefetch_desc(&tm_b1);
-      tma_prefetch_desc(&tm_b2);
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_kv);
+      tma_prefetch_desc(&tm_do);
+      if (!KEYS) {
+        tma_prefetch_desc(&tm_o);
+        tma_prefetch_desc(&tm_olo);
+      }
     }
-    int items = 0, g = 0;
     bool ok = true;
-    for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-      const Item it = item_of(w);
-      if (it.n == 0) continue;
-      const int sa = items & 1;
+    Walk<KIND> w(p);
+    int items = 0, g = 0, a_issued = 0;
+    const int width = (p.H + 2 * p.G) * HD;
+    while (ok && w.next(p)) {
+      const Item& at = w.it;
+      const int sa = items & 1, ya = at.kst + TILE * at.t;
+      // gradients of what nobody sees or asks for: a share, per item, of the rows before the
+      // first valid token (queries: the first query), and valid keys without a query
+      const long long trow0 = static_cast<long long>(at.b) * p.Lk;
+      auto clear = [&](int row) {
+        __nv_bfloat16* dst = p.dqkv + (trow0 + row) * width + (KEYS ? p.H + at.h : at.h) * HD;
+        zero_row(dst, HD);
+        if (KEYS) zero_row(dst + p.G * HD, HD);
+      };
+      for (int k = w.i * 32 + lane; k < at.kst + (KEYS ? 0 : at.qf); k += p.tiles * 32) clear(k);
+      if (at.n == 0) {
+        if (KEYS)
+          for (int k = ya + lane; k < min(ya + TILE, p.Lk); k += 32) clear(k);
+        continue;
+      }
+      const int slot = items % RECS;
+      // parity of the previous use of this stage; a fresh barrier passes parity 1 at once
+      if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
+      if (lane == 0) {
+        recs[slot] = at;
+        mbar_arrive(&rec_full[slot]);
+      }
+      __syncwarp();
       if (!warp_wait(&a_empty[sa], ((items >> 1) + 1) & 1, p.err, abort_flag)) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&a_full[sa], 2 * TILE_BYTES);
-        const int y = it.kst + TILE * it.t;
+        mbar_arrive_expect_tx(&a_full[sa], (KEYS ? 2 : 4) * TILE_BYTES);
         if constexpr (KEYS) {
-          tma_load_3d(sA1 + sa * TILE_BYTES, &tm_a1, &a_full[sa], (p.H + it.h) * HD, y, it.b);
-          tma_load_3d(sA2 + sa * TILE_BYTES, &tm_a2, &a_full[sa], (p.H + p.G + it.h) * HD, y, it.b);
+          load_tile(sA1 + sa * TILE_BYTES, &tm_kv, &a_full[sa], (p.H + at.h) * HD, ya, at.b);
+          load_tile(sA2 + sa * TILE_BYTES, &tm_kv, &a_full[sa], (p.H + p.G + at.h) * HD, ya, at.b);
         } else {
-          tma_load_3d(sA1 + sa * TILE_BYTES, &tm_a1, &a_full[sa], it.h * HD, y - q0, it.b);
-          tma_load_3d(sA2 + sa * TILE_BYTES, &tm_a2, &a_full[sa], it.h * HD, y - q0, it.b);
+          load_tile(sA1 + sa * TILE_BYTES, &tm_q, &a_full[sa], at.h * HD, ya - q0, at.b);
+          load_tile(sA2 + sa * TILE_BYTES, &tm_do, &a_full[sa], at.h * HD, ya - q0, at.b);
+          load_tile(sO + sa * TILE_BYTES, &tm_o, &a_full[sa], at.h * HD, ya - q0, at.b);
+          load_tile(sO + (2 + sa) * TILE_BYTES, &tm_olo, &a_full[sa], at.h * HD, ya - q0, at.b);
         }
       }
-      ++items;
-      for (int j = 0; j < it.n; ++j, ++g) {
+      __syncwarp();
+      a_issued = ++items;
+      if constexpr (!KEYS) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = TILE * at.t + lane + 32 * e;
+          const bool real = c >= at.qf && c < at.len;
+          const long long off = (static_cast<long long>(at.b) * p.H + at.h) * p.Lq + (real ? at.kst + c - q0 : 0);
+          copy4(sLse + sa * TILE + lane + 32 * e, p.lse + off, real);
+        }
+        copies_arrive(&a_full[sa]);
+      }
+      int h = KEYS ? at.h * (p.H / p.G) : at.h;
+      for (int j = 0, s = 0; j < at.n; ++j, ++s, ++g) {
         const int st = g % B_STAGES;
-        // parity of the previous use of this stage; a fresh barrier passes parity 1 at once
         if (!warp_wait(&b_empty[st], (g / B_STAGES + 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
-        const int rel = step_row(it, j), y = it.kst + rel, h = step_head(it, j);
+        if (KEYS && s == at.cs) {  // the next query head of the group
+          s = 0;
+          ++h;
+        }
+        const int rel = step_row<KIND>(s, at.cs, at.k0), y = at.kst + rel;
         if (lane == 0) {
           mbar_arrive_expect_tx(&b_full[st], 2 * HALF_BYTES);
           if constexpr (KEYS) {
-            tma_load_3d(sB1 + st * HALF_BYTES, &tm_b1, &b_full[st], h * HD, y - q0, it.b);
-            tma_load_3d(sB2 + st * HALF_BYTES, &tm_b2, &b_full[st], h * HD, y - q0, it.b);
+            tma_load_3d(sB1 + st * HALF_BYTES, &tm_q, &b_full[st], h * HD, y - q0, at.b);
+            tma_load_3d(sB2 + st * HALF_BYTES, &tm_do, &b_full[st], h * HD, y - q0, at.b);
           } else {
-            const int kvh = h / group;
-            tma_load_3d(sB1 + st * HALF_BYTES, &tm_b1, &b_full[st], (p.H + kvh) * HD, y, it.b);
-            tma_load_3d(sB2 + st * HALF_BYTES, &tm_b2, &b_full[st], (p.H + p.G + kvh) * HD, y, it.b);
+            const int kvh = h / (p.H / p.G);
+            tma_load_3d(sB1 + st * HALF_BYTES, &tm_kv, &b_full[st], (p.H + kvh) * HD, y, at.b);
+            tma_load_3d(sB2 + st * HALF_BYTES, &tm_kv, &b_full[st], (p.H + p.G + kvh) * HD, y, at.b);
           }
         }
-        if constexpr (KEYS) {
+        __syncwarp();
+        if constexpr (KEYS) {  // rows that are no queries get zeros and are never visible
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int c = lane + 32 * e;
-            const bool real = rel + c >= it.qf && rel + c < it.len;
-            const long long off = (static_cast<long long>(it.b) * p.H + h) * p.Lq + (y + c - q0);
-            sLse[st * HALF + c] = real ? p.lse[off] : CUDART_INF_F;
-            sD[st * HALF + c] = real ? p.dsum[off] : 0.f;
+            const bool real = rel + c >= at.qf && rel + c < at.len;
+            const long long off = (static_cast<long long>(at.b) * p.H + h) * p.Lq + (real ? y + c - q0 : 0);
+            copy4(sLse + st * HALF + c, p.lse + off, real);
+            copy4(sD + st * HALF + c, p.dsum + off, real);
           }
-          mbar_arrive(&b_full[st]);
+          copies_arrive(&b_full[st]);
         }
       }
     }
+    const int slot = items % RECS;
+    if (ok && warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag) && lane == 0) {
+      recs[slot].n = -1;
+      mbar_arrive(&rec_full[slot]);
+    }
+    __syncwarp();
     if (lane == 0) {
-      for (int j = max(0, items - 2); j < items; ++j) mbar_wait(&a_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
+      for (int j = max(0, a_issued - 2); j < a_issued; ++j) mbar_wait(&a_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
       for (int j = max(0, g - B_STAGES); j < g; ++j)
         mbar_wait(&b_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr, nullptr);
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = make_idesc_bf16(TILE, HALF, false, false);
-      constexpr uint32_t idesc_acc = make_idesc_bf16(TILE, 64, false, true);
-      int items = 0, g0 = 0;
-      bool ok = true;
-      for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-        const Item it = item_of(w);
-        if (it.n == 0) continue;
+    // see the forward's warp 1
+    constexpr uint32_t idesc_s = make_idesc_bf16(TILE, HALF, false, false);
+    constexpr uint32_t idesc_acc = make_idesc_bf16(TILE, 64, false, true);
+    const uint64_t dA1 = desc_of(sA1), dA2 = desc_of(sA2), dB1 = desc_of(sB1), dB2 = desc_of(sB2);
+    const uint64_t mB1 = desc_mn_of(sB1), mB2 = desc_mn_of(sB2);
+    int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the block
+    bool ok = true;
+    auto steps_of = [&](int i) -> int {
+      if (!warp_wait(&rec_full[i % RECS], (i / RECS) & 1, p.err, abort_flag)) {
+        ok = false;
+        return -1;
+      }
+      return __reduce_max_sync(0xffffffffu, recs[i % RECS].n);
+    };
+    // S and dP of the next step, up to two ahead (each warpgroup's columns, read before its P is
+    // there) and one item ahead (the stationary tiles are double-buffered and released by the
+    // item's last product)
+    auto issue_s = [&]() -> bool {
+      const int st = a_g % B_STAGES, s = a_g & 1, sa = a_items & 1;
+      if ((a_j == 0 && !warp_wait(&a_full[sa], (a_items >> 1) & 1, p.err, abort_flag)) ||
+          !warp_wait(&b_full[st], (a_g / B_STAGES) & 1, p.err, abort_flag))
+        return false;
+      tc_fence_after();
+      const uint64_t a1 = dA1 + sa * TILE_UNITS, a2 = dA2 + sa * TILE_UNITS;
+      const uint64_t b1 = dB1 + st * HALF_UNITS, b2 = dB2 + st * HALF_UNITS;
+      const uint32_t ts = tS(s);
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(ts, a1 + ks * K_STEP, b1 + ks * K_STEP, idesc_s, ks);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(ts + 64, a2 + ks * K_STEP, b2 + ks * K_STEP, idesc_s, ks);
+        tc_commit(&s_full[s]);
+      }
+      __syncwarp();
+      ++a_g;
+      if (++a_j == a_n) {
+        a_j = 0;
+        a_n = steps_of(++a_items);
+      }
+      return ok;
+    };
+    a_n = steps_of(0);
+    int n = a_n, g = 0;
+    for (int items = 0; ok && n > 0; ++items) {
+      for (int j = 0; j < n; ++j, ++g) {
+        const int st = g % B_STAGES, s = g & 1;
+        while (ok && a_n > 0 && a_g <= g + 1 && a_items <= items + 1) ok = issue_s();
+        if (!ok || !warp_wait(&p_full[s], (g >> 1) & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (a_n > 0 && a_g == g + 2 && a_items <= items + 1) ok = issue_s();
+        if (!ok || (j == 0 && items >= 1 && !warp_wait(acc_empty, (items - 1) & 1, p.err, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t b1 = mB1 + st * HALF_UNITS, b2 = mB2 + st * HALF_UNITS;
+        const uint32_t tp = tP(s), acc = j > 0 ? 1u : 0u;
         const int sa = items & 1;
-        const uint32_t a1 = smem_u32(sA1 + sa * TILE_BYTES), a2 = smem_u32(sA2 + sa * TILE_BYTES);
-        if (!mbar_wait(&a_full[sa], (items >> 1) & 1, p.err, abort_flag)) break;
-        auto issue_s = [&](int g) -> bool {
-          const int st = g % B_STAGES, s = g & 1;
-          if (!mbar_wait(&b_full[st], (g / B_STAGES) & 1, p.err, abort_flag) ||
-              (g >= 2 && !mbar_wait(&s_empty[s], ((g >> 1) - 1) & 1, p.err, abort_flag)))
-            return false;
-          tc_fence_after();
-          const uint32_t b1 = smem_u32(sB1 + st * HALF_BYTES), b2 = smem_u32(sB2 + st * HALF_BYTES);
-          for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS(s), desc_k(a1, ks), desc_k(b1, ks), idesc_s, ks);
-          for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS(s) + 64, desc_k(a2, ks), desc_k(b2, ks), idesc_s, ks);
-          tc_commit(&s_full[s]);
-          return true;
-        };
-        if (!issue_s(g0) || (it.n > 1 && !issue_s(g0 + 1))) break;
-        for (int j = 0; j < it.n; ++j) {
-          const int g = g0 + j, st = g % B_STAGES, s = g & 1;
-          // S of two steps ahead goes to the columns that this step's warpgroup has emptied
-          if (j + 2 < it.n && !issue_s(g + 2)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(&p_full[s], (g >> 1) & 1, p.err, abort_flag) ||
-              (j == 0 && items >= 1 && !mbar_wait(acc_empty, (items - 1) & 1, p.err, abort_flag))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t b1 = smem_u32(sB1 + st * HALF_BYTES), b2 = smem_u32(sB2 + st * HALF_BYTES);
+        const bool last = j + 1 == n;
+        if (elect_one()) {
+#pragma unroll
           for (int ks = 0; ks < HALF / 16; ++ks) {
-            const uint32_t acc = (j > 0 || ks > 0) ? 1u : 0u;
-            if constexpr (KEYS) tc_mma_bf16_ts(tAcc0, tP(s) + ks * 8, desc_mn(b2, ks), idesc_acc, acc);
-            tc_mma_bf16_ts(tAcc1, tP(s) + 32 + ks * 8, desc_mn(b1, ks), idesc_acc, acc);
+            if constexpr (KEYS) tc_mma_bf16_ts(tAcc0, tp + ks * 8, b2 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
+            tc_mma_bf16_ts(tAcc1, tp + 32 + ks * 8, b1 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
           }
           tc_commit(&p_empty[s]);
           tc_commit(&b_empty[st]);
+          if (last) {
+            tc_commit(acc_full);
+            tc_commit(&a_empty[sa]);
+          }
         }
-        if (!ok) break;
-        tc_commit(acc_full);
-        tc_commit(&a_empty[sa]);
-        g0 += it.n;
-        ++items;
+        __syncwarp();
       }
+      if (!ok) break;
+      n = steps_of(items + 1);
+      if (elect_one()) mbar_arrive(&rec_empty[items % RECS]);
+      __syncwarp();
+    }
+    if (elect_one()) {
       tc_commit(done);
       mbar_wait(done, 0, nullptr, nullptr);
     }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ compute
-    const int wg = (warp - 2) >> 2;  // takes the steps of its parity
+    const int wg = ((warp - 2) >> 2) & 1;  // takes the steps of its parity,
+    const int half = (warp - 2) >> 3;      // this half of their columns
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const int width = (p.H + 2 * p.G) * HD;
     bool ok = true;
-    int items = 0, g0 = 0;
-    for (int w = blockIdx.x; w < num_items && ok; w += gridDim.x) {
-      const Item it = item_of(w);
-      const long long trow0 = static_cast<long long>(it.b) * p.Lk;
-      // gradients of what nobody sees or asks for (a share per item)
-      if constexpr (KEYS) {
-        for (int k = it.i * TILE + r; k < it.kst; k += p.tiles * TILE)
-          zero_row(p.dqkv + (trow0 + k) * width + (wg == 0 ? p.H + p.G + it.h : p.H + it.h) * HD, HD);
-      } else if (wg == 0) {
-        for (int k = it.i * TILE + r; k < it.kst + it.qf; k += p.tiles * TILE)
-          zero_row(p.dqkv + (trow0 + k) * width + it.h * HD, HD);
+    int items = 0, g = 0;
+    // keys: dV by warpgroup 0, dK by warpgroup 1, half of the columns a warp; queries: a quarter
+    // of dQ each
+    constexpr int COLS = KEYS ? HD / 2 : HD / 4;
+    const int col0 = KEYS ? half * COLS : (2 * wg + half) * COLS;
+    // Gradients of item k: written while its successor's first step is under way.
+    bool pending = false;
+    auto write_grad = [&](int k) -> bool {
+      if (!warp_wait(acc_full, k & 1, p.err, abort_flag)) return false;
+      tc_fence_after();
+      const uint32_t src = (KEYS && wg == 0 ? tAcc0 : tAcc1) + lane_off + col0;
+      uint32_t gr[COLS < 16 ? 16 : COLS];  // eight columns of 32-wide heads: read with eight more
+#pragma unroll
+      for (int c = 0; c < (COLS + 15) / 16; ++c) tmem_ld16(src + c * 16, gr + c * 16);
+      const Item& it = recs[k % RECS];
+      const int own = TILE * it.t + r;
+      const bool store = own < it.len && (KEYS || own >= it.qf);
+      const int head = KEYS ? (wg == 0 ? p.H + p.G + it.h : p.H + it.h) : it.h;
+      __nv_bfloat16* dst = p.dqkv + (static_cast<long long>(it.b) * p.Lk + it.kst + own) * (p.H + 2 * p.G) * HD +
+                           head * HD + col0;
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(acc_empty);
+        mbar_arrive(&rec_empty[k % RECS]);
       }
-      const int own = TILE * it.t + r;  // this thread's row
-      if (it.n == 0) {
-        if constexpr (KEYS) {  // valid keys without a query
-          if (own < it.len)
-            zero_row(p.dqkv + (trow0 + it.kst + own) * width + (wg == 0 ? p.H + p.G + it.h : p.H + it.h) * HD, HD);
+      const float f = (KEYS && wg == 0) ? 1.f : p.scale;
+      if (store) {
+#pragma unroll
+        for (int e = 0; e < COLS / 8; ++e) {
+          uint32_t y[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            y[c] = pack2(__uint_as_float(gr[8 * e + 2 * c]) * f, __uint_as_float(gr[8 * e + 2 * c + 1]) * f);
+          reinterpret_cast<uint4*>(dst)[e] = make_uint4(y[0], y[1], y[2], y[3]);
         }
-        continue;
       }
-      float row_lse = CUDART_INF_F, row_d = 0.f;
+      pending = false;
+      return true;
+    };
+    for (;; ++items) {
+      const int slot = items % RECS;
+      if (!warp_wait(&rec_full[slot], (items / RECS) & 1, p.err, abort_flag)) {
+        ok = false;
+        break;
+      }
+      const Item& at = recs[slot];
+      const int n = at.n;
+      if (n < 0) break;
+      const int cs = at.cs, k0 = at.k0, own = TILE * at.t + r;
+      float row_lse = 0.f, row_d = 0.f;
       if constexpr (!KEYS) {
-        const int qi = it.kst + own - q0;
-        if (own >= it.qf && own < it.len) {
-          const long long o = (static_cast<long long>(it.b) * p.Lq + qi) * p.H * HD + it.h * HD;
-          float acc = 0.f;
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            const uint4 ov = reinterpret_cast<const uint4*>(p.out + o)[c];
-            const uint4 gv = reinterpret_cast<const uint4*>(p.dout + o)[c];
-            const uint32_t a[4] = {ov.x, ov.y, ov.z, ov.w}, e[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              acc = fmaf(__uint_as_float(a[k] << 16), __uint_as_float(e[k] << 16), acc);
-              acc = fmaf(__uint_as_float(a[k] & 0xFFFF0000u), __uint_as_float(e[k] & 0xFFFF0000u), acc);
-            }
-          }
-          const long long s = (static_cast<long long>(it.b) * p.H + it.h) * p.Lq + qi;
-          row_d = acc;
-          row_lse = p.lse[s];
-          if (wg == 0) p.dsum[s] = acc;
+        const int sa = items & 1;
+        if (!warp_wait(&a_full[sa], (items >> 1) & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
         }
+        row_lse = sLse[sa * TILE + r];
+        const uint8_t* go = sA2 + sa * TILE_BYTES + r * 128;
+        const uint8_t* oh = sO + sa * TILE_BYTES + r * 128;
+        const uint8_t* ol = sO + (2 + sa) * TILE_BYTES + r * 128;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const int off = (c ^ (r & 7)) * 16;
+          const uint4 gv = *reinterpret_cast<const uint4*>(go + off);
+          const uint4 hv = *reinterpret_cast<const uint4*>(oh + off);
+          const uint4 lv = *reinterpret_cast<const uint4*>(ol + off);
+          const uint32_t e[4] = {gv.x, gv.y, gv.z, gv.w}, a[4] = {hv.x, hv.y, hv.z, hv.w},
+                         z[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            row_d = fmaf(__uint_as_float(a[k] << 16) + __uint_as_float(z[k] << 16), __uint_as_float(e[k] << 16), row_d);
+            row_d = fmaf(__uint_as_float(a[k] & 0xFFFF0000u) + __uint_as_float(z[k] & 0xFFFF0000u),
+                         __uint_as_float(e[k] & 0xFFFF0000u), row_d);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_empty[sa]);
+        if (wg == 0 && half == 0 && own >= at.qf && own < at.len)
+          p.dsum[(static_cast<long long>(at.b) * p.H + at.h) * p.Lq + at.kst + own - q0] = row_d;
       }
-      for (int j = 0; j < it.n; ++j) {
-        const int g = g0 + j;
+      for (int j = 0, s_ = 0; j < n; ++j, ++s_, ++g) {
+        if (KEYS && s_ == cs) s_ = 0;
         if ((g & 1) != wg) continue;
         const int st = g % B_STAGES;
-        const int rel = step_row(it, j);
+        const int rel = step_row<KIND>(s_, cs, k0);
         if ((KEYS && !warp_wait(&b_full[st], (g / B_STAGES) & 1, p.err, abort_flag)) ||
             !warp_wait(&s_full[wg], (g >> 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t s[64], dp[64];
-        tmem_ld32(tS(wg) + lane_off, s);
-        tmem_ld32(tS(wg) + lane_off + 32, s + 32);
-        tmem_ld32(tS(wg) + lane_off + 64, dp);
-        tmem_ld32(tS(wg) + lane_off + 96, dp + 32);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[wg]);
-        // visible columns of this row: one or two intervals
-        uint32_t vis[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+        uint32_t s[32], dp[32];
+        tmem_ld32(tS(wg) + lane_off + 32 * half, s);
+        tmem_ld32(tS(wg) + lane_off + 64 + 32 * half, dp);
+        // visible columns of this row (see the forward)
+        uint32_t vm = ~0u;
         if constexpr (KEYS) {
-          const bool whole = rel >= TILE * it.t + TILE - 1 && rel >= it.qf && rel + HALF <= it.len &&
-                             (TILE * (it.t + 1) <= p.sinks || rel + HALF - TILE * it.t <= p.window);
+          const bool whole = rel >= TILE * at.t + TILE - 1 && rel >= at.qf && rel + HALF <= at.len &&
+                             (TILE * (at.t + 1) <= p.sinks || rel + HALF - TILE * at.t <= p.window);
           if (!whole) {
-            const int lo = max(own, it.qf) - rel;
-            const int hi = (own < p.sinks ? it.len - 1 : min(it.len - 1, own + p.window - 1)) - rel;
-            vis[0] = range_bits(lo, hi, 0);
-            vis[1] = range_bits(lo, hi, 1);
+            const int lo = max(own, at.qf) - rel;
+            const int hi = (own < p.sinks ? at.len - 1 : min(at.len - 1, own + p.window - 1)) - rel;
+            vm = range_bits(lo, hi, half);
           }
         } else {
-          const bool whole = rel + HALF - 1 <= TILE * it.t &&
-                             (rel + HALF <= p.sinks || TILE * it.t + TILE - rel <= p.window);
+          const bool whole = rel + HALF - 1 <= TILE * at.t && TILE * at.t >= at.qf && TILE * (at.t + 1) <= at.len &&
+                             (rel + HALF <= p.sinks || TILE * at.t + TILE - rel <= p.window);
           if (!whole) {
-            const int d = own - rel;
-            const int lo = d - p.window + 1, sk = min(d, p.sinks - 1 - rel);
-            vis[0] = range_bits(lo, d, 0) | range_bits(0, sk, 0);
-            vis[1] = range_bits(lo, d, 1) | range_bits(0, sk, 1);
+            const bool real = own >= at.qf && own < at.len;
+            const int d = real ? own - rel : -1;
+            vm = range_bits(d - p.window + 1, d, half) | range_bits(0, min(d, p.sinks - 1 - rel), half);
           }
         }
-        const float* lse = sLse + st * HALF;
-        const float* dsv = sD + st * HALF;
-        // P and dS take the registers of S and dP: pair c of each in word c
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          float pv[2], ds[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float lc = KEYS ? lse[c + e] : row_lse;
-            const float dc = KEYS ? dsv[c + e] : row_d;
-            const float x = ex2(fmaf(__uint_as_float(s[c + e]), p.scale2, -lc));
-            const bool v = (vis[c >> 5] >> ((c + e) & 31)) & 1u;
-            pv[e] = v ? x : 0.f;
-            ds[e] = v ? x * (__uint_as_float(dp[c + e]) - dc) : 0.f;
-          }
-          if constexpr (KEYS) s[c / 2] = pack2(pv[0], pv[1]);
-          dp[c / 2] = pack2(ds[0], ds[1]);
-        }
-        if (g >= 2 && !warp_wait(&p_empty[wg], ((g >> 1) - 1) & 1, p.err, abort_flag)) {
+        const bool live = __any_sync(0xffffffffu, vm != 0u), part = __any_sync(0xffffffffu, vm != ~0u);
+        tmem_wait_ld();
+        const float4* lse4 = reinterpret_cast<const float4*>(sLse + st * HALF + 32 * half);
+        const float4* d4 = reinterpret_cast<const float4*>(sD + st * HALF + 32 * half);
+        const F2 sc = {-p.scale2, -p.scale2}, minus = {-1.f, -1.f};
+        if ((pending && !write_grad(items - 1)) ||
+            (g >= 2 && !warp_wait(&p_empty[wg], ((g >> 1) - 1) & 1, p.err, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if constexpr (KEYS) tmem_st32(tP(wg) + lane_off, s);
-        tmem_st32(tP(wg) + lane_off + 32, dp);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 16 columns at a time, stored as they are done: few registers
+          uint32_t pk[8], dk[8];
+          if (live) {
+#pragma unroll
+            for (int k = 16 * c; k < 16 * c + 16; k += 4) {
+              float4 lv = make_float4(row_lse, row_lse, row_lse, row_lse), dv = make_float4(row_d, row_d, row_d, row_d);
+              if constexpr (KEYS) {
+                lv = lse4[k / 4];
+                dv = d4[k / 4];
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const int i = k + e;
+                const F2 x = fma2(pair_of(s + i), sc, e == 0 ? F2{lv.x, lv.y} : F2{lv.z, lv.w});  // lse - score
+                F2 pr = {ex2(-x.x), ex2(-x.y)};
+                if (part) {
+                  if (!((vm >> i) & 1u)) pr.x = 0.f;
+                  if (!((vm >> (i + 1)) & 1u)) pr.y = 0.f;
+                }
+                const F2 ds = mul2(pr, fma2(e == 0 ? F2{dv.x, dv.y} : F2{dv.z, dv.w}, minus, pair_of(dp + i)));
+                if constexpr (KEYS) pk[(i - 16 * c) / 2] = pack2(pr.x, pr.y);
+                dk[(i - 16 * c) / 2] = pack2(ds.x, ds.y);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) pk[k] = dk[k] = 0u;
+          }
+          if constexpr (KEYS) tmem_st8(tP(wg) + lane_off + 16 * half + 8 * c, pk);
+          tmem_st8(tP(wg) + lane_off + 32 + 16 * half + 8 * c, dk);
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
       }
-      if (!ok) break;
-      g0 += it.n;
-      if (!warp_wait(acc_full, items & 1, p.err, abort_flag)) {
+      // a warpgroup without a step of this item still owes the last one's gradients
+      if (!ok || (pending && !write_grad(items - 1))) {
         ok = false;
         break;
       }
-      ++items;
-      tc_fence_after();
-      // keys: dV by warpgroup 0, dK by warpgroup 1; queries: half of dQ each
-      constexpr int COLS = KEYS ? HD : HD / 2;
-      uint32_t gr[64];
-      const uint32_t src = KEYS ? (wg == 0 ? tAcc0 : tAcc1) : tAcc1 + wg * COLS;
-#pragma unroll
-      for (int c = 0; c < (COLS + 31) / 32; ++c) tmem_ld32(src + lane_off + c * 32, gr + c * 32);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
-      const bool store = own < it.len && (KEYS || own >= it.qf);
-      if (store) {
-        const float f = (KEYS && wg == 0) ? 1.f : p.scale;
-        const int col = KEYS ? (wg == 0 ? p.H + p.G + it.h : p.H + it.h) * HD : it.h * HD + wg * COLS;
-        uint4* dst = reinterpret_cast<uint4*>(p.dqkv + (trow0 + it.kst + own) * width + col);
-#pragma unroll
-        for (int c = 0; c < COLS / 8; ++c) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(gr[8 * c + e]) * f;
-          dst[c] = make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
-        }
-      }
+      pending = true;
     }
+    if (ok && pending) write_grad(items - 1);
   }
   tc_fence_before();
   __syncthreads();
@@ -843,10 +1199,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [B, L, W] bf16, row stride ld and batch stride sb (elements); box 64 columns x `rows` rows,
+// [B, L, W] bf16, row stride ld and batch stride sb (elements); box 64 columns x 64 rows,
 // 128-byte swizzle. Rows and columns outside read as zeros.
-bool encode_rows(CUtensorMap* map, const void* base, uint64_t W, uint64_t L, uint64_t B, uint64_t ld, uint64_t sb,
-                 uint32_t rows) {
+bool encode_rows(CUtensorMap* map, const void* base, uint64_t W, uint64_t L, uint64_t B, uint64_t ld, uint64_t sb) {
   thread_local bool bound = false;
   if (!bound) {
     cudaFree(nullptr);  // makes the device's primary context current on this thread
@@ -856,16 +1211,18 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t W, uint64_t L, uin
   if (fn == nullptr) return false;
   cuuint64_t dims[3] = {W, L, B};
   cuuint64_t strides[2] = {ld * 2, sb * 2};
-  cuuint32_t box[3] = {64, rows, 1};
+  cuuint32_t box[3] = {64, HALF, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-Params make_params(const WindowAttnArgs& a, int tiles) {
+// `heads` x B x `tiles` items over a grid of `grid` blocks.
+Params make_params(const WindowAttnArgs& a, int heads, int tiles, int grid) {
   Params p;
   p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out_lo = static_cast<__nv_bfloat16*>(a.out_lo);
   p.lse = a.lse;
   p.kstart = a.kstart;
   p.dout = static_cast<const __nv_bfloat16*>(a.dout);
@@ -879,18 +1236,32 @@ Params make_params(const WindowAttnArgs& a, int tiles) {
   p.hd = a.hd;
   p.window = std::min(a.window, a.Lk);  // wider ones see the same
   p.sinks = std::min(a.sinks, a.Lk);
+  p.heads = heads;
   p.tiles = tiles;
+  p.dh = grid % heads;
+  p.db = grid / heads % a.B;
+  p.di = grid / heads / a.B;
   p.scale = a.scale;
   p.scale2 = a.scale * kLog2e;
   p.err = a.err;
   return p;
 }
 
-int num_sms() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
+constexpr int kMaxDevices = 64;
+
+int device_index() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
+int num_sms(int dev) {
+  static std::atomic<int> n[kMaxDevices];
+  int v = n[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
+    n[dev].store(v, std::memory_order_relaxed);
+  }
+  return v;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -902,58 +1273,62 @@ bool shapes_ok(const WindowAttnArgs& a) {
          a.sb > 0;
 }
 
-// Raised once a kernel and device; an error is returned, not kept.
+// Raises a kernel's shared memory limit, once a device (an error is returned, not kept).
 template <typename K>
-cudaError_t allow_smem(K kern, int bytes) {
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+cudaError_t allow_smem(K kern, int bytes, std::atomic<bool>* done) {
+  if (done->load(std::memory_order_relaxed)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done->store(true, std::memory_order_relaxed);
+  return e;
+}
+
+int grid_of(long long heads, long long samples, long long tiles, long long most) {
+  return static_cast<int>(std::min(heads * samples * tiles, most));
 }
 
 template <int HD>
 cudaError_t fwd_hd(const WindowAttnArgs& a, cudaStream_t stream) {
-  const Params p = make_params(a, (a.Lq + TILE - 1) / TILE + 1);
+  static std::atomic<bool> ready[kMaxDevices];
+  const int dev = device_index();
+  const int tiles = (a.Lq + TILE - 1) / TILE + 1;
+  const int grid = grid_of(a.H, a.B, tiles, 2LL * num_sms(dev));
+  const Params p = make_params(a, a.H, tiles, grid);
   const uint64_t W = static_cast<uint64_t>(a.H + 2 * a.G) * HD;
   const auto* base = static_cast<const __nv_bfloat16*>(a.qkv);
   CUtensorMap tq, tkv;
-  if (!encode_rows(&tq, base + (a.Lk - a.Lq) * a.ld, W, a.Lq, a.B, a.ld, a.sb, TILE) ||
-      !encode_rows(&tkv, base, W, a.Lk, a.B, a.ld, a.sb, TILE))
+  if (!encode_rows(&tq, base + (a.Lk - a.Lq) * a.ld, W, a.Lq, a.B, a.ld, a.sb) ||
+      !encode_rows(&tkv, base, W, a.Lk, a.B, a.ld, a.sb))
     return cudaErrorInvalidValue;
-  const cudaError_t e = allow_smem(window_fwd_kernel<HD>, F_SMEM);
+  const cudaError_t e = allow_smem(window_fwd_kernel<HD>, F_SMEM, &ready[dev]);
   if (e != cudaSuccess) return e;
-  const long long items = static_cast<long long>(a.H) * a.B * p.tiles;
-  if (items > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const int grid = static_cast<int>(std::min<long long>(items, 2LL * num_sms()));
-  window_fwd_kernel<HD><<<grid, F_THREADS, F_SMEM, stream>>>(tq, tkv, p, static_cast<int>(items));
+  window_fwd_kernel<HD><<<grid, F_THREADS, F_SMEM, stream>>>(tq, tkv, p);
   return cudaGetLastError();
 }
 
 template <int HD>
 cudaError_t bwd_hd(const WindowAttnArgs& a, cudaStream_t stream) {
+  static std::atomic<bool> ready_q[kMaxDevices], ready_k[kMaxDevices];
+  const int dev = device_index();
   const uint64_t W = static_cast<uint64_t>(a.H + 2 * a.G) * HD, D = static_cast<uint64_t>(a.H) * HD;
   const auto* base = static_cast<const __nv_bfloat16*>(a.qkv);
-  const auto* qbase = base + (a.Lk - a.Lq) * a.ld;
-  CUtensorMap q128, q64, kv128, kv64, do128, do64;
-  if (!encode_rows(&q128, qbase, W, a.Lq, a.B, a.ld, a.sb, TILE) ||
-      !encode_rows(&q64, qbase, W, a.Lq, a.B, a.ld, a.sb, HALF) ||
-      !encode_rows(&kv128, base, W, a.Lk, a.B, a.ld, a.sb, TILE) ||
-      !encode_rows(&kv64, base, W, a.Lk, a.B, a.ld, a.sb, HALF) ||
-      !encode_rows(&do128, a.dout, D, a.Lq, a.B, D, D * a.Lq, TILE) ||
-      !encode_rows(&do64, a.dout, D, a.Lq, a.B, D, D * a.Lq, HALF))
+  CUtensorMap tq, tkv, tdo, to, tlo;
+  if (!encode_rows(&tq, base + (a.Lk - a.Lq) * a.ld, W, a.Lq, a.B, a.ld, a.sb) ||
+      !encode_rows(&tkv, base, W, a.Lk, a.B, a.ld, a.sb) || !encode_rows(&tdo, a.dout, D, a.Lq, a.B, D, D * a.Lq) ||
+      !encode_rows(&to, a.out, D, a.Lq, a.B, D, D * a.Lq) || !encode_rows(&tlo, a.out_lo, D, a.Lq, a.B, D, D * a.Lq))
     return cudaErrorInvalidValue;
-  cudaError_t e = allow_smem(window_bwd_kernel<HD, false>, B_SMEM);
-  if (e == cudaSuccess) e = allow_smem(window_bwd_kernel<HD, true>, B_SMEM);
+  cudaError_t e = allow_smem(window_bwd_kernel<HD, false>, b_smem(false), &ready_q[dev]);
+  if (e == cudaSuccess) e = allow_smem(window_bwd_kernel<HD, true>, b_smem(true), &ready_k[dev]);
   if (e != cudaSuccess) return e;
-  const int sms = num_sms();
-  const Params pq = make_params(a, (a.Lq + TILE - 1) / TILE + 1);
-  const Params pk = make_params(a, (a.Lk + TILE - 1) / TILE);
-  const long long qi = static_cast<long long>(a.H) * a.B * pq.tiles, ki = static_cast<long long>(a.G) * a.B * pk.tiles;
-  if (qi > 0x7fffffffLL || ki > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int sms = num_sms(dev);
+  const int qtiles = (a.Lq + TILE - 1) / TILE + 1, ktiles = (a.Lk + TILE - 1) / TILE;
+  const int qgrid = grid_of(a.H, a.B, qtiles, sms), kgrid = grid_of(a.G, a.B, ktiles, sms);
   // queries first: they leave D behind
-  window_bwd_kernel<HD, false><<<static_cast<int>(std::min<long long>(qi, sms)), B_THREADS, B_SMEM, stream>>>(
-      q128, do128, kv64, kv64, pq, static_cast<int>(qi));
+  window_bwd_kernel<HD, false><<<qgrid, B_THREADS, b_smem(false), stream>>>(tq, tkv, tdo, to, tlo,
+                                                                           make_params(a, a.H, qtiles, qgrid));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  window_bwd_kernel<HD, true><<<static_cast<int>(std::min<long long>(ki, sms)), B_THREADS, B_SMEM, stream>>>(
-      kv128, kv128, q64, do64, pk, static_cast<int>(ki));
+  window_bwd_kernel<HD, true><<<kgrid, B_THREADS, b_smem(true), stream>>>(tq, tkv, tdo, to, tlo,
+                                                                         make_params(a, a.G, ktiles, kgrid));
   return cudaGetLastError();
 }
 
@@ -965,8 +1340,8 @@ cudaError_t window_attn_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
 }
 
 cudaError_t window_attn_bwd(const WindowAttnArgs& a, cudaStream_t stream) {
-  if (!shapes_ok(a) || a.dout == nullptr || a.dqkv == nullptr || a.dsum == nullptr || !aligned16(a.dout) ||
-      !aligned16(a.dqkv))
+  if (!shapes_ok(a) || a.dout == nullptr || a.dqkv == nullptr || a.dsum == nullptr || a.out_lo == nullptr ||
+      !aligned16(a.dout) || !aligned16(a.dqkv) || !aligned16(a.out_lo))
     return cudaErrorInvalidValue;
   return a.hd == 64 ? bwd_hd<64>(a, stream) : bwd_hd<32>(a, stream);
 }

@@ -11,6 +11,9 @@ namespace mdl {
 //   the queries are the last Lq tokens; with kst = kstart[b], token row p sees key j iff
 //   kst <= j <= p and (p - j < window or j - kst < sinks)
 //   out  [B, Lq, H * hd] bf16; rows before kst see nothing and are zero
+//   out_lo like out: what rounding took off it (out + out_lo holds 16 significant bits); the
+//        backward forms D = rowsum(dout * out) from both, so that the rounding of out does not
+//        reach the gradient. May be null in a forward that no backward follows.
 //   lse  [B, H, Lq] fp32: base-2 log-sum-exp of the scaled scores (+inf: a row that sees nothing)
 // Backward: dqkv [B, Lk, (H + 2 G) * hd] bf16 contiguous, every element written; workspace
 // dsum fp32 [B, H, Lq]. No atomics: results do not depend on the order of execution.
@@ -20,6 +23,7 @@ struct WindowAttnArgs {
   long long ld = 0, sb = 0;
   const int* kstart = nullptr;  // int32 [B]
   void* out = nullptr;
+  void* out_lo = nullptr;
   float* lse = nullptr;
   const void* dout = nullptr;   // bf16 [B, Lq, H * hd] contiguous
   void* dqkv = nullptr;

@@ -59,43 +59,47 @@ def windowed_attention_reference(qkv: torch.Tensor, kstart: torch.Tensor, heads:
     return torch.matmul(p, v).transpose(1, 2).reshape(B, lq, heads * hd)
 
 
-def window_attention_fwd(qkv, ks, out, lse, heads: int, kv_heads: int, lq: int, window: int, sinks: int,
-                         scale: float = 0.0) -> None:
-    """Native forward into ``out [B, lq, heads * hd]`` bf16 and ``lse [B, heads, lq]`` fp32."""
+def window_attention_fwd(qkv, ks, heads: int, kv_heads: int, lq: int, window: int, sinks: int, scale: float = 0.0,
+                         keep: bool = True):
+    """Native forward: ``out [B, lq, heads * hd]`` bf16 and, for a backward (``keep``), what
+    rounding took off it and the log-sum-exp ``[B, heads, lq]`` (else None and a workspace)."""
 
-    ext().window_attn_fwd(qkv, ks, out, lse, heads, kv_heads, lq, window, sinks, scale, error_word(qkv.device))
+    B, _, W = qkv.shape
+    width = W // (heads + 2 * kv_heads) * heads
+    out = torch.empty(B, lq, width, dtype=torch.bfloat16, device=qkv.device)
+    out_lo = torch.empty_like(out) if keep else None
+    lse = torch.empty(B, heads, lq, dtype=torch.float32, device=qkv.device)
+    ext().window_attn_fwd(qkv, ks, out, lse, heads, kv_heads, lq, window, sinks, scale, error_word(qkv.device), out_lo)
+    return out, out_lo, lse
 
 
-def window_attention_bwd(qkv, ks, out, lse, dout, dqkv, heads: int, kv_heads: int, lq: int, window: int, sinks: int,
-                         scale: float = 0.0) -> None:
-    """Native backward: every element of ``dqkv`` is written."""
+def window_attention_bwd(qkv, ks, out, out_lo, lse, dout, heads: int, kv_heads: int, lq: int, window: int, sinks: int,
+                         scale: float = 0.0) -> torch.Tensor:
+    """Native backward: the gradient of ``qkv`` (bf16, contiguous)."""
 
-    dsum = torch.empty_like(lse)
-    ext().window_attn_bwd(qkv, ks, out, lse, dout, dqkv, dsum, heads, kv_heads, lq, window, sinks, scale,
-                          error_word(qkv.device))
+    dqkv = torch.empty(qkv.shape, dtype=torch.bfloat16, device=qkv.device)
+    ext().window_attn_bwd(qkv, ks, out, lse, dout, dqkv, torch.empty_like(lse), heads, kv_heads, lq, window, sinks,
+                          scale, error_word(qkv.device), out_lo)
+    return dqkv
 
 
 class WindowedAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, kstart, heads, kv_heads, lq, window, sinks, scale):
-        B, Lk, W = qkv.shape
-        hd = W // (heads + 2 * kv_heads)
-        out = torch.empty(B, lq, heads * hd, dtype=torch.bfloat16, device=qkv.device)
-        lse = torch.empty(B, heads, lq, dtype=torch.float32, device=qkv.device)
-        window_attention_fwd(qkv, kstart, out, lse, heads, kv_heads, lq, window, sinks, scale)
-        ctx.save_for_backward(qkv, kstart, out, lse)
-        ctx.meta = (heads, kv_heads, lq, window, sinks, scale)
+    def forward(ctx, qkv, kstart, *args):
+        keep = ctx.needs_input_grad[0]
+        out, out_lo, lse = window_attention_fwd(qkv, kstart, *args, keep=keep)
+        if keep:
+            ctx.save_for_backward(qkv, kstart, out, out_lo, lse)
+            ctx.args = args
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        qkv, ks, out, lse = ctx.saved_tensors
+        qkv, ks, out, out_lo, lse = ctx.saved_tensors
         dout = dout.to(torch.bfloat16).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
-        dqkv = torch.empty(qkv.shape, dtype=torch.bfloat16, device=qkv.device)
-        window_attention_bwd(qkv, ks, out, lse, dout, dqkv, *ctx.meta)
-        return dqkv, None, None, None, None, None, None, None
+        return window_attention_bwd(qkv, ks, out, out_lo, lse, dout, *ctx.args), *([None] * 7)
 
 
 def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: int, window: int, sinks: int = 0,
