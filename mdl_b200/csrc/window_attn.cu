@@ -6,25 +6,25 @@
 // that the window's lower edge cuts need a mask. A query tile visits the tiles of the sinks and
 // then those of its window, so the cost grows with the window and not with the history.
 //
-// Forward (192 threads, two persistent CTAs an SM, 256 TMEM columns each: S 128, P 64, O 64).
+// Forward (320 threads, two persistent CTAs an SM, 256 TMEM columns each: S 128, P 64, O 64).
 // Work item = sample, head, query tile.
-//   warp 0     TMA: Q, and K / V tiles of 128 rows in two-stage rings
-//   warp 1     MMA: S = Q K^T; O += P V with P as the A operand straight from TMEM
-//   warps 2-5  softmax, thread = query row: P = exp2(S * c - m) as bf16 into TMEM. m is a
-//              reference that moves only when a score passes it by more than 8 (exp2 of the
-//              excess stays below 256), so O is rarely rescaled and is read once, at the end.
-// S of the next tile is issued as soon as the softmax holds the present one in registers.
+//   warp 0     walks the items; TMA: Q, K and V tiles into two-stage rings
+//   warp 1     issues: S = Q K^T; O += P V with P as the A operand straight from TMEM
+//   warps 2-9  softmax, two warps a set of 32 query rows: P = exp2(S * c - m) as bf16 into
+//              TMEM. m is a reference that moves only when a score passes it by more than 8
+//              (exp2 of the excess stays below 256), so O is rarely rescaled, and is read once.
+// S of the next tile, of the next item too, is issued as soon as the softmax holds the present
+// one in registers.
 //
-// Backward, two launches of one kernel (320 threads, one persistent CTA an SM, 512 columns):
-// a stationary tile of 128 rows meets a stream of 64-row tiles,
+// Backward, two launches of one kernel (320 threads, two persistent CTAs an SM): a stationary
+// tile of 128 rows meets a stream of 64-row tiles,
 //   S = A1 B1^T, dP = A2 B2^T, P = exp2(S * c - lse), dS = P * (dP - D),
 //   queries stationary: A = Q, dO; B = K, V;  dQ += dS K;  D = rowsum(dO * O) on the way
 //   keys stationary:    A = K, V;  B = Q, dO; dV += P dO, dK += dS Q  (all transposed; the query
 //                       heads that share the key head follow one another)
-// Two warpgroups take the stream's steps in turn, each with its own S, dP, P and dS columns, so
-// that the products of one run under the exponentials of the other. Recomputing S and dP in
-// both launches costs two products more than one launch that adds dQ to memory would, and needs
-// no fp32 buffer, no clearing, no atomics: every sum has one owner and one order.
+// Recomputing S and dP in the second launch costs two products more than one launch that adds
+// dQ to memory would, and needs no fp32 buffer, no clearing, no atomics: every sum has one
+// owner and one order.
 //
 // Every wait is bounded (error word + abort flag) and every role drains what it has in flight
 // before the CTA exits.
@@ -42,10 +42,9 @@
 namespace mdl {
 namespace {
 
-constexpr int TILE = 128;               // rows of a stationary tile and of a forward key tile
-constexpr int HALF = 64;                // rows of a streamed tile of the backward
+constexpr int TILE = 128;               // rows of a tile
+constexpr int BOX = 64;                 // rows of a TMA box, and of a step of the backward
 constexpr int TILE_BYTES = TILE * 128;  // 128-byte rows: 64 columns, the head's hd first
-constexpr int HALF_BYTES = HALF * 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr int F_THREADS = 320, F_TMEM = 256;
@@ -53,14 +52,12 @@ constexpr int RECS = 4;                         // item records in flight
 constexpr int TAIL = 512;                       // barriers and item records
 // Q[2] | K[2] | V[2] | row maxima and sums of the column halves, [2][2][128] each | references [2][128]
 constexpr int F_SMEM = 1024 + 6 * TILE_BYTES + 10 * TILE * 4 + TAIL;
-constexpr int B_THREADS = 576, B_TMEM = 512;
-constexpr int B_STAGES = 4;
-// stationary pair [2] | queries stationary: O and its remainder [2] | streamed pair [4] |
-// lse, D of the streamed rows [4][64], or lse of the stationary rows [2][128] | barriers
-constexpr int b_smem(bool keys) {
-  return 1024 + (keys ? 4 : 8) * TILE_BYTES + 2 * B_STAGES * HALF_BYTES + B_STAGES * 2 * HALF * 4 + TAIL;
-}
-static_assert(2 * F_SMEM <= 227 * 1024 && b_smem(false) <= 227 * 1024, "shared memory budget");
+constexpr int B_THREADS = 320, B_TMEM = 256, B_STAGES = 4;
+constexpr int BOX_BYTES = BOX * 128;
+// stationary pair | streamed pair [4] | lse, D of the streamed rows [4][64] (or lse of the
+// stationary rows [128]) | halves of D [2][2][128] | tail
+constexpr int B_SMEM = 1024 + 2 * TILE_BYTES + 2 * B_STAGES * BOX_BYTES + 2 * B_STAGES * BOX * 4 + 4 * TILE * 4 + TAIL;
+static_assert(2 * (F_SMEM + 1024) <= 228 * 1024 && 2 * (B_SMEM + 1024) <= 228 * 1024, "two blocks an SM");
 
 struct Params {
   __nv_bfloat16* out;
@@ -173,7 +170,7 @@ __device__ __forceinline__ uint64_t desc_of(const void* base) { return make_smem
 __device__ __forceinline__ uint64_t desc_mn_of(const void* base) {
   return make_smem_desc(smem_u32(base), TILE_BYTES, 1024);
 }
-constexpr uint32_t K_STEP = 2, MN_STEP = 128, TILE_UNITS = TILE_BYTES / 16, HALF_UNITS = HALF_BYTES / 16;
+constexpr uint32_t K_STEP = 2, MN_STEP = 128, TILE_UNITS = TILE_BYTES / 16, BOX_UNITS = BOX_BYTES / 16;
 
 // True on one lane of a converged warp, always the same one. The compiler knows that a single
 // lane runs what follows and keeps the operands of the tensor instructions in uniform registers.
@@ -259,10 +256,10 @@ __device__ __forceinline__ uint32_t range_bits(int l, int h, int w) {
   return (0xFFFFFFFFu >> (31 - b)) & (0xFFFFFFFFu << a);
 }
 
-// 128 rows as two boxes of 64 (one tensor map serves both tile heights).
+// 128 rows as two boxes of 64.
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int b) {
   tma_load_3d(dst, tm, bar, x, y, b);
-  tma_load_3d(dst + HALF_BYTES, tm, bar, x, y + HALF, b);
+  tma_load_3d(dst + BOX * 128, tm, bar, x, y + BOX, b);
 }
 
 // One row of hd zeros (bf16).
@@ -271,9 +268,9 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int hd) {
 }
 
 // ============================================================================ work items
-// FORWARD and QUERIES: query tiles, key steps of 128 or 64 rows; KEYS: key tiles, query steps
-// of 64 rows of each query head of the group. Positions are relative to the first valid token.
-enum class Kind { FORWARD, QUERIES, KEYS };
+// Query tiles with runs of ROWS keys as their steps (forward, and backward with queries
+// stationary), or key tiles (KEYS) with runs of ROWS queries of each query head of the group.
+// Positions are relative to the first valid token.
 
 struct alignas(16) Item {
   int h, b, kst, n;    // head, sample, first valid token, steps (-1: no more items)
@@ -281,19 +278,17 @@ struct alignas(16) Item {
   int len, pad[3];     // valid tokens
 };
 
-// First row of step j (KEYS: of step s of a query head).
-template <Kind K>
+// First row of step j (key tiles: of step j of a query head).
+template <bool KEYS, int ROWS>
 __device__ __forceinline__ int step_row(int j, int cs, int k0) {
-  constexpr int ROWS = K == Kind::FORWARD ? TILE : HALF;
-  if constexpr (K == Kind::KEYS) return ROWS * (k0 + j);
-  return ROWS * (j < cs ? j : k0 + j - cs);
+  return ROWS * (KEYS ? k0 + j : (j < cs ? j : k0 + j - cs));
 }
 
 // A block's items one after another (every gridDim.x-th). Only the loading warp walks them; it
 // hands the others a record an item in shared memory, so that they carry neither the walk nor
 // its registers (kept beside 64 scores a thread they spilled, and the spills set the pace).
 // kstart of the next item is loaded an item ahead, and the digits are carried along.
-template <Kind K>
+template <bool KEYS, int ROWS>
 struct Walk {
   Item it;
   int i;                // index within the pair (head, sample)
@@ -325,23 +320,21 @@ struct Walk {
     it.len = p.Lk - it.kst;
     it.qf = max(0, p.Lk - p.Lq - it.kst);
     it.n = it.cs = it.k0 = 0;
-    if constexpr (K == Kind::KEYS) {
+    if constexpr (KEYS) {
       // the sinks' tile comes first: every query sees it
       it.t = i;
       if (TILE * it.t >= it.len) return true;
       const int qs = max(TILE * it.t, it.qf);
       const int qe = TILE * it.t < p.sinks ? it.len : min(it.len, TILE * it.t + TILE - 1 + p.window);
-      it.k0 = qs / HALF;
-      it.cs = qe > qs ? (qe + HALF - 1) / HALF - it.k0 : 0;
+      it.k0 = qs / ROWS;
+      it.cs = qe > qs ? (qe + ROWS - 1) / ROWS - it.k0 : 0;
       it.n = it.cs * (p.H / p.G);
     } else {
-      constexpr int ROWS = K == Kind::FORWARD ? TILE : HALF;
       it.t = (it.len + TILE - 1) / TILE - 1 - i;  // the last tile first
       if (it.t < 0 || TILE * (it.t + 1) <= it.qf) return true;
-      const int end = (min(TILE * (it.t + 1), it.len) + ROWS - 1) / ROWS;
       it.k0 = max(0, max(TILE * it.t, it.qf) - p.window + 1) / ROWS;
       it.cs = min((min(p.sinks, it.len) + ROWS - 1) / ROWS, it.k0);
-      it.n = it.cs + end - it.k0;
+      it.n = it.cs + (min(TILE * (it.t + 1), it.len) + ROWS - 1) / ROWS - it.k0;
     }
     return true;
   }
@@ -415,7 +408,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     const int q0 = p.Lk - p.Lq;
     int items = 0, g = 0;
     bool ok = true;
-    Walk<Kind::FORWARD> w(p);
+    Walk<false, TILE> w(p);
     while (ok && w.next(p)) {
       const Item& it = w.it;
       // queries before the first valid token (a share of them per item)
@@ -444,7 +437,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       __syncwarp();
       ++items;
       for (int j = 0; j < it.n; ++j, ++g) {
-        const int st = g & 1, y = it.kst + step_row<Kind::FORWARD>(j, it.cs, it.k0);
+        const int st = g & 1, y = it.kst + step_row<false, TILE>(j, it.cs, it.k0);
         if (!warp_wait(&kv_empty[st], ((g >> 1) + 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
@@ -474,7 +467,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     // The whole warp waits (uniform registers hold its counters and descriptors); lane 0
     // issues. Scores run one step ahead of the products, across items.
     constexpr uint32_t idesc_s = make_idesc_bf16(TILE, TILE, false, false);
-    constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, 64, false, true);
+    constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, HD, false, true);
     const uint64_t dQ = desc_of(sQ), dK = desc_of(sK), dV = desc_mn_of(sV);
     int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the block
     bool ok = true;
@@ -615,7 +608,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         // exponentiated; a full one needs no mask.
         uint32_t vm[2] = {~0u, ~0u};
         bool live[2] = {true, true}, part[2] = {false, false};
-        const int key0 = step_row<Kind::FORWARD>(j, cs, k0);
+        const int key0 = step_row<false, TILE>(j, cs, k0);
         if (key0 == TILE * t || (TILE * t - key0 + TILE > p.window && key0 + TILE > p.sinks)) {
           const int d = TILE * t + r - key0 - 64 * half;  // columns up to d are not in the future
           const int lo = d - p.window + 1, sk = min(d, p.sinks - 1 - key0 - 64 * half);
@@ -728,56 +721,55 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 // ============================================================================ backward
 // KEYS: the stationary tile holds keys (dK, dV), else queries (dQ and D).
 template <int HD, bool KEYS>
-__global__ void __launch_bounds__(B_THREADS, 1)
+__global__ void __launch_bounds__(B_THREADS, 2)
     window_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv,
-                      const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_o,
-                      const __grid_constant__ CUtensorMap tm_olo, const Params p) {
+                      const __grid_constant__ CUtensorMap tm_do, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
-  uint8_t* sA1 = smem;                                // [2]
-  uint8_t* sA2 = sA1 + 2 * TILE_BYTES;                // [2]
-  uint8_t* sO = sA2 + 2 * TILE_BYTES;                 // queries stationary: O | remainder, [2]
-  uint8_t* sB1 = sO + (KEYS ? 0 : 4) * TILE_BYTES;    // [4]
-  uint8_t* sB2 = sB1 + B_STAGES * HALF_BYTES;         // [4]
-  float* sLse = reinterpret_cast<float*>(sB2 + B_STAGES * HALF_BYTES);  // [4][64], or [2][128]
-  float* sD = sLse + B_STAGES * HALF;                                  // [4][64]
-  Item* recs = reinterpret_cast<Item*>(sD + B_STAGES * HALF);          // [RECS]
+  uint8_t* sA1 = smem;
+  uint8_t* sA2 = sA1 + TILE_BYTES;
+  uint8_t* sB1 = sA2 + TILE_BYTES;               // [4]
+  uint8_t* sB2 = sB1 + B_STAGES * BOX_BYTES;     // [4]
+  float* sLse = reinterpret_cast<float*>(sB2 + B_STAGES * BOX_BYTES);  // [4][64], or [128]
+  float* sD = sLse + B_STAGES * BOX;                                   // [4][64]
+  float* sHalf = sD + B_STAGES * BOX;                                  // [2 items][2 halves][128]
+  Item* recs = reinterpret_cast<Item*>(sHalf + 4 * TILE);              // [RECS]
   uint64_t* bars = reinterpret_cast<uint64_t*>(recs + RECS);
-  uint64_t* a_full = bars;        // [2]
-  uint64_t* a_empty = bars + 2;   // [2]
-  uint64_t* b_full = bars + 4;    // [4]
-  uint64_t* b_empty = bars + 8;   // [4]
-  uint64_t* s_full = bars + 12;   // [2]
-  uint64_t* p_full = bars + 16;   // [2]
-  uint64_t* p_empty = bars + 18;  // [2]
-  uint64_t* acc_full = bars + 20;
-  uint64_t* acc_empty = bars + 21;
-  uint64_t* done = bars + 22;
-  uint64_t* rec_full = bars + 23;   // [RECS]
-  uint64_t* rec_empty = bars + 27;  // [RECS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
+  uint64_t* a_full = bars;
+  uint64_t* a_empty = bars + 1;
+  uint64_t* b_full = bars + 2;    // [4]
+  uint64_t* b_empty = bars + 6;   // [4]
+  uint64_t* s_full = bars + 10;
+  uint64_t* s_empty = bars + 11;
+  uint64_t* p_full = bars + 12;
+  uint64_t* p_empty = bars + 13;
+  uint64_t* acc_full = bars + 14;
+  uint64_t* acc_empty = bars + 15;
+  uint64_t* done = bars + 16;
+  uint64_t* rec_full = bars + 17;   // [RECS]
+  uint64_t* rec_empty = bars + 21;  // [RECS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(RECS * sizeof(Item) + 32 * 8 <= TAIL, "records and barriers");
+  static_assert(RECS * sizeof(Item) + 26 * 8 <= TAIL, "records and barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&a_full[s], KEYS ? 1 : 33);   // TMA bytes (+ the 32 lanes that copy lse, D)
-      mbar_init(&a_empty[s], KEYS ? 1 : 17);  // the products (+ the warps that read O and dO)
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 8);
-      mbar_init(&p_empty[s], 1);
+    mbar_init(a_full, KEYS ? 1 : 33);  // TMA bytes (+ the 32 lanes that copy lse)
+    mbar_init(a_empty, KEYS ? 1 : 9);  // the last scores (+ the warps that read dO)
+    for (int s = 0; s < B_STAGES; ++s) {
+      mbar_init(&b_full[s], KEYS ? 33 : 1);  // TMA bytes (+ the 32 lanes that copy lse and D)
+      mbar_init(&b_empty[s], 1);
     }
     for (int s = 0; s < RECS; ++s) {
       mbar_init(&rec_full[s], 1);
-      mbar_init(&rec_empty[s], 17);  // the issuing warp and the computing warps
+      mbar_init(&rec_empty[s], 9);  // the issuing warp and the computing warps
     }
-    for (int s = 0; s < B_STAGES; ++s) {
-      mbar_init(&b_full[s], KEYS ? 33 : 1);
-      mbar_init(&b_empty[s], 1);
-    }
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 8);
+    mbar_init(p_full, 8);
+    mbar_init(p_empty, 1);
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 16);
+    mbar_init(acc_empty, 8);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -790,112 +782,103 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // per warpgroup: S, dP (64 fp32 columns each), P, dS (32 columns of bf16 pairs); accumulators
-  auto tS = [&](int s) { return tmem + s * 128; };
-  auto tP = [&](int s) { return tmem + 256 + s * 64; };
-  const uint32_t tAcc0 = tmem + 384, tAcc1 = tmem + 448;
-  constexpr Kind KIND = KEYS ? Kind::KEYS : Kind::QUERIES;
+  // S 64 | dP 64 | P 32 | dS 32 | accumulators hd each. With dK and dV 64 wide there is no room
+  // for P and dS: each warp then puts them over the first half of its own scores, and the next
+  // scores wait for the products that read them.
+  constexpr bool OVER = KEYS && HD == 64;
+  const uint32_t tS = tmem, tDP = tmem + 64, tP = OVER ? tS : tmem + 128, tDS = OVER ? tDP : tmem + 160;
+  const uint32_t tAcc0 = tmem + (OVER ? 128 : 192), tAcc1 = KEYS ? tAcc0 + HD : tAcc0;
+  constexpr uint32_t PAIR_STEP = OVER ? 32 : 16;  // columns from one half's P to the other's
   const int q0 = p.Lk - p.Lq;
 
   if (warp == 0) {
+    // ------------------------------------------------------------ walk and load
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_kv);
       tma_prefetch_desc(&tm_do);
-      if (!KEYS) {
-        tma_prefetch_desc(&tm_o);
-        tma_prefetch_desc(&tm_olo);
-      }
     }
     bool ok = true;
-    Walk<KIND> w(p);
-    int items = 0, g = 0, a_issued = 0;
+    Walk<KEYS, BOX> w(p);
+    int items = 0, g = 0;
     const int width = (p.H + 2 * p.G) * HD;
     while (ok && w.next(p)) {
-      const Item& at = w.it;
-      const int sa = items & 1, ya = at.kst + TILE * at.t;
+      const Item& it = w.it;
+      const int ya = it.kst + TILE * it.t;
       // gradients of what nobody sees or asks for: a share, per item, of the rows before the
       // first valid token (queries: the first query), and valid keys without a query
-      const long long trow0 = static_cast<long long>(at.b) * p.Lk;
+      const long long trow0 = static_cast<long long>(it.b) * p.Lk;
       auto clear = [&](int row) {
-        __nv_bfloat16* dst = p.dqkv + (trow0 + row) * width + (KEYS ? p.H + at.h : at.h) * HD;
+        __nv_bfloat16* dst = p.dqkv + (trow0 + row) * width + (KEYS ? p.H + it.h : it.h) * HD;
         zero_row(dst, HD);
         if (KEYS) zero_row(dst + p.G * HD, HD);
       };
-      for (int k = w.i * 32 + lane; k < at.kst + (KEYS ? 0 : at.qf); k += p.tiles * 32) clear(k);
-      if (at.n == 0) {
+      for (int k = w.i * 32 + lane; k < it.kst + (KEYS ? 0 : it.qf); k += p.tiles * 32) clear(k);
+      if (it.n == 0) {
         if (KEYS)
           for (int k = ya + lane; k < min(ya + TILE, p.Lk); k += 32) clear(k);
         continue;
       }
       const int slot = items % RECS;
-      // parity of the previous use of this stage; a fresh barrier passes parity 1 at once
+      // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
       if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
       if (lane == 0) {
-        recs[slot] = at;
+        recs[slot] = it;
         mbar_arrive(&rec_full[slot]);
       }
       __syncwarp();
-      if (!warp_wait(&a_empty[sa], ((items >> 1) + 1) & 1, p.err, abort_flag)) break;
+      if (!warp_wait(a_empty, (items + 1) & 1, p.err, abort_flag)) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&a_full[sa], (KEYS ? 2 : 4) * TILE_BYTES);
+        mbar_arrive_expect_tx(a_full, 2 * TILE_BYTES);
         if constexpr (KEYS) {
-          load_tile(sA1 + sa * TILE_BYTES, &tm_kv, &a_full[sa], (p.H + at.h) * HD, ya, at.b);
-          load_tile(sA2 + sa * TILE_BYTES, &tm_kv, &a_full[sa], (p.H + p.G + at.h) * HD, ya, at.b);
+          load_tile(sA1, &tm_kv, a_full, (p.H + it.h) * HD, ya, it.b);
+          load_tile(sA2, &tm_kv, a_full, (p.H + p.G + it.h) * HD, ya, it.b);
         } else {
-          load_tile(sA1 + sa * TILE_BYTES, &tm_q, &a_full[sa], at.h * HD, ya - q0, at.b);
-          load_tile(sA2 + sa * TILE_BYTES, &tm_do, &a_full[sa], at.h * HD, ya - q0, at.b);
-          load_tile(sO + sa * TILE_BYTES, &tm_o, &a_full[sa], at.h * HD, ya - q0, at.b);
-          load_tile(sO + (2 + sa) * TILE_BYTES, &tm_olo, &a_full[sa], at.h * HD, ya - q0, at.b);
+          load_tile(sA1, &tm_q, a_full, it.h * HD, ya - q0, it.b);
+          load_tile(sA2, &tm_do, a_full, it.h * HD, ya - q0, it.b);
         }
       }
       __syncwarp();
-      a_issued = ++items;
-      if constexpr (!KEYS) {
+      ++items;
+      // lse (and D) of queries from `rel` on; rows that are no queries get zeros and are never
+      // visible
+      auto copy_rows = [&](float* lse, float* d, int rel, int h, uint64_t* bar) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = TILE * at.t + lane + 32 * e;
-          const bool real = c >= at.qf && c < at.len;
-          const long long off = (static_cast<long long>(at.b) * p.H + at.h) * p.Lq + (real ? at.kst + c - q0 : 0);
-          copy4(sLse + sa * TILE + lane + 32 * e, p.lse + off, real);
+        for (int e = 0; e < (KEYS ? BOX : TILE) / 32; ++e) {
+          const int c = lane + 32 * e;
+          const bool real = rel + c >= it.qf && rel + c < it.len;
+          const long long off = (static_cast<long long>(it.b) * p.H + h) * p.Lq + (real ? it.kst + rel + c - q0 : 0);
+          copy4(lse + c, p.lse + off, real);
+          if (KEYS) copy4(d + c, p.dsum + off, real);
         }
-        copies_arrive(&a_full[sa]);
-      }
-      int h = KEYS ? at.h * (p.H / p.G) : at.h;
-      for (int j = 0, s = 0; j < at.n; ++j, ++s, ++g) {
+        copies_arrive(bar);
+      };
+      if constexpr (!KEYS) copy_rows(sLse, nullptr, TILE * it.t, it.h, a_full);
+      int h = KEYS ? it.h * (p.H / p.G) : it.h;
+      for (int j = 0, s = 0; j < it.n; ++j, ++s, ++g) {
         const int st = g % B_STAGES;
         if (!warp_wait(&b_empty[st], (g / B_STAGES + 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
-        if (KEYS && s == at.cs) {  // the next query head of the group
+        if (KEYS && s == it.cs) {  // the next query head of the group
           s = 0;
           ++h;
         }
-        const int rel = step_row<KIND>(s, at.cs, at.k0), y = at.kst + rel;
+        const int rel = step_row<KEYS, BOX>(s, it.cs, it.k0), y = it.kst + rel;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&b_full[st], 2 * HALF_BYTES);
+          mbar_arrive_expect_tx(&b_full[st], 2 * BOX_BYTES);
           if constexpr (KEYS) {
-            tma_load_3d(sB1 + st * HALF_BYTES, &tm_q, &b_full[st], h * HD, y - q0, at.b);
-            tma_load_3d(sB2 + st * HALF_BYTES, &tm_do, &b_full[st], h * HD, y - q0, at.b);
+            tma_load_3d(sB1 + st * BOX_BYTES, &tm_q, &b_full[st], h * HD, y - q0, it.b);
+            tma_load_3d(sB2 + st * BOX_BYTES, &tm_do, &b_full[st], h * HD, y - q0, it.b);
           } else {
             const int kvh = h / (p.H / p.G);
-            tma_load_3d(sB1 + st * HALF_BYTES, &tm_kv, &b_full[st], (p.H + kvh) * HD, y, at.b);
-            tma_load_3d(sB2 + st * HALF_BYTES, &tm_kv, &b_full[st], (p.H + p.G + kvh) * HD, y, at.b);
+            tma_load_3d(sB1 + st * BOX_BYTES, &tm_kv, &b_full[st], (p.H + kvh) * HD, y, it.b);
+            tma_load_3d(sB2 + st * BOX_BYTES, &tm_kv, &b_full[st], (p.H + p.G + kvh) * HD, y, it.b);
           }
         }
         __syncwarp();
-        if constexpr (KEYS) {  // rows that are no queries get zeros and are never visible
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = lane + 32 * e;
-            const bool real = rel + c >= at.qf && rel + c < at.len;
-            const long long off = (static_cast<long long>(at.b) * p.H + h) * p.Lq + (real ? y + c - q0 : 0);
-            copy4(sLse + st * HALF + c, p.lse + off, real);
-            copy4(sD + st * HALF + c, p.dsum + off, real);
-          }
-          copies_arrive(&b_full[st]);
-        }
+        if constexpr (KEYS) copy_rows(sLse + st * BOX, sD + st * BOX, rel, h, &b_full[st]);
       }
     }
     const int slot = items % RECS;
@@ -904,16 +887,16 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       mbar_arrive(&rec_full[slot]);
     }
     __syncwarp();
-    if (lane == 0) {
-      for (int j = max(0, a_issued - 2); j < a_issued; ++j) mbar_wait(&a_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
+    if (lane == 0) {  // every copy into this CTA's smem has landed before the CTA may exit
+      if (items > 0) mbar_wait(a_full, (items - 1) & 1, nullptr, nullptr);
       for (int j = max(0, g - B_STAGES); j < g; ++j)
         mbar_wait(&b_full[j % B_STAGES], (j / B_STAGES) & 1, nullptr, nullptr);
     }
     __syncwarp();
   } else if (warp == 1) {
-    // see the forward's warp 1
-    constexpr uint32_t idesc_s = make_idesc_bf16(TILE, HALF, false, false);
-    constexpr uint32_t idesc_acc = make_idesc_bf16(TILE, 64, false, true);
+    // ------------------------------------------------------------ issue (see the forward)
+    constexpr uint32_t idesc_s = make_idesc_bf16(TILE, BOX, false, false);
+    constexpr uint32_t idesc_acc = make_idesc_bf16(TILE, HD, false, true);
     const uint64_t dA1 = desc_of(sA1), dA2 = desc_of(sA2), dB1 = desc_of(sB1), dB2 = desc_of(sB2);
     const uint64_t mB1 = desc_mn_of(sB1), mB2 = desc_mn_of(sB2);
     int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the block
@@ -925,28 +908,27 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       }
       return __reduce_max_sync(0xffffffffu, recs[i % RECS].n);
     };
-    // S and dP of the next step, up to two ahead (each warpgroup's columns, read before its P is
-    // there) and one item ahead (the stationary tiles are double-buffered and released by the
-    // item's last product)
     auto issue_s = [&]() -> bool {
-      const int st = a_g % B_STAGES, s = a_g & 1, sa = a_items & 1;
-      if ((a_j == 0 && !warp_wait(&a_full[sa], (a_items >> 1) & 1, p.err, abort_flag)) ||
-          !warp_wait(&b_full[st], (a_g / B_STAGES) & 1, p.err, abort_flag))
+      const int st = a_g % B_STAGES;
+      if ((a_j == 0 && !warp_wait(a_full, a_items & 1, p.err, abort_flag)) ||
+          !warp_wait(&b_full[st], (a_g / B_STAGES) & 1, p.err, abort_flag) ||
+          (a_g > 0 && !warp_wait(OVER ? p_empty : s_empty, (a_g - 1) & 1, p.err, abort_flag)))
         return false;
       tc_fence_after();
-      const uint64_t a1 = dA1 + sa * TILE_UNITS, a2 = dA2 + sa * TILE_UNITS;
-      const uint64_t b1 = dB1 + st * HALF_UNITS, b2 = dB2 + st * HALF_UNITS;
-      const uint32_t ts = tS(s);
+      const uint64_t b1 = dB1 + st * BOX_UNITS, b2 = dB2 + st * BOX_UNITS;
+      const bool last = a_j + 1 == a_n;
       if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(ts, a1 + ks * K_STEP, b1 + ks * K_STEP, idesc_s, ks);
+        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS, dA1 + ks * K_STEP, b1 + ks * K_STEP, idesc_s, ks);
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(ts + 64, a2 + ks * K_STEP, b2 + ks * K_STEP, idesc_s, ks);
-        tc_commit(&s_full[s]);
+        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tDP, dA2 + ks * K_STEP, b2 + ks * K_STEP, idesc_s, ks);
+        tc_commit(s_full);
+        if (last) tc_commit(a_empty);
       }
       __syncwarp();
       ++a_g;
-      if (++a_j == a_n) {
+      ++a_j;
+      if (last) {
         a_j = 0;
         a_n = steps_of(++a_items);
       }
@@ -954,38 +936,36 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     };
     a_n = steps_of(0);
     int n = a_n, g = 0;
+    if (ok && a_n > 0) ok = issue_s();
     for (int items = 0; ok && n > 0; ++items) {
       for (int j = 0; j < n; ++j, ++g) {
-        const int st = g % B_STAGES, s = g & 1;
-        while (ok && a_n > 0 && a_g <= g + 1 && a_items <= items + 1) ok = issue_s();
-        if (!ok || !warp_wait(&p_full[s], (g >> 1) & 1, p.err, abort_flag)) {
-          ok = false;
-          break;
-        }
-        if (a_n > 0 && a_g == g + 2 && a_items <= items + 1) ok = issue_s();
-        if (!ok || (j == 0 && items >= 1 && !warp_wait(acc_empty, (items - 1) & 1, p.err, abort_flag))) {
+        const int st = g % B_STAGES;
+        // (OVER: the next scores come after this step's products)
+        if ((!OVER && a_n > 0 && !issue_s()) || !warp_wait(p_full, g & 1, p.err, abort_flag) ||
+            (j == 0 && items >= 1 && !warp_wait(acc_empty, (items - 1) & 1, p.err, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint64_t b1 = mB1 + st * HALF_UNITS, b2 = mB2 + st * HALF_UNITS;
-        const uint32_t tp = tP(s), acc = j > 0 ? 1u : 0u;
-        const int sa = items & 1;
+        const uint64_t b1 = mB1 + st * BOX_UNITS, b2 = mB2 + st * BOX_UNITS;
+        const uint32_t acc = j > 0 ? 1u : 0u;
         const bool last = j + 1 == n;
         if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < HALF / 16; ++ks) {
-            if constexpr (KEYS) tc_mma_bf16_ts(tAcc0, tp + ks * 8, b2 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
-            tc_mma_bf16_ts(tAcc1, tp + 32 + ks * 8, b1 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
+          for (int ks = 0; ks < BOX / 16; ++ks) {
+            const uint32_t off = (ks >> 1) * PAIR_STEP + (ks & 1) * 8;
+            if constexpr (KEYS) tc_mma_bf16_ts(tAcc0, tP + off, b2 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
+            tc_mma_bf16_ts(tAcc1, tDS + off, b1 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
           }
-          tc_commit(&p_empty[s]);
+          tc_commit(p_empty);
           tc_commit(&b_empty[st]);
-          if (last) {
-            tc_commit(acc_full);
-            tc_commit(&a_empty[sa]);
-          }
+          if (last) tc_commit(acc_full);
         }
         __syncwarp();
+        if (OVER && a_n > 0 && !issue_s()) {
+          ok = false;
+          break;
+        }
       }
       if (!ok) break;
       n = steps_of(items + 1);
@@ -999,51 +979,44 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ compute
-    const int wg = ((warp - 2) >> 2) & 1;  // takes the steps of its parity,
-    const int half = (warp - 2) >> 3;      // this half of their columns
-    const int quarter = warp & 3;
+    // Two warps share 32 rows, 32 of the 64 columns each.
+    const int half = (warp - 2) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t tS_own = tS + lane_off + 32 * half, tDP_own = tDP + lane_off + 32 * half;
+    const uint32_t tP_own = tP + lane_off + PAIR_STEP * half, tDS_own = tDS + lane_off + PAIR_STEP * half;
     bool ok = true;
     int items = 0, g = 0;
-    // keys: dV by warpgroup 0, dK by warpgroup 1, half of the columns a warp; queries: a quarter
-    // of dQ each
-    constexpr int COLS = KEYS ? HD / 2 : HD / 4;
-    const int col0 = KEYS ? half * COLS : (2 * wg + half) * COLS;
+    // keys: dV or dK; queries: half of dQ
+    constexpr int COLS = KEYS ? HD : HD / 2;
+    const int col0 = KEYS ? 0 : half * COLS;
+    const uint32_t tAcc_own = (KEYS && half == 0 ? tAcc0 : tAcc1) + lane_off + col0;
     // Gradients of item k: written while its successor's first step is under way.
-    bool pending = false;
     auto write_grad = [&](int k) -> bool {
       if (!warp_wait(acc_full, k & 1, p.err, abort_flag)) return false;
       tc_fence_after();
-      const uint32_t src = (KEYS && wg == 0 ? tAcc0 : tAcc1) + lane_off + col0;
-      uint32_t gr[COLS < 16 ? 16 : COLS];  // eight columns of 32-wide heads: read with eight more
-#pragma unroll
-      for (int c = 0; c < (COLS + 15) / 16; ++c) tmem_ld16(src + c * 16, gr + c * 16);
       const Item& it = recs[k % RECS];
       const int own = TILE * it.t + r;
       const bool store = own < it.len && (KEYS || own >= it.qf);
-      const int head = KEYS ? (wg == 0 ? p.H + p.G + it.h : p.H + it.h) : it.h;
+      const int head = KEYS ? (half == 0 ? p.H + p.G + it.h : p.H + it.h) : it.h;
       __nv_bfloat16* dst = p.dqkv + (static_cast<long long>(it.b) * p.Lk + it.kst + own) * (p.H + 2 * p.G) * HD +
                            head * HD + col0;
-      tmem_wait_ld();
+      const float f = (KEYS && half == 0) ? 1.f : p.scale;
+#pragma unroll
+      for (int e = 0; e < COLS / 8; ++e) {  // few registers at a time: the scores are held
+        uint32_t gr[8], y[4];
+        tmem_ld8(tAcc_own + 8 * e, gr);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = pack2(__uint_as_float(gr[2 * c]) * f, __uint_as_float(gr[2 * c + 1]) * f);
+        if (store) reinterpret_cast<uint4*>(dst)[e] = make_uint4(y[0], y[1], y[2], y[3]);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(acc_empty);
         mbar_arrive(&rec_empty[k % RECS]);
       }
-      const float f = (KEYS && wg == 0) ? 1.f : p.scale;
-      if (store) {
-#pragma unroll
-        for (int e = 0; e < COLS / 8; ++e) {
-          uint32_t y[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            y[c] = pack2(__uint_as_float(gr[8 * e + 2 * c]) * f, __uint_as_float(gr[8 * e + 2 * c + 1]) * f);
-          reinterpret_cast<uint4*>(dst)[e] = make_uint4(y[0], y[1], y[2], y[3]);
-        }
-      }
-      pending = false;
       return true;
     };
     for (;; ++items) {
@@ -1052,81 +1025,94 @@ __global__ void __launch_bounds__(B_THREADS, 1)
         ok = false;
         break;
       }
-      const Item& at = recs[slot];
-      const int n = at.n;
+      const Item& it = recs[slot];
+      const int n = it.n;
       if (n < 0) break;
-      const int cs = at.cs, k0 = at.k0, own = TILE * at.t + r;
+      const int cs = it.cs, k0 = it.k0, t = it.t, own = TILE * t + r;
       float row_lse = 0.f, row_d = 0.f;
       if constexpr (!KEYS) {
-        const int sa = items & 1;
-        if (!warp_wait(&a_full[sa], (items >> 1) & 1, p.err, abort_flag)) {
+        // D of the row from dO (shared memory) and the output (16 bits: out + out_lo), half of
+        // the head a warp; the output's loads are under way while the tile is waited for
+        constexpr int V = HD / 16;  // 16-byte pieces of half a row
+        const bool real = own >= it.qf && own < it.len;
+        const long long o = ((static_cast<long long>(it.b) * p.Lq + it.kst + own - q0) * p.H + it.h) * HD + half * (HD / 2);
+        uint4 hv[V], lv[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          hv[c] = lv[c] = make_uint4(0, 0, 0, 0);
+          if (real) {
+            hv[c] = __ldg(reinterpret_cast<const uint4*>(p.out + o) + c);
+            lv[c] = __ldg(reinterpret_cast<const uint4*>(p.out_lo + o) + c);
+          }
+        }
+        if (!warp_wait(a_full, items & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
-        row_lse = sLse[sa * TILE + r];
-        const uint8_t* go = sA2 + sa * TILE_BYTES + r * 128;
-        const uint8_t* oh = sO + sa * TILE_BYTES + r * 128;
-        const uint8_t* ol = sO + (2 + sa) * TILE_BYTES + r * 128;
+        row_lse = sLse[r];
+        const uint8_t* go = sA2 + r * 128;
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          const int off = (c ^ (r & 7)) * 16;
-          const uint4 gv = *reinterpret_cast<const uint4*>(go + off);
-          const uint4 hv = *reinterpret_cast<const uint4*>(oh + off);
-          const uint4 lv = *reinterpret_cast<const uint4*>(ol + off);
-          const uint32_t e[4] = {gv.x, gv.y, gv.z, gv.w}, a[4] = {hv.x, hv.y, hv.z, hv.w},
-                         z[4] = {lv.x, lv.y, lv.z, lv.w};
+        for (int c = 0; c < V; ++c) {
+          const uint4 gv = *reinterpret_cast<const uint4*>(go + ((half * V + c) ^ (r & 7)) * 16);
+          const uint32_t e[4] = {gv.x, gv.y, gv.z, gv.w}, a[4] = {hv[c].x, hv[c].y, hv[c].z, hv[c].w},
+                         z[4] = {lv[c].x, lv[c].y, lv[c].z, lv[c].w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            row_d = fmaf(__uint_as_float(a[k] << 16) + __uint_as_float(z[k] << 16), __uint_as_float(e[k] << 16), row_d);
-            row_d = fmaf(__uint_as_float(a[k] & 0xFFFF0000u) + __uint_as_float(z[k] & 0xFFFF0000u),
-                         __uint_as_float(e[k] & 0xFFFF0000u), row_d);
+          for (int i = 0; i < 4; ++i) {
+            row_d = fmaf(__uint_as_float(a[i] << 16) + __uint_as_float(z[i] << 16), __uint_as_float(e[i] << 16), row_d);
+            row_d = fmaf(__uint_as_float(a[i] & 0xFFFF0000u) + __uint_as_float(z[i] & 0xFFFF0000u),
+                         __uint_as_float(e[i] & 0xFFFF0000u), row_d);
           }
         }
+        float* part = sHalf + (items & 1) * 2 * TILE;
+        part[half * TILE + r] = row_d;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&a_empty[sa]);
-        if (wg == 0 && half == 0 && own >= at.qf && own < at.len)
-          p.dsum[(static_cast<long long>(at.b) * p.H + at.h) * p.Lq + at.kst + own - q0] = row_d;
+        if (lane == 0) mbar_arrive(a_empty);
+        pair_sync(1 + quarter);
+        row_d = part[r] + part[TILE + r];
+        if (half == 0 && real)
+          p.dsum[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.kst + own - q0] = row_d;
       }
       for (int j = 0, s_ = 0; j < n; ++j, ++s_, ++g) {
         if (KEYS && s_ == cs) s_ = 0;
-        if ((g & 1) != wg) continue;
         const int st = g % B_STAGES;
-        const int rel = step_row<KIND>(s_, cs, k0);
+        const int c0 = step_row<KEYS, BOX>(s_, cs, k0) + 32 * half;  // this warp's first column
         if ((KEYS && !warp_wait(&b_full[st], (g / B_STAGES) & 1, p.err, abort_flag)) ||
-            !warp_wait(&s_full[wg], (g >> 1) & 1, p.err, abort_flag)) {
+            !warp_wait(s_full, g & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint32_t s[32], dp[32];
-        tmem_ld32(tS(wg) + lane_off + 32 * half, s);
-        tmem_ld32(tS(wg) + lane_off + 64 + 32 * half, dp);
+        tmem_ld32(tS_own, s);
+        tmem_ld32(tDP_own, dp);
         // visible columns of this row (see the forward)
+        const int r0 = TILE * t + 32 * quarter;  // this warp's first row
         uint32_t vm = ~0u;
         if constexpr (KEYS) {
-          const bool whole = rel >= TILE * at.t + TILE - 1 && rel >= at.qf && rel + HALF <= at.len &&
-                             (TILE * (at.t + 1) <= p.sinks || rel + HALF - TILE * at.t <= p.window);
+          const bool whole = c0 >= r0 + 31 && c0 >= it.qf && c0 + 32 <= it.len &&
+                             (r0 + 32 <= p.sinks || c0 + 32 - r0 <= p.window);
           if (!whole) {
-            const int lo = max(own, at.qf) - rel;
-            const int hi = (own < p.sinks ? at.len - 1 : min(at.len - 1, own + p.window - 1)) - rel;
-            vm = range_bits(lo, hi, half);
+            const int hi = own < p.sinks ? it.len - 1 : min(it.len - 1, own + p.window - 1);
+            vm = range_bits(max(own, it.qf) - c0, hi - c0, 0);
           }
         } else {
-          const bool whole = rel + HALF - 1 <= TILE * at.t && TILE * at.t >= at.qf && TILE * (at.t + 1) <= at.len &&
-                             (rel + HALF <= p.sinks || TILE * at.t + TILE - rel <= p.window);
+          const bool whole = c0 + 31 <= r0 && r0 >= it.qf && r0 + 32 <= it.len &&
+                             (c0 + 32 <= p.sinks || r0 + 32 - c0 <= p.window);
           if (!whole) {
-            const bool real = own >= at.qf && own < at.len;
-            const int d = real ? own - rel : -1;
-            vm = range_bits(d - p.window + 1, d, half) | range_bits(0, min(d, p.sinks - 1 - rel), half);
+            const int d = own >= it.qf && own < it.len ? own - c0 : -1;
+            vm = range_bits(d - p.window + 1, d, 0) | range_bits(0, min(d, p.sinks - 1 - c0), 0);
           }
         }
         const bool live = __any_sync(0xffffffffu, vm != 0u), part = __any_sync(0xffffffffu, vm != ~0u);
         tmem_wait_ld();
-        const float4* lse4 = reinterpret_cast<const float4*>(sLse + st * HALF + 32 * half);
-        const float4* d4 = reinterpret_cast<const float4*>(sD + st * HALF + 32 * half);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty);
+        const float4* lse4 = reinterpret_cast<const float4*>(sLse + st * BOX + 32 * half);
+        const float4* d4 = reinterpret_cast<const float4*>(sD + st * BOX + 32 * half);
         const F2 sc = {-p.scale2, -p.scale2}, minus = {-1.f, -1.f};
-        if ((pending && !write_grad(items - 1)) ||
-            (g >= 2 && !warp_wait(&p_empty[wg], ((g >> 1) - 1) & 1, p.err, abort_flag))) {
+        if ((j == 0 && items > 0 && !write_grad(items - 1)) ||
+            (g > 0 && !warp_wait(p_empty, (g - 1) & 1, p.err, abort_flag))) {
           ok = false;
           break;
         }
@@ -1160,22 +1146,17 @@ __global__ void __launch_bounds__(B_THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) pk[k] = dk[k] = 0u;
           }
-          if constexpr (KEYS) tmem_st8(tP(wg) + lane_off + 16 * half + 8 * c, pk);
-          tmem_st8(tP(wg) + lane_off + 32 + 16 * half + 8 * c, dk);
+          if constexpr (KEYS) tmem_st8(tP_own + 8 * c, pk);
+          tmem_st8(tDS_own + 8 * c, dk);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (lane == 0) mbar_arrive(p_full);
       }
-      // a warpgroup without a step of this item still owes the last one's gradients
-      if (!ok || (pending && !write_grad(items - 1))) {
-        ok = false;
-        break;
-      }
-      pending = true;
+      if (!ok) break;
     }
-    if (ok && pending) write_grad(items - 1);
+    if (ok && items > 0) write_grad(items - 1);
   }
   tc_fence_before();
   __syncthreads();
@@ -1211,7 +1192,7 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t W, uint64_t L, uin
   if (fn == nullptr) return false;
   cuuint64_t dims[3] = {W, L, B};
   cuuint64_t strides[2] = {ld * 2, sb * 2};
-  cuuint32_t box[3] = {64, HALF, 1};
+  cuuint32_t box[3] = {64, BOX, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1311,23 +1292,22 @@ cudaError_t bwd_hd(const WindowAttnArgs& a, cudaStream_t stream) {
   const int dev = device_index();
   const uint64_t W = static_cast<uint64_t>(a.H + 2 * a.G) * HD, D = static_cast<uint64_t>(a.H) * HD;
   const auto* base = static_cast<const __nv_bfloat16*>(a.qkv);
-  CUtensorMap tq, tkv, tdo, to, tlo;
+  CUtensorMap tq, tkv, tdo;
   if (!encode_rows(&tq, base + (a.Lk - a.Lq) * a.ld, W, a.Lq, a.B, a.ld, a.sb) ||
-      !encode_rows(&tkv, base, W, a.Lk, a.B, a.ld, a.sb) || !encode_rows(&tdo, a.dout, D, a.Lq, a.B, D, D * a.Lq) ||
-      !encode_rows(&to, a.out, D, a.Lq, a.B, D, D * a.Lq) || !encode_rows(&tlo, a.out_lo, D, a.Lq, a.B, D, D * a.Lq))
+      !encode_rows(&tkv, base, W, a.Lk, a.B, a.ld, a.sb) || !encode_rows(&tdo, a.dout, D, a.Lq, a.B, D, D * a.Lq))
     return cudaErrorInvalidValue;
-  cudaError_t e = allow_smem(window_bwd_kernel<HD, false>, b_smem(false), &ready_q[dev]);
-  if (e == cudaSuccess) e = allow_smem(window_bwd_kernel<HD, true>, b_smem(true), &ready_k[dev]);
+  cudaError_t e = allow_smem(window_bwd_kernel<HD, false>, B_SMEM, &ready_q[dev]);
+  if (e == cudaSuccess) e = allow_smem(window_bwd_kernel<HD, true>, B_SMEM, &ready_k[dev]);
   if (e != cudaSuccess) return e;
-  const int sms = num_sms(dev);
+  const long long most = 2LL * num_sms(dev);
   const int qtiles = (a.Lq + TILE - 1) / TILE + 1, ktiles = (a.Lk + TILE - 1) / TILE;
-  const int qgrid = grid_of(a.H, a.B, qtiles, sms), kgrid = grid_of(a.G, a.B, ktiles, sms);
+  const int qgrid = grid_of(a.H, a.B, qtiles, most), kgrid = grid_of(a.G, a.B, ktiles, most);
   // queries first: they leave D behind
-  window_bwd_kernel<HD, false><<<qgrid, B_THREADS, b_smem(false), stream>>>(tq, tkv, tdo, to, tlo,
+  window_bwd_kernel<HD, false><<<qgrid, B_THREADS, B_SMEM, stream>>>(tq, tkv, tdo,
                                                                            make_params(a, a.H, qtiles, qgrid));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  window_bwd_kernel<HD, true><<<kgrid, B_THREADS, b_smem(true), stream>>>(tq, tkv, tdo, to, tlo,
+  window_bwd_kernel<HD, true><<<kgrid, B_THREADS, B_SMEM, stream>>>(tq, tkv, tdo,
                                                                          make_params(a, a.G, ktiles, kgrid));
   return cudaGetLastError();
 }
