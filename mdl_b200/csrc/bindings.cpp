@@ -956,9 +956,9 @@ mdl::KvCache kv_cache_of(const at::Tensor& codes, const at::Tensor& scales, cons
   TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 5 && codes.size(2) == 2 && codes.is_contiguous(),
               "codes must be contiguous uint8 [pages, G, 2, page, hd / 2]");
   TORCH_CHECK(scales.scalar_type() == at::kBFloat16 && scales.is_contiguous() && scales.dim() == 4 &&
-                  scales.numel() * (codes.size(4)) == codes.numel() && scales.size(0) == codes.size(0) &&
-                  scales.size(1) == codes.size(1),
-              "scales must be contiguous bf16 [pages, G, 2, page]");
+                  scales.size(0) == codes.size(0) && scales.size(1) == codes.size(1) &&
+                  scales.size(2) == codes.size(3) && scales.size(3) == 2,
+              "scales must be contiguous bf16 [pages, G, page, 2]");
   TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous(), "table must be int32 [R, n]");
   TORCH_CHECK(lengths.scalar_type() == at::kInt && lengths.is_contiguous() && lengths.numel() == table.size(0),
               "lengths must be int32 [R]");

@@ -10,6 +10,8 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -47,54 +49,94 @@ __device__ __forceinline__ int page_of(const KvCache& c, int r, int p) {
   return -1;
 }
 
-// First slot row of (page, head, K|V): times hd / 2 in the codes, as it is in the scales.
+// Scales of K (low half) and V (high half) of position p in page pg, as one word.
+__device__ __forceinline__ long long scale_index(const KvCache& c, int pg, int g, int p) {
+  return ((static_cast<long long>(pg) * c.G + g) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
+}
+
+// First slot row of (page, head, K|V) in the codes, hd / 2 bytes each.
 __device__ __forceinline__ long long slot_base(const KvCache& c, int pg, int g, int kv) {
   return ((static_cast<long long>(pg) * c.G + g) * 2 + kv) << c.page_shift;
 }
 
 // ============================================================================ write
-// Eight lanes' worth of a row: hd / 8 lanes hold a row, 8 values each.
+// A lane holds 16 values of a row, hd / 16 lanes the row.
+//
+// c = rint(x / s) without a division: x / s of two bf16 numbers is either a tie (an odd
+// multiple of 1/2) or at least 1/1020 away from one, and |x / s| <= 7.03 (up to 8-bit
+// significands X, S: |X 2^e / S - (2k+1)/2| is a multiple of 1 / (2S), or of 1 / (4S) for the
+// tie 1/2). x * (1/s) + 1.5 * 2^12 rounds to a multiple of 2^-11, which moves it by 2^-12 at
+// most: ties become exact, nothing else reaches one. Adding 1.5 * 2^23 + 8 - 1.5 * 2^12 then
+// rounds to whole numbers, ties to even, and leaves c + 8 in the low bits. In the same way
+// top / 7 (8 bits over 7) stays 2^-12 of itself away from where bf16 rounding changes, so that a
+// multiplication by 1/7 gives the same s. Scales near the subnormal range take the division.
 template <int HD>
-__device__ __forceinline__ uint32_t quantise8(const uint4 x, uint16_t& scale_bits) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ uint2 quantise16(const uint4 x0, const uint4 x1, uint16_t& scale_bits) {
+  const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
   // |x| as 15-bit integers: ordered like the values, infinities and NaN on top
-  uint32_t top = 0;
+  uint32_t m = w[0] & 0x7FFF7FFFu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
+  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
 #pragma unroll
-  for (int o = 1; o < HD / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int o = 1; o < HD / 16; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const uint32_t top = max(m & 0xFFFFu, m >> 16);
+  const float largest = __uint_as_float(top << 16);
+  uint32_t word[2] = {0x88888888u, 0x88888888u};  // c = 0
   if (top >= 0x7F80u) {
     scale_bits = 0x7FFFu;  // NaN
-    return 0x88888888u;    // c = 0
-  }
-  const __nv_bfloat16 s16 = __float2bfloat16_rn(__uint_as_float(top << 16) / 7.f);
-  scale_bits = __bfloat16_as_ushort(s16);
-  const float s = __bfloat162float(s16);
-  if (s == 0.f) return 0x88888888u;
-  uint32_t word = 0;
+  } else if (top >= 0x0800u) {  // 2^-111
+    const __nv_bfloat16 s16 = __float2bfloat16_rn(largest * (1.f / 7.f));
+    scale_bits = __bfloat16_as_ushort(s16);
+    const float inv = __fdividef(1.f, __bfloat162float(s16));
+    constexpr float SNAP = 6144.f, ROUND = 12582912.f + 8.f - 6144.f;  // 1.5 * 2^12, to 1.5 * 2^23 + 8
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = (i & 1) ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]);
-    const int c = static_cast<int>(fminf(fmaxf(rintf(v / s), -7.f), 7.f));
-    word |= static_cast<uint32_t>(c + 8) << (4 * i);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t sum = 0;  // the exponent bits shifted in add up to a constant
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = w[4 * h + (i >> 1)];
+        const float v = (i & 1) ? bf16_hi(u) : bf16_lo(u);
+        sum += __float_as_uint(fmaf(v, inv, SNAP) + ROUND) << (4 * i);
+      }
+      constexpr uint32_t BASE = 0x4B400000u;  // 1.5 * 2^23
+      constexpr uint32_t CONST = BASE * 0x11111111u;
+      word[h] = sum - CONST;
+    }
+  } else {
+    const __nv_bfloat16 s16 = __float2bfloat16_rn(largest / 7.f);
+    scale_bits = __bfloat16_as_ushort(s16);
+    const float s = __bfloat162float(s16);
+    if (s > 0.f) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        word[h] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t u = w[4 * h + (i >> 1)];
+          const float v = (i & 1) ? bf16_hi(u) : bf16_lo(u);
+          const int c = static_cast<int>(fminf(fmaxf(rintf(v / s), -7.f), 7.f));
+          word[h] |= static_cast<uint32_t>(c + 8) << (4 * i);
+        }
+      }
+    }
   }
-  return word;
+  return make_uint2(word[0], word[1]);
 }
 
 // One block: a run of `chunk` tokens of one source row, every head, K and V. A unit = the row
-// of one token and head (hd / 8 lanes). Long runs number the units token-fastest, so that a
-// warp reads whole 32-byte sectors of 4 or 8 tokens and writes one dense run of a page;
-// single tokens number them head-fastest, so that a warp reads densely.
+// of one token and head (hd / 16 lanes). Long runs number the units token-fastest, so that a
+// warp reads whole sectors of neighbouring tokens and writes one dense run of a page; single
+// tokens number them head-fastest, so that a warp reads densely.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int chunk, int chunks) {
-  constexpr int LPU = HD / 8;
+  constexpr int LPU = HD / 16;
   const KvCache& c = a.c;
   const int i = blockIdx.x / chunks;
   const int r = row_of(c, a.rows, i);
   if (r < 0) return;
   const int cap = c.max_pages << c.page_shift;
   const int first = a.kstart != nullptr ? min(max(a.kstart[i], 0), a.T) : 0;
-  int start = a.start != nullptr ? a.start[i] : c.lengths[r];
+  const int start = a.start != nullptr ? a.start[i] : c.lengths[r];
   if (start < 0 || start > cap) {
     if (threadIdx.x == 0) record_error(c.err, MDL_ERR_BAD_INDEX);
     return;
@@ -103,35 +145,35 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int c
   const bool token_fast = nt >= 32 / LPU;
   const int units = nt * c.G;
   const int sub = threadIdx.x % LPU;
+  const __nv_bfloat16* kb = a.k + i * a.k_sb + sub * 16;
+  const __nv_bfloat16* vb = a.v + i * a.v_sb + sub * 16;
   for (int base = 0; base < units; base += kThreads / LPU) {  // whole warps stay together: shuffles below
     const int u = base + threadIdx.x / LPU;
     const bool live = u < units;
-    const int g = live ? (token_fast ? u / nt : u % c.G) : 0;
-    const int t = t0 + (live ? (token_fast ? u % nt : u / c.G) : 0);
+    const int q = token_fast ? u / nt : u / c.G, rem = u - q * (token_fast ? nt : c.G);
+    const int g = token_fast ? q : rem, t = t0 + (token_fast ? rem : q);
     const int pos = start + t - first;
     const bool in = live && t >= first;
-    uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+    uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
+    int pg = -1;
     if (in) {
-      kx = *reinterpret_cast<const uint4*>(a.k + i * a.k_sb + t * a.k_st + g * HD + sub * 8);
-      vx = *reinterpret_cast<const uint4*>(a.v + i * a.v_sb + t * a.v_st + g * HD + sub * 8);
+      const uint4* kp = reinterpret_cast<const uint4*>(kb + t * a.k_st + g * HD);
+      const uint4* vp = reinterpret_cast<const uint4*>(vb + t * a.v_st + g * HD);
+      k0 = kp[0];
+      k1 = kp[1];
+      v0 = vp[0];
+      v1 = vp[1];
+      if (pos >= cap) record_error(c.err, MDL_ERR_CAPACITY);
+      else pg = page_of(c, r, pos);
     }
     uint16_t ks, vs;
-    const uint32_t kc = quantise8<HD>(kx, ks), vc = quantise8<HD>(vx, vs);
-    if (!in) continue;
-    if (pos >= cap) {
-      record_error(c.err, MDL_ERR_CAPACITY);
-      continue;
-    }
-    const int pg = page_of(c, r, pos);
+    const uint2 kc = quantise16<HD>(k0, k1, ks), vc = quantise16<HD>(v0, v1, vs);
     if (pg < 0) continue;
-    const int slot = pos & ((1 << c.page_shift) - 1);
-    const long long bk = slot_base(c, pg, g, 0) + slot, bv = slot_base(c, pg, g, 1) + slot;
-    reinterpret_cast<uint32_t*>(c.codes)[bk * LPU + sub] = kc;
-    reinterpret_cast<uint32_t*>(c.codes)[bv * LPU + sub] = vc;
-    if (sub == 0) {
-      reinterpret_cast<uint16_t*>(c.scales)[bk] = ks;
-      reinterpret_cast<uint16_t*>(c.scales)[bv] = vs;
-    }
+    const long long bk = slot_base(c, pg, g, 0) + (pos & ((1 << c.page_shift) - 1));
+    const long long bv = bk + (1ll << c.page_shift);
+    reinterpret_cast<uint2*>(c.codes)[bk * LPU + sub] = kc;
+    reinterpret_cast<uint2*>(c.codes)[bv * LPU + sub] = vc;
+    if (sub == 0) reinterpret_cast<uint32_t*>(c.scales)[scale_index(c, pg, g, pos)] = ks | (static_cast<uint32_t>(vs) << 16);
   }
   // only the single block of a row may write the length that its threads read above
   if (chunks == 1) {
@@ -178,12 +220,12 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
       const int pg = page_of(c, r, static_cast<int>(pos));
       if (pg >= 0) {
         const int slot = static_cast<int>(pos) & ((1 << c.page_shift) - 1);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const long long b = slot_base(c, pg, g, kv) + slot;
-          w[kv] = reinterpret_cast<const uint32_t*>(c.codes)[b * LPU + sub];
-          s[kv] = __bfloat162float(c.scales[b]);
-        }
+        const long long b = slot_base(c, pg, g, 0) + slot;
+        w[0] = reinterpret_cast<const uint32_t*>(c.codes)[b * LPU + sub];
+        w[1] = reinterpret_cast<const uint32_t*>(c.codes)[(b + (1ll << c.page_shift)) * LPU + sub];
+        const uint32_t sc = reinterpret_cast<const uint32_t*>(c.scales)[scale_index(c, pg, g, static_cast<int>(pos))];
+        s[0] = bf16_lo(sc);
+        s[1] = bf16_hi(sc);
       }
     }
     const long long off = (static_cast<long long>(i) * a.count + t) * (c.G * HD) + g * HD + sub * 8;
@@ -226,9 +268,6 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 // operation), since the same shortcut over a long sum of keys would cancel. The scales enter
 // in fp32: s_k multiplies the scores, s_v the probabilities.
 //
-// Which key sits in which row of a 16-key tile is free as long as both products agree: lane
-// group g8 = lane / 4 owns 2 KT neighbouring keys of a step, so a lane's scales are one load
-// and its K rows neighbouring 32-byte sectors.
 constexpr uint32_t kMagic = 0x43004300u;   // bf16 128, twice
 constexpr uint32_t kOffset = 0x43084308u;  // bf16 136, twice
 
@@ -263,16 +302,60 @@ __device__ __forceinline__ void split_pairs(const uint4 v, uint32_t* p) {
   p[3] = __byte_perm(v.y, v.w, 0x7632);
 }
 
-template <int HD, int KT>
-struct Step {  // a lane's share of one step of 16 * KT keys
-  uint32_t k[2 * KT][HD / 32];  // its 2 KT keys, dims of lane % 4
-  uint32_t v[4 * KT];           // 4 KT keys of the other product, the word of its dims
-  uint32_t ks[KT], vs[KT];      // scales of its 2 KT keys (bf16 pairs)
+// Pairs of fp32: one instruction for two queries.
+struct F2 {
+  float x, y;
 };
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// Blocks an SM that the registers have to allow: the kernel hides its latencies with warps.
+template <int HD, int NT, int WPI>
+constexpr int min_blocks() {
+  return WPI == 1 ? (NT == 4 ? (HD == 64 ? 2 : 3) : (HD == 64 && NT == 2 ? 3 : 4)) : (NT == 1 ? 2 : 1);
+}
+template <int NT>
+constexpr int tiles_a_step() { return NT == 1 ? 4 : 2; }
+// Shared memory: a warp's ring of steps (K codes | V codes | scales), then their barriers; the
+// join of eight warps takes the same space afterwards.
+template <int HD, int NT>
+constexpr int step_bytes() { return 16 * tiles_a_step<NT>() * (HD + 4); }
+template <int HD>
+constexpr int ring_steps() { return HD == 64 ? 3 : 4; }
+template <int HD, int NT, int WPI>
+constexpr int attend_smem() {
+  constexpr int warps = WPI == 1 ? 4 : WPI;
+  constexpr int ring = warps * ring_steps<HD>() * (step_bytes<HD, NT>() + 8);
+  constexpr int join = WPI == 1 ? 0 : WPI * 8 * NT * (HD + 6) * 4;
+  return ring > join ? ring : join;
+}
+
+// Bulk copy into this CTA's shared memory, 16-byte aligned, counted on `bar`.
+__device__ __forceinline__ void bulk_copy(uint8_t* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 
 template <int HD, int NT, int WPI>
-__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(KvAttendArgs a, int qblocks, int splits) {
-  constexpr int KT = NT == 4 ? 2 : 4;   // 16-key tiles a step
+__global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, WPI>())
+    kv_attend_kernel(KvAttendArgs a, int qblocks, int splits) {
+  constexpr int KT = tiles_a_step<NT>();  // 16-key tiles a step
   constexpr int CH = 16 * KT;
   constexpr int KW = HD / 32;           // code words of a key a lane
   constexpr int KS = HD / 16;           // k steps of the score product
@@ -307,7 +390,6 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
   // ---- queries: B operand (column g8 of each tile), and sum(q) of columns 2t, 2t + 1
   uint32_t qf[NT][KS][2];
   float init[NT][2];
-  int qn[NT][2];  // query index n of columns 2t, 2t + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int m = min(m0 + nt * 8 + g8, M - 1);
@@ -329,10 +411,11 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       init[nt][e] = -136.f * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
-      qn[nt][e] = min(m0 + nt * 8 + 2 * t + e, M - 1) / group;
     }
   }
   const float scale2 = a.scale * 1.4426950408889634f;
+  // query of columns 2t + e of a tile (only where a mask is needed)
+  auto query_of = [&](int nt, int e) { return min(m0 + nt * 8 + 2 * t + e, M - 1) / group; };
 
   float o[MT][NT][4];
   float mx[NT][2], l[NT][2];
@@ -383,66 +466,96 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
     total = cs + end - cw;
   }
   auto step_key = [&](int i) { return (i < cs ? i : cw + i - cs) * CH; };
-  // page of the lane's K keys and of its V keys; 0 (any valid page) past the length
-  auto pages = [&](int i, int& pk, int& pv) {
+  // Row rho of a 16-key tile is key (rho >> 1 & 3) + 4 (rho & 1) + (rho & 8): the second product
+  // then reads four neighbouring keys at once, without bank conflicts. The lane's rows: g8, + 8.
+  const int row8 = (g8 >> 1) + 4 * (g8 & 1);
+  // A ring of steps in shared memory, filled by bulk copies: enough bytes under way to cover
+  // the memory latency without registers for them.
+  constexpr int RING = ring_steps<HD>(), STEP = step_bytes<HD, NT>(), TILE_CODES = 16 * HD / 2;
+  extern __shared__ __align__(128) uint8_t sm_ring[];
+  constexpr int WARPS = WPI == 1 ? 4 : WPI;
+  uint8_t* ring = sm_ring + warp * RING * STEP;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ring + WARPS * RING * STEP) + warp * RING;
+  if (lane == 0) {
+    for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  // Page of each 16-key tile of a step, read a step before its copies are issued; one where a
+  // page holds the whole step.
+  const bool one_page = (1 << c.page_shift) >= CH;
+  int pg[KT];
+  auto pages = [&](int i) {
+    if (i >= total) return;
     const int k0 = step_key(i);
-    const int a0 = k0 + 2 * KT * g8, a1 = k0 + 4 * KT * t;
-    pk = a0 < len ? max(page_of(c, r, a0), 0) : 0;
-    pv = a1 < len ? max(page_of(c, r, a1), 0) : 0;
-  };
-  auto load = [&](int i, int pk, int pv, Step<HD, KT>& s) {
-    const int mask = (1 << c.page_shift) - 1;
-    const int k0 = step_key(i);
-    const int slot = (k0 + 2 * KT * g8) & mask;
-    const long long bk = slot_base(c, pk, g, 0) + slot;
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(c.codes) + bk * (HD / 8) + t * KW;
+    pg[0] = max(page_of(c, r, k0), 0);  // k0 < len
+    if (!one_page) {
 #pragma unroll
-    for (int e = 0; e < 2 * KT; ++e) {
-      if constexpr (KW == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp + e * (HD / 8));
-        s.k[e][0] = x.x;
-        s.k[e][1] = x.y;
+      for (int j = 1; j < KT; ++j) pg[j] = k0 + 16 * j < len ? max(page_of(c, r, k0 + 16 * j), 0) : 0;
+    }
+  };
+  const int slot_mask = (1 << c.page_shift) - 1;
+  auto fetch = [&](int i, int st) {
+    if (i < total && lane == 0) {
+      const int k0 = step_key(i), slot = k0 & slot_mask;
+      uint8_t* dst = ring + st * STEP;
+      if (one_page) {
+        mbar_arrive_expect_tx(&full[st], STEP);
+        const long long row = slot_base(c, pg[0], g, 0) + slot;
+        bulk_copy(dst, c.codes + row * (HD / 2), KT * TILE_CODES, &full[st]);
+        bulk_copy(dst + KT * TILE_CODES, c.codes + (row + slot_mask + 1) * (HD / 2), KT * TILE_CODES, &full[st]);
+        bulk_copy(dst + 2 * KT * TILE_CODES, c.scales + 2 * scale_index(c, pg[0], g, slot), CH * 4, &full[st]);
       } else {
-        s.k[e][0] = kp[e * (HD / 8)];
+        const int tiles = min(KT, (len - k0 + 15) / 16);  // the rest is masked, whatever lies there
+        mbar_arrive_expect_tx(&full[st], tiles * (2 * TILE_CODES + 64));
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          if (j >= tiles) break;
+          const int sj = (slot + 16 * j) & slot_mask;
+          const long long row = slot_base(c, pg[j], g, 0) + sj;
+          bulk_copy(dst + j * TILE_CODES, c.codes + row * (HD / 2), TILE_CODES, &full[st]);
+          bulk_copy(dst + (KT + j) * TILE_CODES, c.codes + (row + slot_mask + 1) * (HD / 2), TILE_CODES, &full[st]);
+          bulk_copy(dst + 2 * KT * TILE_CODES + 64 * j, c.scales + 2 * scale_index(c, pg[j], g, sj), 64, &full[st]);
+        }
       }
     }
-    const __nv_bfloat16* sp = c.scales + bk;
-    const __nv_bfloat16* sv = sp + (1 << c.page_shift);  // V follows K
-    if constexpr (KT == 4) {
-      const uint4 x = *reinterpret_cast<const uint4*>(sp), y = *reinterpret_cast<const uint4*>(sv);
-      s.ks[0] = x.x; s.ks[1] = x.y; s.ks[2] = x.z; s.ks[3] = x.w;
-      s.vs[0] = y.x; s.vs[1] = y.y; s.vs[2] = y.z; s.vs[3] = y.w;
-    } else {
-      const uint2 x = *reinterpret_cast<const uint2*>(sp), y = *reinterpret_cast<const uint2*>(sv);
-      s.ks[0] = x.x; s.ks[1] = x.y;
-      s.vs[0] = y.x; s.vs[1] = y.y;
-    }
-    const long long bv = slot_base(c, pv, g, 1) + ((k0 + 4 * KT * t) & mask);
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(c.codes) + bv * (HD / 8) + (HD == 64 ? g8 : g8 >> 1);
-#pragma unroll
-    for (int e = 0; e < 4 * KT; ++e) s.v[e] = vp[e * (HD / 8)];
+    __syncwarp();
   };
-
-  Step<HD, KT> cur;
-  int pk = 0, pv = 0;
-  if (part < total) {
-    pages(part, pk, pv);
-    load(part, pk, pv, cur);
-    if (part + parts < total) pages(part + parts, pk, pv);
+#pragma unroll 1
+  for (int s = 0; s < RING; ++s) {
+    pages(part + s * parts);
+    fetch(part + s * parts, s);
   }
+  pages(part + RING * parts);
+  int st = 0, phase = 0;
   for (int i = part; i < total; i += parts) {
-    const Step<HD, KT> s = cur;
-    if (i + parts < total) {
-      load(i + parts, pk, pv, cur);
-      if (i + 2 * parts < total) pages(i + 2 * parts, pk, pv);
-    }
     const int k0 = step_key(i);
-    float x[KT][NT][4];
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, c.err, nullptr))) break;
+    const uint8_t* sk = ring + st * STEP;
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(sk) + row8 * (HD / 8) + t * KW;
+    const uint32_t* vw = reinterpret_cast<const uint32_t*>(sk + KT * TILE_CODES) + t * (HD / 8) + (HD == 64 ? g8 : g8 >> 1);
+    const uint32_t* scw = reinterpret_cast<const uint32_t*>(sk + 2 * KT * TILE_CODES) + row8;
+    F2 x[KT][NT][2];  // scores: [tile][queries][row g8 or g8 + 8], columns 2t and 2t + 1
+    uint32_t vs[2 * KT];
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
+      float d[NT][4];
+      uint32_t wk[2][KW];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t* src = kw + (16 * j + 8 * h) * (HD / 8);
+        if constexpr (KW == 2) {
+          const uint2 y = *reinterpret_cast<const uint2*>(src);
+          wk[h][0] = y.x;
+          wk[h][1] = y.y;
+        } else {
+          wk[h][0] = *src;
+        }
+        vs[2 * j + h] = scw[16 * j + 8 * h];
+      }
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t wa = s.k[2 * j][w], wb = s.k[2 * j + 1][w];
+        const uint32_t wa = wk[0][w], wb = wk[1][w];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t a0 = code_pair(wa >> (8 * h)), a1 = code_pair(wb >> (8 * h));
@@ -451,102 +564,119 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
           for (int nt = 0; nt < NT; ++nt) {
             const int ks = 2 * w + h;
             if (ks == 0)
-              mma16816(x[j][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], init[nt][0], init[nt][1], init[nt][0],
+              mma16816(d[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], init[nt][0], init[nt][1], init[nt][0],
                        init[nt][1]);
             else
-              mma16816(x[j][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], x[j][nt][0], x[j][nt][1], x[j][nt][2],
-                       x[j][nt][3]);
+              mma16816(d[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], d[nt][0], d[nt][1], d[nt][2], d[nt][3]);
           }
         }
       }
-      const float s0 = bf16_lo(s.ks[j]) * scale2, s1 = bf16_hi(s.ks[j]) * scale2;
+      const float s0 = bf16_lo(vs[2 * j]) * scale2, s1 = bf16_lo(vs[2 * j + 1]) * scale2;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        x[j][nt][0] *= s0;
-        x[j][nt][1] *= s0;
-        x[j][nt][2] *= s1;
-        x[j][nt][3] *= s1;
+        x[j][nt][0] = mul2({d[nt][0], d[nt][1]}, {s0, s0});
+        x[j][nt][1] = mul2({d[nt][2], d[nt][3]}, {s1, s1});
       }
     }
     // every key of the step visible to every query of the block?
     const bool whole = k0 + CH <= min(len, qmin + 1) && (W == 0 || k0 > qmax - W || k0 + CH <= S);
     if (!whole) {
 #pragma unroll
-      for (int j = 0; j < KT; ++j)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
+          const int qp = base + query_of(nt, e);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kp = k0 + 2 * KT * g8 + 2 * j + (e >> 1);
-            const int qp = base + qn[nt][e & 1];
-            const bool vis = kp < len && kp <= qp && (W == 0 || qp - kp < W || kp < S);
-            if (!vis) x[j][nt][e] = -CUDART_INF_F;
-          }
+          for (int j = 0; j < KT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int kp = k0 + 16 * j + 8 * h + row8;
+              const bool vis = kp < len && kp <= qp && (W == 0 || qp - kp < W || kp < S);
+              float& y = e ? x[j][nt][h].y : x[j][nt][h].x;
+              if (!vis) y = -CUDART_INF_F;
+            }
+        }
     }
     float lm[NT][2];
     bool grow = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      lm[nt][0] = fmaxf(x[0][nt][0].x, x[0][nt][1].x);
+      lm[nt][1] = fmaxf(x[0][nt][0].y, x[0][nt][1].y);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = -CUDART_INF_F;
-#pragma unroll
-        for (int j = 0; j < KT; ++j) v = fmaxf(v, fmaxf(x[j][nt][e], x[j][nt][e + 2]));
-        lm[nt][e] = v;
-        grow |= v > mx[nt][e] + 8.f;
+      for (int j = 1; j < KT; ++j) {
+        lm[nt][0] = fmaxf(lm[nt][0], fmaxf(x[j][nt][0].x, x[j][nt][1].x));
+        lm[nt][1] = fmaxf(lm[nt][1], fmaxf(x[j][nt][0].y, x[j][nt][1].y));
       }
+      grow |= lm[nt][0] > mx[nt][0] + 8.f || lm[nt][1] > mx[nt][1] + 8.f;
+    }
     if (__any_sync(0xffffffffu, grow)) raise(lm);
-    float use[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) use[nt][e] = mx[nt][e] == -CUDART_INF_F ? 0.f : mx[nt][e];
-#pragma unroll
-    for (int j = 0; j < KT; ++j) {
-      uint32_t pb[NT][2];
-      const float v0 = bf16_lo(s.vs[j]), v1 = bf16_hi(s.vs[j]);
+    // P (times the scale of V) as the B operand of the second product
+    uint32_t pb[KT][NT][2];
+    auto weigh = [&](auto masked) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = x[j][nt][e];
-          p[e] = ex2(y - use[nt][e & 1]);
-          l[nt][e & 1] += p[e];
-          p[e] *= e < 2 ? v0 : v1;
-          // the scale of a hidden key may be anything, a NaN too
-          if (!whole && y == -CUDART_INF_F) p[e] = 0.f;
+        F2 use = {-mx[nt][0], -mx[nt][1]}, sum = {l[nt][0], l[nt][1]};
+        if constexpr (decltype(masked)::value) {
+          if (mx[nt][0] == -CUDART_INF_F) use.x = 0.f;
+          if (mx[nt][1] == -CUDART_INF_F) use.y = 0.f;
         }
-        pb[nt][0] = transpose8(pack_bf16(p[0], p[1]));
-        pb[nt][1] = transpose8(pack_bf16(p[2], p[3]));
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float v = bf16_hi(vs[2 * j + h]);
+            const F2 y = add2(x[j][nt][h], use);
+            F2 e = {ex2(y.x), ex2(y.y)};
+            sum = add2(sum, e);
+            e = mul2(e, {v, v});
+            if constexpr (decltype(masked)::value) {  // the scale of a hidden key may be a NaN
+              if (y.x == -CUDART_INF_F) e.x = 0.f;
+              if (y.y == -CUDART_INF_F) e.y = 0.f;
+            }
+            pb[j][nt][h] = transpose8(pack_bf16(e.x, e.y));
+          }
+        l[nt][0] = sum.x;
+        l[nt][1] = sum.y;
       }
-      // keys in tile rows 2t, 2t+1, 2t+8, 2t+9
-      const uint32_t va = s.v[2 * j], vb = s.v[2 * KT + 2 * j], vc = s.v[2 * j + 1], vd = s.v[2 * KT + 2 * j + 1];
+    };
+    if (whole) weigh(std::false_type{});
+    else weigh(std::true_type{});
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      // rows 2t, 2t + 1, 2t + 8, 2t + 9 of the tile: keys t, t + 4, t + 8, t + 12
+      const uint32_t va = vw[16 * j * (HD / 8)], vb = vw[(16 * j + 4) * (HD / 8)];
+      const uint32_t vc = vw[(16 * j + 8) * (HD / 8)], vd = vw[(16 * j + 12) * (HD / 8)];
+      uint32_t u0, u1, u2, u3;
       if constexpr (HD == 64) {
-        const uint32_t lo0 = __byte_perm(va, vb, 0x5410), hi0 = __byte_perm(va, vb, 0x7632);
-        const uint32_t lo1 = __byte_perm(vc, vd, 0x5410), hi1 = __byte_perm(vc, vd, 0x7632);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint32_t a0 = code_pair_signed(lo0 >> (4 * mt)), a1 = code_pair_signed(hi0 >> (4 * mt));
-          const uint32_t a2 = code_pair_signed(lo1 >> (4 * mt)), a3 = code_pair_signed(hi1 >> (4 * mt));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1], o[mt][nt][0], o[mt][nt][1], o[mt][nt][2],
-                     o[mt][nt][3]);
-        }
+        u0 = __byte_perm(va, vb, 0x5410);
+        u1 = __byte_perm(va, vb, 0x7632);
+        u2 = __byte_perm(vc, vd, 0x5410);
+        u3 = __byte_perm(vc, vd, 0x7632);
       } else {
         const uint32_t sel = (g8 & 1) ? 0x7632 : 0x5410;
-        const uint32_t u0 = __byte_perm(va, vb, sel), u1 = __byte_perm(vc, vd, sel);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint32_t a0 = code_pair_signed(u0 >> (8 * mt)), a1 = code_pair_signed(u0 >> (8 * mt + 4));
-          const uint32_t a2 = code_pair_signed(u1 >> (8 * mt)), a3 = code_pair_signed(u1 >> (8 * mt + 4));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            mma16816(o[mt][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1], o[mt][nt][0], o[mt][nt][1], o[mt][nt][2],
-                     o[mt][nt][3]);
-        }
+        u0 = __byte_perm(va, vb, sel);
+        u2 = __byte_perm(vc, vd, sel);
+        u1 = u0 >> 4;
+        u3 = u2 >> 4;
       }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        constexpr int STEP = HD == 64 ? 4 : 8;
+        const uint32_t a0 = code_pair_signed(u0 >> (STEP * mt)), a1 = code_pair_signed(u1 >> (STEP * mt));
+        const uint32_t a2 = code_pair_signed(u2 >> (STEP * mt)), a3 = code_pair_signed(u3 >> (STEP * mt));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma16816(o[mt][nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1], o[mt][nt][0], o[mt][nt][1], o[mt][nt][2],
+                   o[mt][nt][3]);
+      }
+    }
+    __syncwarp();  // the warp has read the stage
+    fetch(i + RING * parts, st);
+    pages(i + (RING + 1) * parts);
+    if (++st == RING) {
+      st = 0;
+      phase ^= 1;
     }
   }
 
@@ -583,7 +713,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int kp = k0 + g8 + 8 * (e >> 1), n = qn[nt][e & 1];
+          const int kp = k0 + g8 + 8 * (e >> 1), n = query_of(nt, e & 1);
           const bool vis = kp <= n && (W == 0 || n - kp < W || len + kp < S);
           x[nt][e] = vis ? x[nt][e] * scale2 : -CUDART_INF_F;
         }
@@ -696,7 +826,8 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI) kv_attend_kernel(Kv
       }
   } else {
     // join the warps: per column the common maximum, then the weighted sums
-    extern __shared__ float sm[];
+    __syncthreads();  // every warp is through with its ring
+    float* sm = reinterpret_cast<float*>(sm_ring);
     float* so = sm;                              // [WPI][COLS][HD + 4]
     float* smx = sm + WPI * COLS * (HD + 4);     // [WPI][COLS]
     float* sl = smx + WPI * COLS;                // [WPI][COLS]
@@ -786,11 +917,22 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(KvAttendArgs a, int qbl
       make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
+constexpr int kMaxDevices = 64;
+
+int device_index() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices ? dev : 0;
+}
+
 int num_sms() {
-  int dev = 0, n = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
+  static std::atomic<int> n[kMaxDevices];
+  const int dev = device_index();
+  int v = n[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) return 148;
+    n[dev].store(v, std::memory_order_relaxed);
+  }
+  return v;
 }
 
 struct Plan {
@@ -809,32 +951,46 @@ Plan plan_of(const KvAttendArgs& a) {
   p.items = static_cast<long long>(a.B) * a.c.G * p.qblocks;
   const long long cap = static_cast<long long>(a.c.max_pages) << a.c.page_shift;
   const long long keys = a.window > 0 ? std::min<long long>(cap, static_cast<long long>(a.window) + a.sinks) : cap;
-  static const int sms = num_sms();
+  const int sms = num_sms();
   p.wpi = (p.items >= 16LL * sms && keys <= 4096) ? 1 : 8;
   p.splits = 1;
   if (p.wpi == 8) {
-    const long long want = (2LL * sms + p.items - 1) / p.items;
-    const long long most = std::max<long long>(1, keys / (8 * 64));
-    p.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({want, most, 64})));
+    // the least (waves of blocks) x (keys a block + what a block costs besides, as keys)
+    const long long slots = 2LL * sms, most = std::min<long long>(32, std::max<long long>(1, keys / 512));
+    double best = 0;
+    for (int n = 1; n <= most; ++n) {
+      const double cost = static_cast<double>((p.items * n + slots - 1) / slots) * (static_cast<double>(keys) / n + 1024);
+      if (n == 1 || cost < 0.98 * best) {
+        best = cost;
+        p.splits = n;
+      }
+    }
   }
   return p;
 }
 
+template <int HD, int NT, int WPI>
+cudaError_t launch_wpi(const KvAttendArgs& a, const Plan& p, cudaStream_t stream) {
+  constexpr int smem = attend_smem<HD, NT, WPI>();
+  static std::atomic<bool> ready[kMaxDevices];
+  if (smem > 48 * 1024) {
+    std::atomic<bool>& done = ready[device_index()];
+    if (!done.load(std::memory_order_relaxed)) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(kv_attend_kernel<HD, NT, WPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+      done.store(true, std::memory_order_relaxed);
+    }
+  }
+  const long long blocks = WPI == 1 ? (p.items + 3) / 4 : p.items * p.splits;
+  kv_attend_kernel<HD, NT, WPI>
+      <<<static_cast<unsigned>(blocks), WPI == 1 ? 128 : 32 * WPI, smem, stream>>>(a, p.qblocks, p.splits);
+  return cudaGetLastError();
+}
+
 template <int HD, int NT>
 cudaError_t launch_attend(const KvAttendArgs& a, const Plan& p, cudaStream_t stream) {
-  if (p.wpi == 1) {
-    kv_attend_kernel<HD, NT, 1><<<static_cast<unsigned>((p.items + 3) / 4), 128, 0, stream>>>(a, p.qblocks, 1);
-  } else {
-    constexpr int smem = 8 * 8 * NT * (HD + 6) * 4;
-    if constexpr (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<HD, NT, 8>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return e;
-    }
-    kv_attend_kernel<HD, NT, 8>
-        <<<static_cast<unsigned>(p.items * p.splits), 256, smem, stream>>>(a, p.qblocks, p.splits);
-  }
-  return cudaGetLastError();
+  return p.wpi == 1 ? launch_wpi<HD, NT, 1>(a, p, stream) : launch_wpi<HD, NT, 8>(a, p, stream);
 }
 
 template <int HD>

@@ -9,7 +9,7 @@ namespace mdl {
 // The cache. Row r's token at position p lives in page table[r, p / page], slot p % page:
 //   codes  [num_pages, G, 2, page, hd / 2] uint8: K (0) and V (1); element 2i of a head's row in
 //          the low half of byte i, element 2i + 1 in the high half, each c + 8 for c = -7 .. 7
-//   scales [num_pages, G, 2, page] bf16: one a token, head and K|V; the value is scale * c
+//   scales [num_pages, G, page, 2] bf16: one a token, head and K|V; the value is scale * c
 // page is a power of two of at least 16, hd is 32 or 64.
 struct KvCache {
   uint8_t* codes = nullptr;

@@ -76,7 +76,7 @@ class QuantizedKVCache:
         self.table = table
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
         self.codes = torch.empty(num_pages, kv_heads, 2, page, head_dim // 2, dtype=torch.uint8, device=device)
-        self.scales = torch.empty(num_pages, kv_heads, 2, page, dtype=torch.bfloat16, device=device)
+        self.scales = torch.empty(num_pages, kv_heads, page, 2, dtype=torch.bfloat16, device=device)
 
     @property
     def capacity(self) -> int:
@@ -111,7 +111,7 @@ class QuantizedKVCache:
         pg, slot = self._slots(rows, pos)
         n = self.codes[pg, :, :, slot]
         c = torch.stack([n & 15, n >> 4], -1).flatten(-2).float() - 8.0
-        return c * self.scales[pg, :, :, slot].float().unsqueeze(-1)
+        return c * self.scales[pg, :, slot].float().unsqueeze(-1)
 
 
 # ----------------------------------------------------------------------------- checks
@@ -190,7 +190,7 @@ def kv_cache_write_reference(cache: QuantizedKVCache, k, v, start=None, kstart=N
     i, ti = live.nonzero(as_tuple=True)
     pg, slot = cache._slots(r[i], pos[i, ti])
     cache.codes[pg, :, :, slot] = packed[i, ti]
-    cache.scales[pg, :, :, slot] = s.transpose(2, 3)[i, ti]
+    cache.scales[pg, :, slot] = s.transpose(2, 3)[i, ti]
     cache.lengths[r] = (begin + T - first).to(torch.int32)
 
 
