@@ -271,10 +271,16 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 constexpr uint32_t kMagic = 0x43004300u;   // bf16 128, twice
 constexpr uint32_t kOffset = 0x43084308u;  // bf16 136, twice
 
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) { return (w & 0x000F000Fu) | kMagic; }
+// (w & 0x000F000F) | magic in one instruction: it takes one immediate, so the magic number has to
+// sit in a register (`magic`, which the compiler does not see through).
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(d) : "r"(w), "r"(magic));
+  return d;
+}
 
-__device__ __forceinline__ uint32_t code_pair_signed(uint32_t w) {
-  const uint32_t u = code_pair(w), o = kOffset;
+__device__ __forceinline__ uint32_t code_pair_signed(uint32_t w, uint32_t magic) {
+  const uint32_t u = code_pair(w, magic), o = kOffset;
   const __nv_bfloat162 r =
       __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&o));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -302,24 +308,9 @@ __device__ __forceinline__ void split_pairs(const uint4 v, uint32_t* p) {
   p[3] = __byte_perm(v.y, v.w, 0x7632);
 }
 
-// Pairs of fp32: one instruction for two queries.
-struct F2 {
-  float x, y;
-};
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -350,6 +341,11 @@ __device__ __forceinline__ void bulk_copy(uint8_t* dst, const void* src, uint32_
                    smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+
+// The rest of a wait that is not over at once; the same outcome on every lane.
+__device__ __noinline__ bool ring_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, nullptr));
 }
 
 template <int HD, int NT, int WPI>
@@ -389,7 +385,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
 
   // ---- queries: B operand (column g8 of each tile), and sum(q) of columns 2t, 2t + 1
   uint32_t qf[NT][KS][2];
-  float init[NT][2];
+  float init[NT][4];  // a whole operand: building it for each product would cost four moves
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int m = min(m0 + nt * 8 + g8, M - 1);
@@ -410,10 +406,12 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      init[nt][e] = -136.f * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+      init[nt][e] = init[nt][e + 2] = -136.f * __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
     }
   }
   const float scale2 = a.scale * 1.4426950408889634f;
+  uint32_t magic;
+  asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(kMagic));
   // query of columns 2t + e of a tile (only where a mask is needed)
   auto query_of = [&](int nt, int e) { return min(m0 + nt * 8 + 2 * t + e, M - 1) / group; };
 
@@ -482,40 +480,56 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   }
   __syncwarp();
   // Page of each 16-key tile of a step, read a step before its copies are issued; one where a
-  // page holds the whole step.
+  // page holds the whole step. The addresses are kept short: what a step costs besides its keys
+  // is a fifth of its instructions.
   const bool one_page = (1 << c.page_shift) >= CH;
+  const int slot_mask = (1 << c.page_shift) - 1;
+  const int* table = c.table + static_cast<long long>(r < 0 ? 0 : r) * c.max_pages;
+  const uint8_t* codes_g = c.codes + (slot_base(c, 0, g, 0) * (HD / 2));
+  const uint8_t* scales_g = reinterpret_cast<const uint8_t*>(c.scales) + 4 * scale_index(c, 0, g, 0);
+  const uint32_t v_off = (slot_mask + 1) * (HD / 2), sc_page = c.G << (c.page_shift + 2);
+  const long long code_page = static_cast<long long>(c.G) * 2 * v_off;
   int pg[KT];
+  auto page_at = [&](int k0) {
+    const int q = __ldg(table + (k0 >> c.page_shift));
+    if (static_cast<unsigned>(q) < static_cast<unsigned>(c.num_pages)) return q;
+    record_error(c.err, MDL_ERR_BAD_INDEX);
+    return 0;
+  };
   auto pages = [&](int i) {
     if (i >= total) return;
     const int k0 = step_key(i);
-    pg[0] = max(page_of(c, r, k0), 0);  // k0 < len
+    pg[0] = page_at(k0);  // k0 < len
     if (!one_page) {
 #pragma unroll
-      for (int j = 1; j < KT; ++j) pg[j] = k0 + 16 * j < len ? max(page_of(c, r, k0 + 16 * j), 0) : 0;
+      for (int j = 1; j < KT; ++j) pg[j] = k0 + 16 * j < len ? page_at(k0 + 16 * j) : 0;
     }
   };
-  const int slot_mask = (1 << c.page_shift) - 1;
   auto fetch = [&](int i, int st) {
     if (i < total && lane == 0) {
-      const int k0 = step_key(i), slot = k0 & slot_mask;
+      const int k0 = step_key(i);
       uint8_t* dst = ring + st * STEP;
       if (one_page) {
+        const uint32_t slot = k0 & slot_mask;
+        const uint8_t* kp = codes_g + pg[0] * code_page + slot * (HD / 2);
         mbar_arrive_expect_tx(&full[st], STEP);
-        const long long row = slot_base(c, pg[0], g, 0) + slot;
-        bulk_copy(dst, c.codes + row * (HD / 2), KT * TILE_CODES, &full[st]);
-        bulk_copy(dst + KT * TILE_CODES, c.codes + (row + slot_mask + 1) * (HD / 2), KT * TILE_CODES, &full[st]);
-        bulk_copy(dst + 2 * KT * TILE_CODES, c.scales + 2 * scale_index(c, pg[0], g, slot), CH * 4, &full[st]);
+        bulk_copy(dst, kp, KT * TILE_CODES, &full[st]);
+        bulk_copy(dst + KT * TILE_CODES, kp + v_off, KT * TILE_CODES, &full[st]);
+        bulk_copy(dst + 2 * KT * TILE_CODES, scales_g + static_cast<long long>(pg[0]) * sc_page + slot * 4, CH * 4,
+                  &full[st]);
       } else {
         const int tiles = min(KT, (len - k0 + 15) / 16);  // the rest is masked, whatever lies there
         mbar_arrive_expect_tx(&full[st], tiles * (2 * TILE_CODES + 64));
+        for (int j = 0; j < tiles; ++j) {
+          int page = pg[0];
 #pragma unroll
-        for (int j = 0; j < KT; ++j) {
-          if (j >= tiles) break;
-          const int sj = (slot + 16 * j) & slot_mask;
-          const long long row = slot_base(c, pg[j], g, 0) + sj;
-          bulk_copy(dst + j * TILE_CODES, c.codes + row * (HD / 2), TILE_CODES, &full[st]);
-          bulk_copy(dst + (KT + j) * TILE_CODES, c.codes + (row + slot_mask + 1) * (HD / 2), TILE_CODES, &full[st]);
-          bulk_copy(dst + 2 * KT * TILE_CODES + 64 * j, c.scales + 2 * scale_index(c, pg[j], g, sj), 64, &full[st]);
+          for (int e = 1; e < KT; ++e) page = j == e ? pg[e] : page;
+          const uint32_t slot = (k0 + 16 * j) & slot_mask;
+          const uint8_t* kp = codes_g + page * code_page + slot * (HD / 2);
+          bulk_copy(dst + j * TILE_CODES, kp, TILE_CODES, &full[st]);
+          bulk_copy(dst + (KT + j) * TILE_CODES, kp + v_off, TILE_CODES, &full[st]);
+          bulk_copy(dst + 2 * KT * TILE_CODES + 64 * j, scales_g + static_cast<long long>(page) * sc_page + slot * 4, 64,
+                    &full[st]);
         }
       }
     }
@@ -527,19 +541,22 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     fetch(part + s * parts, s);
   }
   pages(part + RING * parts);
-  int st = 0, phase = 0;
+  // steps from all_lo + 1 (or up to S) to all_hi are visible to every query of the block
+  const int all_hi = min(len, qmin + 1) - CH, all_lo = W > 0 ? qmax - W : -1, all_sink = S - CH;
+  int st = 0;
+  uint32_t phase = 0;
+#pragma unroll 1
   for (int i = part; i < total; i += parts) {
     const int k0 = step_key(i);
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], phase, c.err, nullptr))) break;
+    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], phase)) && !ring_wait(&full[st], phase, c.err)) break;
     const uint8_t* sk = ring + st * STEP;
     const uint32_t* kw = reinterpret_cast<const uint32_t*>(sk) + row8 * (HD / 8) + t * KW;
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(sk + KT * TILE_CODES) + t * (HD / 8) + (HD == 64 ? g8 : g8 >> 1);
     const uint32_t* scw = reinterpret_cast<const uint32_t*>(sk + 2 * KT * TILE_CODES) + row8;
-    F2 x[KT][NT][2];  // scores: [tile][queries][row g8 or g8 + 8], columns 2t and 2t + 1
+    float x[KT][NT][4];  // scores: rows g8 (0, 1) and g8 + 8 (2, 3), columns 2t and 2t + 1
     uint32_t vs[2 * KT];
 #pragma unroll
     for (int j = 0; j < KT; ++j) {
-      float d[NT][4];
       uint32_t wk[2][KW];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -558,28 +575,31 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
         const uint32_t wa = wk[0][w], wb = wk[1][w];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t a0 = code_pair(wa >> (8 * h)), a1 = code_pair(wb >> (8 * h));
-          const uint32_t a2 = code_pair(wa >> (8 * h + 4)), a3 = code_pair(wb >> (8 * h + 4));
+          const uint32_t a0 = code_pair(wa >> (8 * h), magic), a1 = code_pair(wb >> (8 * h), magic);
+          const uint32_t a2 = code_pair(wa >> (8 * h + 4), magic), a3 = code_pair(wb >> (8 * h + 4), magic);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const int ks = 2 * w + h;
             if (ks == 0)
-              mma16816(d[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], init[nt][0], init[nt][1], init[nt][0],
-                       init[nt][1]);
+              mma16816(x[j][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], init[nt][0], init[nt][1], init[nt][2],
+                       init[nt][3]);
             else
-              mma16816(d[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], d[nt][0], d[nt][1], d[nt][2], d[nt][3]);
+              mma16816(x[j][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1], x[j][nt][0], x[j][nt][1], x[j][nt][2],
+                       x[j][nt][3]);
           }
         }
       }
       const float s0 = bf16_lo(vs[2 * j]) * scale2, s1 = bf16_lo(vs[2 * j + 1]) * scale2;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        x[j][nt][0] = mul2({d[nt][0], d[nt][1]}, {s0, s0});
-        x[j][nt][1] = mul2({d[nt][2], d[nt][3]}, {s1, s1});
+        x[j][nt][0] *= s0;
+        x[j][nt][1] *= s0;
+        x[j][nt][2] *= s1;
+        x[j][nt][3] *= s1;
       }
     }
     // every key of the step visible to every query of the block?
-    const bool whole = k0 + CH <= min(len, qmin + 1) && (W == 0 || k0 > qmax - W || k0 + CH <= S);
+    const bool whole = k0 <= all_hi && (k0 > all_lo || k0 <= all_sink);
     if (!whole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -592,52 +612,52 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
             for (int h = 0; h < 2; ++h) {
               const int kp = k0 + 16 * j + 8 * h + row8;
               const bool vis = kp < len && kp <= qp && (W == 0 || qp - kp < W || kp < S);
-              float& y = e ? x[j][nt][h].y : x[j][nt][h].x;
-              if (!vis) y = -CUDART_INF_F;
+              if (!vis) x[j][nt][2 * h + e] = -CUDART_INF_F;
             }
         }
     }
-    float lm[NT][2];
-    bool grow = false;
+    float lm[NT][2], over = -CUDART_INF_F;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      lm[nt][0] = fmaxf(x[0][nt][0].x, x[0][nt][1].x);
-      lm[nt][1] = fmaxf(x[0][nt][0].y, x[0][nt][1].y);
 #pragma unroll
-      for (int j = 1; j < KT; ++j) {
-        lm[nt][0] = fmaxf(lm[nt][0], fmaxf(x[j][nt][0].x, x[j][nt][1].x));
-        lm[nt][1] = fmaxf(lm[nt][1], fmaxf(x[j][nt][0].y, x[j][nt][1].y));
+      for (int e = 0; e < 2; ++e) {
+        float v = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+#pragma unroll
+        for (int j = 1; j < KT; ++j) v = max3(v, x[j][nt][e], x[j][nt][e + 2]);
+        lm[nt][e] = v;
       }
-      grow |= lm[nt][0] > mx[nt][0] + 8.f || lm[nt][1] > mx[nt][1] + 8.f;
+      // -inf - -inf (nothing seen so far, nothing here) is a NaN, which the maximum passes over
+      over = max3(over, lm[nt][0] - mx[nt][0], lm[nt][1] - mx[nt][1]);
     }
-    if (__any_sync(0xffffffffu, grow)) raise(lm);
+    if (__any_sync(0xffffffffu, over > 8.f)) raise(lm);
     // P (times the scale of V) as the B operand of the second product
     uint32_t pb[KT][NT][2];
     auto weigh = [&](auto masked) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        F2 use = {-mx[nt][0], -mx[nt][1]}, sum = {l[nt][0], l[nt][1]};
+        float use[2] = {mx[nt][0], mx[nt][1]};
         if constexpr (decltype(masked)::value) {
-          if (mx[nt][0] == -CUDART_INF_F) use.x = 0.f;
-          if (mx[nt][1] == -CUDART_INF_F) use.y = 0.f;
+          if (use[0] == -CUDART_INF_F) use[0] = 0.f;
+          if (use[1] == -CUDART_INF_F) use[1] = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < KT; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float v = bf16_hi(vs[2 * j + h]);
-            const F2 y = add2(x[j][nt][h], use);
-            F2 e = {ex2(y.x), ex2(y.y)};
-            sum = add2(sum, e);
-            e = mul2(e, {v, v});
-            if constexpr (decltype(masked)::value) {  // the scale of a hidden key may be a NaN
-              if (y.x == -CUDART_INF_F) e.x = 0.f;
-              if (y.y == -CUDART_INF_F) e.y = 0.f;
+            float e[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float y = x[j][nt][2 * h + c] - use[c];
+              e[c] = ex2(y);
+              l[nt][c] += e[c];
+              e[c] *= v;
+              if constexpr (decltype(masked)::value) {  // the scale of a hidden key may be a NaN
+                if (y == -CUDART_INF_F) e[c] = 0.f;
+              }
             }
-            pb[j][nt][h] = transpose8(pack_bf16(e.x, e.y));
+            pb[j][nt][h] = transpose8(pack_bf16(e[0], e[1]));
           }
-        l[nt][0] = sum.x;
-        l[nt][1] = sum.y;
       }
     };
     if (whole) weigh(std::false_type{});
@@ -663,8 +683,8 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         constexpr int STEP = HD == 64 ? 4 : 8;
-        const uint32_t a0 = code_pair_signed(u0 >> (STEP * mt)), a1 = code_pair_signed(u1 >> (STEP * mt));
-        const uint32_t a2 = code_pair_signed(u2 >> (STEP * mt)), a3 = code_pair_signed(u3 >> (STEP * mt));
+        const uint32_t a0 = code_pair_signed(u0 >> (STEP * mt), magic), a1 = code_pair_signed(u1 >> (STEP * mt), magic);
+        const uint32_t a2 = code_pair_signed(u2 >> (STEP * mt), magic), a3 = code_pair_signed(u3 >> (STEP * mt), magic);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           mma16816(o[mt][nt], a0, a1, a2, a3, pb[j][nt][0], pb[j][nt][1], o[mt][nt][0], o[mt][nt][1], o[mt][nt][2],
