@@ -10,6 +10,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 
 #include "kernels.h"
 
@@ -1136,32 +1137,39 @@ mdl::WindowAttnArgs window_args(const at::Tensor& qkv, const at::Tensor& kstart,
   return a;
 }
 
-void window_attn_fwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
-                     int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale,
-                     const at::Tensor& err, const std::optional<at::Tensor>& out_lo) {
+// (out, out_lo or None, lse)
+std::tuple<at::Tensor, std::optional<at::Tensor>, at::Tensor> window_attn_fwd(
+    const at::Tensor& qkv, const at::Tensor& kstart, int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks,
+    double scale, const at::Tensor& err, bool keep) {
+  require_cuda(qkv, "qkv");
+  TORCH_CHECK(qkv.dim() == 3 && H > 0 && G > 0 && qkv.size(2) % (H + 2 * G) == 0, "qkv must be [B, Lk, (H + 2 G) * hd]");
   c10::cuda::CUDAGuard guard(qkv.device());
+  const int64_t B = qkv.size(0), width = qkv.size(2) / (H + 2 * G) * H;
+  at::Tensor out = at::empty({B, Lq, width}, qkv.options());
+  std::optional<at::Tensor> out_lo;
+  if (keep) out_lo = at::empty({B, Lq, width}, qkv.options());
+  at::Tensor lse = at::empty({B, H, Lq}, qkv.options().dtype(at::kFloat));
   auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err, out_lo);
   check(mdl::window_attn_fwd(a, stream_of(qkv)), "window_attn_fwd");
   g_launches += 1;
+  return {out, out_lo, lse};
 }
 
-void window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out, const at::Tensor& lse,
-                     const at::Tensor& dout, const at::Tensor& dqkv, const at::Tensor& dsum, int64_t H, int64_t G,
-                     int64_t Lq, int64_t window, int64_t sinks, double scale, const at::Tensor& err,
-                     const at::Tensor& out_lo) {
+at::Tensor window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, const at::Tensor& out,
+                           const at::Tensor& out_lo, const at::Tensor& lse, const at::Tensor& dout, int64_t H,
+                           int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale, const at::Tensor& err) {
   c10::cuda::CUDAGuard guard(qkv.device());
   auto a = window_args(qkv, kstart, out, lse, H, G, Lq, window, sinks, scale, err, out_lo);
   TORCH_CHECK(dout.device() == qkv.device() && dout.scalar_type() == at::kBFloat16 && dout.is_contiguous() &&
                   dout.numel() == out.numel(), "dout must be contiguous bf16 like out");
-  TORCH_CHECK(dqkv.device() == qkv.device() && dqkv.scalar_type() == at::kBFloat16 && dqkv.is_contiguous() &&
-                  dqkv.sizes() == qkv.sizes(), "dqkv must be contiguous bf16 like qkv");
-  TORCH_CHECK(dsum.device() == qkv.device() && dsum.scalar_type() == at::kFloat && dsum.is_contiguous() &&
-                  dsum.numel() == lse.numel(), "dsum must be fp32 [B, H, Lq]");
+  at::Tensor dqkv = at::empty(qkv.sizes(), qkv.options());
+  at::Tensor dsum = at::empty(lse.sizes(), lse.options());
   a.dout = dout.data_ptr();
   a.dqkv = dqkv.data_ptr();
   a.dsum = dsum.data_ptr<float>();
   check(mdl::window_attn_bwd(a, stream_of(qkv)), "window_attn_bwd");
   g_launches += 2;
+  return dqkv;
 }
 
 }  // namespace

@@ -317,7 +317,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Blocks an SM that the registers have to allow: the kernel hides its latencies with warps.
 template <int HD, int NT, int WPI>
 constexpr int min_blocks() {
-  return WPI == 1 ? (NT == 4 ? (HD == 64 ? 2 : 3) : (HD == 64 && NT == 2 ? 3 : 4)) : (NT == 1 ? 2 : 1);
+  return WPI == 1 ? (NT == 1 ? (HD == 64 ? 5 : 6) : (NT == 2 ? 4 : 3)) : (NT == 1 ? 3 : (NT == 2 ? 2 : 1));
 }
 template <int NT>
 constexpr int tiles_a_step() { return NT == 1 ? 4 : 2; }
@@ -326,7 +326,7 @@ constexpr int tiles_a_step() { return NT == 1 ? 4 : 2; }
 template <int HD, int NT>
 constexpr int step_bytes() { return 16 * tiles_a_step<NT>() * (HD + 4); }
 template <int HD>
-constexpr int ring_steps() { return HD == 64 ? 3 : 4; }
+constexpr int ring_steps() { return HD == 64 ? 2 : 3; }
 template <int HD, int NT, int WPI>
 constexpr int attend_smem() {
   constexpr int warps = WPI == 1 ? 4 : WPI;
@@ -413,7 +413,10 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   uint32_t magic;
   asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(kMagic));
   // query of columns 2t + e of a tile (only where a mask is needed)
-  auto query_of = [&](int nt, int e) { return min(m0 + nt * 8 + 2 * t + e, M - 1) / group; };
+  auto query_of = [&](int nt, int e) {
+    const int m = min(m0 + nt * 8 + 2 * t + e, M - 1);
+    return group == 1 ? m : m / group;
+  };
 
   float o[MT][NT][4];
   float mx[NT][2], l[NT][2];
@@ -601,6 +604,14 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     // every key of the step visible to every query of the block?
     const bool whole = k0 <= all_hi && (k0 > all_lo || k0 <= all_sink);
     if (!whole) {
+      uint32_t reach[KT][2];  // a key is visible to the queries less than this far on
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int kp = k0 + 16 * j + 8 * h + row8;
+          reach[j][h] = kp >= len ? 0u : (W == 0 || kp < S ? 0x80000000u : static_cast<uint32_t>(W));
+        }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -609,11 +620,9 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
 #pragma unroll
           for (int j = 0; j < KT; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int kp = k0 + 16 * j + 8 * h + row8;
-              const bool vis = kp < len && kp <= qp && (W == 0 || qp - kp < W || kp < S);
-              if (!vis) x[j][nt][2 * h + e] = -CUDART_INF_F;
-            }
+            for (int h = 0; h < 2; ++h)
+              if (static_cast<uint32_t>(qp - (k0 + 16 * j + 8 * h + row8)) >= reach[j][h])
+                x[j][nt][2 * h + e] = -CUDART_INF_F;
         }
     }
     float lm[NT][2], over = -CUDART_INF_F;
@@ -731,10 +740,12 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const int qn[2] = {query_of(nt, 0), query_of(nt, 1)};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int kp = k0 + g8 + 8 * (e >> 1), n = query_of(nt, e & 1);
-          const bool vis = kp <= n && (W == 0 || n - kp < W || len + kp < S);
+          const int kp = k0 + g8 + 8 * (e >> 1);
+          const uint32_t reach = W == 0 || len + kp < S ? 0x80000000u : static_cast<uint32_t>(W);
+          const bool vis = static_cast<uint32_t>(qn[e & 1] - kp) < reach;
           x[nt][e] = vis ? x[nt][e] * scale2 : -CUDART_INF_F;
         }
 #pragma unroll
@@ -960,13 +971,14 @@ struct Plan {
   long long items;
 };
 
-// Query rows a block: 8, 16 or 32. One warp an item where the items alone fill the device and
+// Query rows a block: 8, 16 or, of 32-wide heads, 32 (of 64-wide ones the accumulators of 32 rows
+// leave 8 warps a multiprocessor: 512 candidates of 32 tokens took 168 us instead of 76). One warp an item where the items alone fill the device and
 // each has few keys; else eight warps an item, and several blocks an item while the items
 // leave multiprocessors idle.
 Plan plan_of(const KvAttendArgs& a) {
   Plan p;
   const int M = a.N * (a.H / a.c.G);
-  p.nt = M <= 8 ? 1 : (M <= 16 ? 2 : 4);
+  p.nt = M <= 8 ? 1 : (M <= 16 || a.c.hd == 64 ? 2 : 4);
   p.qblocks = (M + 8 * p.nt - 1) / (8 * p.nt);
   p.items = static_cast<long long>(a.B) * a.c.G * p.qblocks;
   const long long cap = static_cast<long long>(a.c.max_pages) << a.c.page_shift;
@@ -976,7 +988,7 @@ Plan plan_of(const KvAttendArgs& a) {
   p.splits = 1;
   if (p.wpi == 8) {
     // the least (waves of blocks) x (keys a block + what a block costs besides, as keys)
-    const long long slots = 2LL * sms, most = std::min<long long>(32, std::max<long long>(1, keys / 512));
+    const long long slots = 3LL * sms, most = std::min<long long>(32, std::max<long long>(1, keys / 512));
     double best = 0;
     for (int n = 1; n <= most; ++n) {
       const double cost = static_cast<double>((p.items * n + slots - 1) / slots) * (static_cast<double>(keys) / n + 1024);
@@ -1015,8 +1027,14 @@ cudaError_t launch_attend(const KvAttendArgs& a, const Plan& p, cudaStream_t str
 
 template <int HD>
 cudaError_t attend_hd(const KvAttendArgs& a, const Plan& p, cudaStream_t stream, int* launches) {
-  cudaError_t e = p.nt == 1 ? launch_attend<HD, 1>(a, p, stream)
-                            : (p.nt == 2 ? launch_attend<HD, 2>(a, p, stream) : launch_attend<HD, 4>(a, p, stream));
+  cudaError_t e;
+  if (p.nt == 1) {
+    e = launch_attend<HD, 1>(a, p, stream);
+  } else if (HD == 64 || p.nt == 2) {
+    e = launch_attend<HD, 2>(a, p, stream);
+  } else {
+    if constexpr (HD == 32) e = launch_attend<HD, 4>(a, p, stream);
+  }
   *launches += 1;
   if (e != cudaSuccess || p.splits == 1) return e;
   const long long threads = static_cast<long long>(a.B) * a.N * a.H * (HD / 4);

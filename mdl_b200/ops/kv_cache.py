@@ -76,6 +76,7 @@ class QuantizedKVCache:
         self.table = table
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
         self.codes = torch.empty(num_pages, kv_heads, 2, page, head_dim // 2, dtype=torch.uint8, device=device)
+        self.err = error_word(device) if device.type == "cuda" else None
         self.scales = torch.empty(num_pages, kv_heads, page, 2, dtype=torch.bfloat16, device=device)
 
     @property
@@ -116,8 +117,9 @@ class QuantizedKVCache:
 
 # ----------------------------------------------------------------------------- checks
 def _index(t: torch.Tensor | None, n: int, cache: QuantizedKVCache, name: str) -> torch.Tensor | None:
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and t.device == cache.device
+                     and t.is_contiguous()):
+        return t
     if t.dtype != torch.int32:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
@@ -149,8 +151,9 @@ def _tokens(t: torch.Tensor, width: int, cache: QuantizedKVCache, name: str) -> 
     return t
 
 
-def _no_grad(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(a: torch.Tensor, b: torch.Tensor | None, c: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
+                                    or (c is not None and c.requires_grad)):
         raise RuntimeError("the key/value cache has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -203,7 +206,7 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, st
 
     with trace_range("mdl.kv_cache.write"):
         width = cache.kv_heads * cache.head_dim
-        _no_grad(k, v)
+        _no_grad(k, v, None)
         k, v = _tokens(k, width, cache, "k"), _tokens(v, width, cache, "v")
         n = k.shape[0]
         if v.shape != k.shape:
@@ -218,7 +221,7 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, st
             return
         if start is not None and start.untyped_storage().data_ptr() == cache.lengths.untyped_storage().data_ptr():
             start = start.clone()  # the kernel writes the lengths
-        ext().kv_write(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), k, v, rows,
+        ext().kv_write(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, k, v, rows,
                        start, kstart)
 
 
@@ -252,7 +255,7 @@ def kv_cache_read(cache: QuantizedKVCache, count: int, start: torch.Tensor | Non
             return x[..., 0, :].reshape(n, count, width), x[..., 1, :].reshape(n, count, width)
         k = torch.empty(n, count, width, dtype=dtype, device=cache.device)
         v = torch.empty_like(k)
-        ext().kv_read(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), k, v, rows,
+        ext().kv_read(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, k, v, rows,
                       start)
         return k, v
 
@@ -331,6 +334,6 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKVCache, rows: torch.Tenso
         if cache.device.type != "cuda":
             return cached_attention_reference(q, cache, rows, k_new, v_new, window, sinks, scale).to(q.dtype)
         out = torch.empty(B, N, width, dtype=torch.bfloat16, device=q.device)
-        ext().kv_attend(cache.codes, cache.scales, cache.table, cache.lengths, error_word(cache.device), q, k_new,
+        ext().kv_attend(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, q, k_new,
                         v_new, rows, out, int(window), int(sinks), float(scale) if scale else 1.0 / math.sqrt(hd))
         return out

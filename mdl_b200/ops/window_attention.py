@@ -64,23 +64,15 @@ def window_attention_fwd(qkv, ks, heads: int, kv_heads: int, lq: int, window: in
     """Native forward: ``out [B, lq, heads * hd]`` bf16 and, for a backward (``keep``), what
     rounding took off it and the log-sum-exp ``[B, heads, lq]`` (else None and a workspace)."""
 
-    B, _, W = qkv.shape
-    width = W // (heads + 2 * kv_heads) * heads
-    out = torch.empty(B, lq, width, dtype=torch.bfloat16, device=qkv.device)
-    out_lo = torch.empty_like(out) if keep else None
-    lse = torch.empty(B, heads, lq, dtype=torch.float32, device=qkv.device)
-    ext().window_attn_fwd(qkv, ks, out, lse, heads, kv_heads, lq, window, sinks, scale, error_word(qkv.device), out_lo)
-    return out, out_lo, lse
+    return ext().window_attn_fwd(qkv, ks, heads, kv_heads, lq, window, sinks, scale, error_word(qkv.device), keep)
 
 
 def window_attention_bwd(qkv, ks, out, out_lo, lse, dout, heads: int, kv_heads: int, lq: int, window: int, sinks: int,
                          scale: float = 0.0) -> torch.Tensor:
     """Native backward: the gradient of ``qkv`` (bf16, contiguous)."""
 
-    dqkv = torch.empty(qkv.shape, dtype=torch.bfloat16, device=qkv.device)
-    ext().window_attn_bwd(qkv, ks, out, lse, dout, dqkv, torch.empty_like(lse), heads, kv_heads, lq, window, sinks,
-                          scale, error_word(qkv.device), out_lo)
-    return dqkv
+    return ext().window_attn_bwd(qkv, ks, out, out_lo, lse, dout, heads, kv_heads, lq, window, sinks, scale,
+                                 error_word(qkv.device))
 
 
 class WindowedAttentionFn(torch.autograd.Function):
@@ -96,7 +88,8 @@ class WindowedAttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         qkv, ks, out, out_lo, lse = ctx.saved_tensors
-        dout = dout.to(torch.bfloat16).contiguous()
+        if dout.dtype is not torch.bfloat16 or not dout.is_contiguous():
+            dout = dout.to(torch.bfloat16).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
         return window_attention_bwd(qkv, ks, out, out_lo, lse, dout, *ctx.args), *([None] * 7)
@@ -136,6 +129,8 @@ def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: 
             qkv = qkv.contiguous()
             if qkv.data_ptr() % 16:
                 qkv = qkv.clone()
-        ks = kstart.to(torch.int32).contiguous()
+        ks = kstart
+        if ks.dtype is not torch.int32 or not ks.is_contiguous():
+            ks = ks.to(torch.int32).contiguous()
         return WindowedAttentionFn.apply(qkv, ks, heads, G, lq, min(window, Lk), min(sinks, Lk),
                                          float(scale) if scale else 1.0 / math.sqrt(hd))
