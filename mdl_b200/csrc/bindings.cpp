@@ -1167,8 +1167,14 @@ at::Tensor window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, cons
   a.dout = dout.data_ptr();
   a.dqkv = dqkv.data_ptr();
   a.dsum = dsum.data_ptr<float>();
+  at::Tensor ws;
+  const long long need = mdl::window_attn_workspace(a);
+  if (need > 0) {
+    ws = at::empty({need}, lse.options());
+    a.partial = ws.data_ptr<float>();
+  }
   check(mdl::window_attn_bwd(a, stream_of(qkv)), "window_attn_bwd");
-  g_launches += 2;
+  g_launches += need > 0 ? 3 : 2;
   return dqkv;
 }
 

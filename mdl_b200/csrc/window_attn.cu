@@ -70,6 +70,10 @@ struct Params {
   int B, H, G, Lk, Lq, hd, window, sinks;
   int heads, tiles;  // work items = (head, sample, tile index): heads x B x tiles
   int dh, db, di;    // gridDim.x items further on, in these digits
+  // key tiles: the first `stiles` (those with sinks) come in `parts` items of `psteps` steps each,
+  // whose sums go to `partial` (parts == 1: like any other tile)
+  int stiles, parts, psteps;
+  float* partial;
   float scale, scale2;
   int* err;
 };
@@ -275,8 +279,17 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int hd) {
 struct alignas(16) Item {
   int h, b, kst, n;    // head, sample, first valid token, steps (-1: no more items)
   int t, cs, k0, qf;   // tile; steps: cs from 0, then from k0 on (KEYS: cs a head, from k0); first query
-  int len, pad[3];     // valid tokens
+  int len;             // valid tokens
+  int j0, part, pad;   // first step, and slot of the partial sums (-1: none)
 };
+
+// Query steps of key tile t: from k0 on, cs a query head.
+__device__ __forceinline__ void key_steps(const Params& p, int t, int len, int qf, int& k0, int& cs) {
+  const int qs = max(TILE * t, qf);
+  const int qe = TILE * t < p.sinks ? len : min(len, TILE * t + TILE - 1 + p.window);
+  k0 = qs / BOX;
+  cs = qe > qs && TILE * t < len ? (qe + BOX - 1) / BOX - k0 : 0;
+}
 
 // First row of step j (key tiles: of step j of a query head).
 template <bool KEYS, int ROWS>
@@ -320,15 +333,20 @@ struct Walk {
     it.len = p.Lk - it.kst;
     it.qf = max(0, p.Lk - p.Lq - it.kst);
     it.n = it.cs = it.k0 = 0;
+    it.j0 = 0;
+    it.part = -1;
     if constexpr (KEYS) {
-      // the sinks' tile comes first: every query sees it
-      it.t = i;
-      if (TILE * it.t >= it.len) return true;
-      const int qs = max(TILE * it.t, it.qf);
-      const int qe = TILE * it.t < p.sinks ? it.len : min(it.len, TILE * it.t + TILE - 1 + p.window);
-      it.k0 = qs / ROWS;
-      it.cs = qe > qs ? (qe + ROWS - 1) / ROWS - it.k0 : 0;
+      // the sinks' tiles come first: every query sees them
+      const int split = p.stiles * p.parts;
+      it.t = i < split ? i / p.parts : i - split + p.stiles;
+      key_steps(p, it.t, it.len, it.qf, it.k0, it.cs);
       it.n = it.cs * (p.H / p.G);
+      if (p.parts > 1 && i < split) {
+        const int c = i - it.t * p.parts;
+        it.j0 = c * p.psteps;
+        it.n = max(0, min(it.n - it.j0, p.psteps));
+        it.part = ((it.b * p.G + it.h) * p.stiles + it.t) * p.parts + c;
+      }
     } else {
       it.t = (it.len + TILE - 1) / TILE - 1 - i;  // the last tile first
       if (it.t < 0 || TILE * (it.t + 1) <= it.qf) return true;
@@ -815,7 +833,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       };
       for (int k = w.i * 32 + lane; k < it.kst + (KEYS ? 0 : it.qf); k += p.tiles * 32) clear(k);
       if (it.n == 0) {
-        if (KEYS)
+        if (KEYS && it.part < 0)
           for (int k = ya + lane; k < min(ya + TILE, p.Lk); k += 32) clear(k);
         continue;
       }
@@ -854,8 +872,9 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         copies_arrive(bar);
       };
       if constexpr (!KEYS) copy_rows(sLse, nullptr, TILE * it.t, it.h, a_full);
-      int h = KEYS ? it.h * (p.H / p.G) : it.h;
-      for (int j = 0, s = 0; j < it.n; ++j, ++s, ++g) {
+      const int a0 = KEYS && it.j0 > 0 ? it.j0 / it.cs : 0;
+      int h = KEYS ? it.h * (p.H / p.G) + a0 : it.h;
+      for (int j = 0, s = it.j0 - a0 * it.cs; j < it.n; ++j, ++s, ++g) {
         const int st = g % B_STAGES;
         if (!warp_wait(&b_empty[st], (g / B_STAGES + 1) & 1, p.err, abort_flag)) {
           ok = false;
@@ -1002,11 +1021,21 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       __nv_bfloat16* dst = p.dqkv + (static_cast<long long>(it.b) * p.Lk + it.kst + own) * (p.H + 2 * p.G) * HD +
                            head * HD + col0;
       const float f = (KEYS && half == 0) ? 1.f : p.scale;
+      float4* sums = KEYS && it.part >= 0
+                         ? reinterpret_cast<float4*>(p.partial + ((static_cast<long long>(it.part) * TILE + r) * 2 + half) * HD)
+                         : nullptr;
 #pragma unroll
       for (int e = 0; e < COLS / 8; ++e) {  // few registers at a time: the scores are held
         uint32_t gr[8], y[4];
         tmem_ld8(tAcc_own + 8 * e, gr);
         tmem_wait_ld();
+        if (KEYS && sums != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            sums[2 * e + c] = make_float4(__uint_as_float(gr[4 * c]) * f, __uint_as_float(gr[4 * c + 1]) * f,
+                                          __uint_as_float(gr[4 * c + 2]) * f, __uint_as_float(gr[4 * c + 3]) * f);
+          continue;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = pack2(__uint_as_float(gr[2 * c]) * f, __uint_as_float(gr[2 * c + 1]) * f);
         if (store) reinterpret_cast<uint4*>(dst)[e] = make_uint4(y[0], y[1], y[2], y[3]);
@@ -1072,7 +1101,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         if (half == 0 && real)
           p.dsum[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.kst + own - q0] = row_d;
       }
-      for (int j = 0, s_ = 0; j < n; ++j, ++s_, ++g) {
+      for (int j = 0, s_ = KEYS && it.j0 > 0 ? it.j0 % cs : 0; j < n; ++j, ++s_, ++g) {
         if (KEYS && s_ == cs) s_ = 0;
         const int st = g % B_STAGES;
         const int c0 = step_row<KEYS, BOX>(s_, cs, k0) + 32 * half;  // this warp's first column
@@ -1166,6 +1195,36 @@ __global__ void __launch_bounds__(B_THREADS, 2)
   }
 }
 
+// dV and dK of the sinks' tiles from their parts, in the parts' order. JOIN_ROWS rows a block;
+// a thread = four neighbouring elements.
+constexpr int JOIN_ROWS = 8;
+template <int HD>
+__global__ void __launch_bounds__(128) window_join_kernel(const Params p) {
+  const int tile = blockIdx.x / (TILE / JOIN_ROWS), r0 = blockIdx.x % (TILE / JOIN_ROWS) * JOIN_ROWS;
+  const int t = tile % p.stiles, bg = tile / p.stiles;
+  const int g = bg % p.G, b = bg / p.G;
+  const int kst = min(max(p.kstart[b], 0), p.Lk), len = p.Lk - kst;
+  int k0, cs;
+  key_steps(p, t, len, max(0, p.Lk - p.Lq - kst), k0, cs);
+  const int parts = (cs * (p.H / p.G) + p.psteps - 1) / p.psteps;
+  const float4* src = reinterpret_cast<const float4*>(p.partial + static_cast<long long>(tile) * p.parts * TILE * 2 * HD);
+  constexpr int ROW = 2 * (HD / 4);
+  for (int i = r0 * ROW + threadIdx.x; i < (r0 + JOIN_ROWS) * ROW; i += blockDim.x) {
+    const int row = TILE * t + i / ROW, kv = i / (HD / 4) & 1, c = i % (HD / 4);  // kv 0: V, 1: K
+    if (row >= len) break;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c2 = 0; c2 < parts; ++c2) {
+      const float4 y = src[c2 * (TILE * ROW) + i];
+      sum.x += y.x;
+      sum.y += y.y;
+      sum.z += y.z;
+      sum.w += y.w;
+    }
+    const long long o = (static_cast<long long>(b) * p.Lk + kst + row) * (p.H + 2 * p.G) + (kv ? p.H + g : p.H + p.G + g);
+    reinterpret_cast<uint2*>(p.dqkv + o * HD)[c] = make_uint2(pack2(sum.x, sum.y), pack2(sum.z, sum.w));
+  }
+}
+
 // ============================================================================ host side
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -1217,6 +1276,10 @@ Params make_params(const WindowAttnArgs& a, int heads, int tiles, int grid) {
   p.hd = a.hd;
   p.window = std::min(a.window, a.Lk);  // wider ones see the same
   p.sinks = std::min(a.sinks, a.Lk);
+  p.stiles = 0;
+  p.parts = 1;
+  p.psteps = 0;
+  p.partial = a.partial;
   p.heads = heads;
   p.tiles = tiles;
   p.dh = grid % heads;
@@ -1263,6 +1326,30 @@ cudaError_t allow_smem(K kern, int bytes, std::atomic<bool>* done) {
   return e;
 }
 
+// How the sinks' key tiles are cut. Every query sees them, so with few samples and a long history
+// one of them would be the critical path: 2 samples of 8,191 tokens, 4 heads, took 223 us for the
+// launch, 128 steps in one block where the average was 35. Parts of about half the average load.
+struct Cut {
+  int stiles = 0, parts = 1, psteps = 1;
+};
+Cut cut_of(const WindowAttnArgs& a) {
+  Cut c;
+  const long long group = a.H / a.G, ktiles = (a.Lk + TILE - 1) / TILE;
+  const int window = std::min(a.window, a.Lk), sinks = std::min(a.sinks, a.Lk);
+  c.stiles = (sinks + TILE - 1) / TILE;
+  if (c.stiles == 0) return c;
+  const long long most = (std::min(a.Lq, a.Lk) + BOX - 1) / BOX * group + group;  // steps of a sinks' tile
+  const long long usual = std::min<long long>(most, ((window + TILE) / BOX + 1) * group);
+  const long long total = static_cast<long long>(a.B) * a.G * (c.stiles * most + (ktiles - c.stiles) * usual);
+  const long long load = total / (2LL * num_sms(device_index())) + 1;
+  const long long steps = std::max<long long>(16, load / 2);
+  const long long parts = (most + steps - 1) / steps;
+  if (most <= load || parts < 2) return c;
+  c.parts = static_cast<int>(parts);
+  c.psteps = static_cast<int>(steps);
+  return c;
+}
+
 int grid_of(long long heads, long long samples, long long tiles, long long most) {
   return static_cast<int>(std::min(heads * samples * tiles, most));
 }
@@ -1300,19 +1387,34 @@ cudaError_t bwd_hd(const WindowAttnArgs& a, cudaStream_t stream) {
   if (e == cudaSuccess) e = allow_smem(window_bwd_kernel<HD, true>, B_SMEM, &ready_k[dev]);
   if (e != cudaSuccess) return e;
   const long long most = 2LL * num_sms(dev);
-  const int qtiles = (a.Lq + TILE - 1) / TILE + 1, ktiles = (a.Lk + TILE - 1) / TILE;
+  const Cut cut = cut_of(a);
+  if (cut.parts > 1 && a.partial == nullptr) return cudaErrorInvalidValue;
+  const int qtiles = (a.Lq + TILE - 1) / TILE + 1;
+  const int ktiles = (a.Lk + TILE - 1) / TILE + cut.stiles * (cut.parts - 1);
   const int qgrid = grid_of(a.H, a.B, qtiles, most), kgrid = grid_of(a.G, a.B, ktiles, most);
   // queries first: they leave D behind
   window_bwd_kernel<HD, false><<<qgrid, B_THREADS, B_SMEM, stream>>>(tq, tkv, tdo,
                                                                            make_params(a, a.H, qtiles, qgrid));
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  window_bwd_kernel<HD, true><<<kgrid, B_THREADS, B_SMEM, stream>>>(tq, tkv, tdo,
-                                                                         make_params(a, a.G, ktiles, kgrid));
+  Params pk = make_params(a, a.G, ktiles, kgrid);
+  pk.stiles = cut.stiles;
+  pk.parts = cut.parts;
+  pk.psteps = cut.psteps;
+  window_bwd_kernel<HD, true><<<kgrid, B_THREADS, B_SMEM, stream>>>(tq, tkv, tdo, pk);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || cut.parts == 1) return e;
+  window_join_kernel<HD><<<a.B * a.G * cut.stiles * (TILE / JOIN_ROWS), 128, 0, stream>>>(pk);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+long long window_attn_workspace(const WindowAttnArgs& a) {
+  if (!shapes_ok(a)) return 0;
+  const Cut c = cut_of(a);
+  return c.parts == 1 ? 0 : static_cast<long long>(a.B) * a.G * c.stiles * c.parts * TILE * 2 * a.hd;
+}
 
 cudaError_t window_attn_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
   if (!shapes_ok(a)) return cudaErrorInvalidValue;

@@ -28,11 +28,14 @@ struct WindowAttnArgs {
   const void* dout = nullptr;   // bf16 [B, Lq, H * hd] contiguous
   void* dqkv = nullptr;
   float* dsum = nullptr;
+  float* partial = nullptr;     // window_attn_workspace() floats
   int B = 0, H = 0, G = 0, Lk = 0, Lq = 0, hd = 0, window = 0, sinks = 0;
   float scale = 1.f;
   int* err = nullptr;
 };
 
+// Floats of workspace that the backward needs (0 unless the sinks' tiles are cut into parts).
+long long window_attn_workspace(const WindowAttnArgs& a);
 cudaError_t window_attn_fwd(const WindowAttnArgs& a, cudaStream_t stream);
 cudaError_t window_attn_bwd(const WindowAttnArgs& a, cudaStream_t stream);
 

@@ -296,3 +296,24 @@ def test_refusals(device):
             windowed_attention(qkv, ks, 2, 10, 3)
         with pytest.raises(ValueError):
             windowed_attention(qkv, ks.cpu(), 1, 10, 3)
+
+
+@GPU
+@pytest.mark.parametrize("B,Lk,lq,H,G,hd,window,sinks,kstart", [
+    (1, 6000, 6000, 2, 1, 64, 40, 3, [0]), (2, 5000, 4500, 1, 1, 32, 100, 200, [0, 4400]),
+    (2, 4096, 4096, 2, 2, 32, 64, 1, [4095, 1]), (1, 9000, 9000, 1, 1, 64, 1, 129, [17]),
+])
+def test_sinks_of_few_long_samples(B, Lk, lq, H, G, hd, window, sinks, kstart):
+    """The sinks' key tiles, which every query sees, are summed in parts."""
+
+    qkv, dout = _inputs(B, Lk, lq, H, G, hd, "cuda", 8)
+    ks = torch.tensor(kstart, dtype=torch.int32, device="cuda")
+    x = qkv.clone().requires_grad_()
+    o = windowed_attention(x, ks, H, lq, window, sinks, kv_heads=G)
+    (dx,) = torch.autograd.grad(o, x, dout)
+    o2 = windowed_attention(x, ks, H, lq, window, sinks, kv_heads=G)
+    assert torch.equal(dx, torch.autograd.grad(o2, x, dout)[0])
+    _errors()
+    (out, otol), (grad, gtol) = _exact(qkv, kstart, dout, H, G, lq, window, sinks)
+    _close(o, out, otol)
+    _close(dx, grad, gtol)
