@@ -30,6 +30,8 @@ SCHEMA_EXTENSIONS = {
     "training.adam_beta1/adam_beta2/adam_eps/weight_decay": "Adam hyper-parameters",
     "model.tokens_per_scenario": "N domain tokens per scene (pooled by DomainFused)",
     "model.pyramid_schedule/pyramid_halve_every": "OneTrans pyramid: linear or halve every k layers",
+    "model.attention_window/attention_sinks": "OneTrans: tokens a query sees back (0: all) and first tokens it always sees",
+    "model.request_cache_format": "OneTrans request cache: 'full' precision or '4bit' (quantised keys and values)",
     "model.sequence_head": "LONGER sequence encoder feeding a MixFormer-style head",
     "runtime.kernel_backend": "'native' (sm_100a kernels, mandatory on CUDA) or 'torch' (CPU oracle)",
     "training.comm": "fused NVLink collectives ('fused') or NCCL baseline ('nccl')",
@@ -448,6 +450,9 @@ class ModelConfig:
     pyramid_round_to: int = 32
     pyramid_schedule: Literal["linear", "halve"] = "linear"
     pyramid_halve_every: int = 2
+    attention_window: int = 0
+    attention_sinks: int = 0
+    request_cache_format: Literal["full", "4bit"] = "full"
     ns_tokenizer: Literal["auto_split", "groupwise", "dcnv2"] = "auto_split"
     num_ns_tokens: int | None = None
     ns_dcn_cross_layers: int = 3

@@ -75,6 +75,14 @@ def validate_app_config(config: AppConfig) -> None:
                  f"rankmixer requires token_dim ({model.token_dim}) divisible by the feature token count ({count})")
     if model.name in ("onetrans", "mdl_onetrans", "mixformer", "mdl_mixformer", "longer"):
         _require(model.token_dim % model.num_heads == 0, "token_dim must be divisible by num_heads")
+    _require(model.attention_window >= 0 and model.attention_sinks >= 0,
+             "model.attention_window and model.attention_sinks must not be negative")
+    _require(model.attention_window > 0 or model.attention_sinks == 0,
+             "model.attention_sinks keeps first tokens visible beside a window: set model.attention_window")
+    if model.name not in ("onetrans", "mdl_onetrans"):
+        _require(model.attention_window == 0, f"model.attention_window: {model.name} has no windowed attention")
+    _require(model.request_cache_format == "full" or model.name == "onetrans",
+             "model.request_cache_format 4bit is the OneTrans request cache")
     if model.name.startswith("mdl_"):
         _require(model.tokens_per_scenario >= 1, "tokens_per_scenario must be >= 1")
     if model.name in ("mdl_onetrans", "mdl_mixformer"):

@@ -27,6 +27,11 @@ over the NS tokens, both writing straight into the buffer, and the weight
 gradient of a shared weight sums the per-sample row ranges inside one GEMM. The
 attention is the tcgen05 flash attention of ``ops/attention.py``.
 
+``model.attention_window`` bounds the view of every layer's queries to the last ``window``
+tokens of the layer's token sequence and its first ``attention_sinks`` valid tokens
+(``ops/window_attention.py``); ``model.request_cache_format: 4bit`` keeps the request cache
+quantised (``ops/kv_cache.py``).
+
 Pyramid schedules: ``linear`` is the reference's (``_layer_s_count``
 ``src/model.py:6181-6198``); ``halve`` keeps ``initial >> ((l + 1) // k)`` S
 queries at layer ``l`` (halving every ``k`` layers), rounded like ``linear``.
@@ -44,6 +49,8 @@ from ..config.schema import AppConfig
 from ..ops._ext import error_word, ext
 from ..ops.attention import (NATIVE_HEAD_DIMS, attention_bwd, attention_fwd, suffix_attention,
                              suffix_attention_reference)
+from ..ops.window_attention import (HEAD_DIMS as WINDOW_HEAD_DIMS, window_attention_bwd, window_attention_fwd,
+                                    windowed_attention_reference)
 from ..ops.gemm import ACT_ADD, ACT_DMUL, ACT_GELU_GRAD, bgemm
 from ..ops.layers import _grad, _kaiming_uniform_, _shadow, gemm_param
 from .features import FeatureEncoder
@@ -162,9 +169,13 @@ class OneTransLayerFn(torch.autograd.Function):
         _mixed_fwd(xn, Lk, s_in, D, _shadow(layer.wqkv_s), layer.bqkv_s, _shadow(layer.wqkv_ns), layer.bqkv_ns, qkv,
                    3 * D)
         ks = kstart.to(torch.int32).contiguous()
-        att = torch.empty(B, Lq, D, dtype=torch.bfloat16, device=dev)
-        lse = torch.empty(B, heads, Lq, dtype=torch.float32, device=dev)
-        attention_fwd(qkv, ks, att, lse, heads, Lq, True)
+        if layer.window:
+            att, att_lo, lse = window_attention_fwd(qkv, ks, heads, heads, Lq, layer.window, layer.sinks)
+        else:
+            att = torch.empty(B, Lq, D, dtype=torch.bfloat16, device=dev)
+            att_lo = None
+            lse = torch.empty(B, heads, Lq, dtype=torch.float32, device=dev)
+            attention_fwd(qkv, ks, att, lse, heads, Lq, True)
         h = torch.empty(B, Lq, D, dtype=torch.bfloat16, device=dev)
         # h = X[:, Lk-Lq:] + att W_o^T + b_o
         bgemm(att, _shadow(layer.wo), h, M=Lq, N=D, K=D, G=B, lda=D, gsA=Lq * D, ldb=D, gsB=0, ldc=D, gsC=Lq * D,
@@ -179,13 +190,13 @@ class OneTransLayerFn(torch.autograd.Function):
         Y = torch.empty(B, Lq, D, dtype=torch.bfloat16, device=dev)
         _mixed_fwd(u, Lq, q, Hd, _shadow(layer.w2_s), layer.b2_s, _shadow(layer.w2_ns), layer.b2_ns, Y, D,
                    act=ACT_ADD, aux=h)
-        ctx.save_for_backward(X, xn, rstd1, qkv, ks, att, lse, h, hn, rstd2, ug, u)
+        ctx.save_for_backward(X, xn, rstd1, qkv, ks, att, att_lo, lse, h, hn, rstd2, ug, u)
         ctx.meta = (layer, s_in, q, heads)
         return Y
 
     @staticmethod
     def backward(ctx, dY):
-        X, xn, rstd1, qkv, ks, att, lse, h, hn, rstd2, ug, u = ctx.saved_tensors
+        X, xn, rstd1, qkv, ks, att, att_lo, lse, h, hn, rstd2, ug, u = ctx.saved_tensors
         layer, s_in, q, heads = ctx.meta
         C = ext()
         B, Lk, D = X.shape
@@ -213,8 +224,11 @@ class OneTransLayerFn(torch.autograd.Function):
               accumulate=True)
         C.colsum(dh, _grad(layer.bo), 1, B * Lq, D, D, 0, 1.0)
         # ---- attention
-        dqkv = torch.empty_like(qkv)
-        attention_bwd(qkv, ks, att, lse, datt, dqkv, heads, Lq, True)
+        if layer.window:
+            dqkv = window_attention_bwd(qkv, ks, att, att_lo, lse, datt, heads, heads, Lq, layer.window, layer.sinks)
+        else:
+            dqkv = torch.empty_like(qkv)
+            attention_bwd(qkv, ks, att, lse, datt, dqkv, heads, Lq, True)
         del datt
         # ---- Q/K/V projections
         dxn = torch.empty_like(X)
@@ -375,9 +389,11 @@ def _mixed_reference(x, s, w_s, b_s, w_ns, b_ns):
 class OneTransLayer(nn.Module):
     """Parameters of one block (reference ``OneTransBlock`` ``src/model.py:5821-5840``)."""
 
-    def __init__(self, token_dim: int, hidden_dim: int, num_ns: int, device=None) -> None:
+    def __init__(self, token_dim: int, hidden_dim: int, num_ns: int, device=None, window: int = 0,
+                 sinks: int = 0) -> None:
         super().__init__()
         D, H, N = token_dim, hidden_dim, num_ns
+        self.window, self.sinks = window, sinks  # 0: every earlier token is visible
         self.token_dim, self.hidden_dim, self.num_ns = D, H, N
         self.norm1 = nn.Parameter(torch.ones(D, device=device))
         self.wqkv_s = gemm_param(torch.empty(3 * D, D, device=device))
@@ -410,7 +426,10 @@ class OneTransLayer(nn.Module):
         Lq = q + N
         xn = _rms_reference(X, self.norm1, eps)
         qkv = _mixed_reference(xn, s_in, self.wqkv_s, self.bqkv_s, self.wqkv_ns, self.bqkv_ns)
-        att = suffix_attention_reference(qkv, kstart, heads, Lq)
+        if self.window:
+            att = windowed_attention_reference(qkv, kstart, heads, Lq, self.window, self.sinks)
+        else:
+            att = suffix_attention_reference(qkv, kstart, heads, Lq)
         h = X[:, Lk - Lq:].float() + att @ self.wo.t() + self.bo
         hn = _rms_reference(h, self.norm2, eps)
         u = F.gelu(_mixed_reference(hn, q, self.w1_s, self.b1_s, self.w1_ns, self.b1_ns))
@@ -533,7 +552,9 @@ class OneTransModel(nn.Module):
                                         m.ffn_activation, device=device)
         P = max(int(config.resolved.onetrans_max_position_embeddings), self.L + N)
         self.pos = nn.Parameter(torch.empty(P, D, device=device).normal_(0.0, m.init_std))
-        self.layers = nn.ModuleList(OneTransLayer(D, Hd, N, device=device) for _ in range(m.num_layers))
+        self.window, self.sinks = int(m.attention_window), int(m.attention_sinks)
+        self.layers = nn.ModuleList(OneTransLayer(D, Hd, N, device=device, window=self.window, sinks=self.sinks)
+                                    for _ in range(m.num_layers))
         self.query_counts = pyramid_query_counts(config, self.L, N)
         self.ntask = len(config.task_names)
         self.task_query = None
@@ -611,9 +632,10 @@ class OneTransModel(nn.Module):
         seq_in = grad_ready(seq_in, hooks, nl + 1)
         if self.ns_mode != "auto_split":
             ns_in = self.ns_tokens(ns_in).to(torch.bfloat16)
-        if self.head_dim not in NATIVE_HEAD_DIMS:
+        native_dims = WINDOW_HEAD_DIMS if self.window else NATIVE_HEAD_DIMS
+        if self.head_dim not in native_dims:
             raise NotImplementedError(f"OneTrans head_dim {self.head_dim}: the native attention kernels take "
-                                      f"{NATIVE_HEAD_DIMS} (set runtime.kernel_backend: torch for this model)")
+                                      f"{native_dims} (set runtime.kernel_backend: torch for this model)")
         if self.multi:
             X = OneTransAssembleFn.apply(seq_in.to(torch.bfloat16), ns_in, kstart, self, self.L)
         else:
@@ -680,7 +702,9 @@ class OneTransModel(nn.Module):
         precede the NS tokens and the attention is causal, so every S token's output is
         independent of the candidate: per layer the cache keeps the K/V of the layer's S
         keys and their padding count; candidates then run only their NS tokens. Rows are the
-        requests of the sequence payload (``row_indices``; one per row without it)."""
+        requests of the sequence payload (``row_indices``; one per row without it). With
+        ``model.request_cache_format: 4bit`` a layer's K/V are a ``QuantizedKVCache``
+        (``head_dim + 4`` bytes a token and head instead of ``8 * head_dim``)."""
 
         from .features import lookup_sequence
 
@@ -697,12 +721,21 @@ class OneTransModel(nn.Module):
         e = torch.arange(L, device=S.device)
         valid = e.view(1, -1) >= ks.view(-1, 1)
         S = S + self.pos[(e.view(1, -1) - ks.view(-1, 1)).clamp(min=0)] * valid.unsqueeze(-1)
+        from ..ops.kv_cache import QuantizedKVCache, kv_cache_write
+
+        four_bits = self.config.model.request_cache_format == "4bit"
         layers, s_in, kst = [], L, ks
         for i, layer in enumerate(self.layers):
             q = self.query_counts[i]
             xn = _rms_reference(S, layer.norm1, self.eps)
             kv = xn @ layer.wqkv_s[D:].t() + layer.bqkv_s[D:]                   # [R, s_in, 2D]
-            layers.append((kv, kst))
+            if four_bits:
+                cache = QuantizedKVCache(R, s_in, self.attn_heads, self.head_dim, device=kv.device)
+                kv = kv.to(torch.bfloat16)
+                kv_cache_write(cache, kv[..., :D], kv[..., D:], kstart=kst)
+                layers.append((cache, kst))
+            else:
+                layers.append((kv, kst))
             S = layer.forward_reference(S, kst, s_in, q, self.attn_heads, self.eps)  # S-only: q outputs
             kst = (kst - (s_in - q)).clamp(min=0)
             s_in = q
@@ -712,9 +745,11 @@ class OneTransModel(nn.Module):
     def forward_with_cache(self, batch, request_cache: dict) -> torch.Tensor:
         """Logits ``[rows, tasks]`` of candidate rows from a request cache: the NS tokens
         attend to their request's cached S keys (valid from the cached padding count) and
-        causally to each other; the per-NS-token projections and FFNs run per candidate."""
+        causally to each other (within the model's window); the per-NS-token projections and
+        FFNs run per candidate. A 4-bit cache is attended to as it is (``cached_attention``)."""
 
         from ..ops.embedding import fused_lookup
+        from ..ops.kv_cache import QuantizedKVCache, cached_attention
 
         anchor = torch.zeros(0, device=batch.ids.device)
         B, L, D, N, H = batch.rows, self.L, self.token_dim, self.num_ns, self.attn_heads
@@ -730,20 +765,32 @@ class OneTransModel(nn.Module):
         ks0 = request_cache["kstart"].index_select(0, ri)
         X = X + self.pos[(L + torch.arange(N, device=X.device).view(1, -1) - ks0.view(-1, 1)).clamp(min=0)]
         hd = D // H
-        causal = torch.ones(N, N, dtype=torch.bool, device=X.device).tril()
+        n = torch.arange(N, device=X.device)
+        ri32 = ri.to(torch.int32)
         for layer, (kv_s, kst) in zip(self.layers, request_cache["layers"]):
             xn = _rms_reference(X, layer.norm1, self.eps)
             qkv = torch.einsum("bnk,nok->bno", xn, layer.wqkv_ns) + layer.bqkv_ns.unsqueeze(0)   # [B, N, 3D]
-            kv = torch.cat([kv_s.index_select(0, ri), qkv[..., D:]], dim=1)                    # [B, s + N, 2D]
-            s_in = kv_s.shape[1]
-            k = kv[..., :D].reshape(B, s_in + N, H, hd).transpose(1, 2)
-            v = kv[..., D:].reshape(B, s_in + N, H, hd).transpose(1, 2)
-            qh = qkv[..., :D].reshape(B, N, H, hd).transpose(1, 2)
-            s_ok = torch.arange(s_in, device=X.device).view(1, 1, s_in) >= kst.index_select(0, ri).view(B, 1, 1)
-            allowed = torch.cat([s_ok.expand(B, N, s_in), causal.view(1, N, N).expand(B, N, N)], dim=2)
-            sc = (qh @ k.transpose(-1, -2)) / math.sqrt(hd)
-            att = torch.softmax(sc.masked_fill(~allowed.unsqueeze(1), float("-inf")), -1) @ v
-            h = X + att.transpose(1, 2).reshape(B, N, D) @ layer.wo.t() + layer.bo
+            if isinstance(kv_s, QuantizedKVCache):
+                x16 = qkv.to(torch.bfloat16) if qkv.is_cuda else qkv
+                att = cached_attention(x16[..., :D], kv_s, rows=ri32, k_new=x16[..., D:2 * D], v_new=x16[..., 2 * D:],
+                                       window=layer.window, sinks=layer.sinks).float()
+            else:
+                kv = torch.cat([kv_s.index_select(0, ri), qkv[..., D:]], dim=1)                # [B, s + N, 2D]
+                s_in = kv_s.shape[1]
+                k = kv[..., :D].reshape(B, s_in + N, H, hd).transpose(1, 2)
+                v = kv[..., D:].reshape(B, s_in + N, H, hd).transpose(1, 2)
+                qh = qkv[..., :D].reshape(B, N, H, hd).transpose(1, 2)
+                # positions count from the request's first valid token; NS tokens follow the S keys
+                start = kst.index_select(0, ri).view(B, 1, 1)
+                pos = torch.arange(s_in + N, device=X.device).view(1, 1, -1) - start
+                at = s_in + n.view(1, N, 1) - start
+                allowed = (pos >= 0) & (pos <= at)
+                if layer.window:
+                    allowed = allowed & ((at - pos < layer.window) | (pos < layer.sinks))
+                sc = (qh @ k.transpose(-1, -2)) / math.sqrt(hd)
+                att = torch.softmax(sc.masked_fill(~allowed.unsqueeze(1), float("-inf")), -1) @ v
+                att = att.transpose(1, 2).reshape(B, N, D)
+            h = X + att @ layer.wo.t() + layer.bo
             hn = _rms_reference(h, layer.norm2, self.eps)
             u = F.gelu(torch.einsum("bnk,nok->bno", hn, layer.w1_ns) + layer.b1_ns.unsqueeze(0))
             X = h + torch.einsum("bnk,nok->bno", u, layer.w2_ns) + layer.b2_ns.unsqueeze(0)

@@ -6,6 +6,9 @@ will run has a kernel here, and describe which (reference ``_attention_runtime_d
   tcgen05 flash attention (``csrc/fmha.cu``) for head_dim 32 and the CUDA-core kernels
   (``csrc/attn_simt.cu``) for head_dim 8, 16 and 64, on sm_100 devices (any width with
   ``runtime.kernel_backend: torch``);
+* OneTrans with ``model.attention_window`` runs the tcgen05 windowed attention
+  (``csrc/window_attn.cu``) and with ``model.request_cache_format: 4bit`` the 4-bit cache
+  kernels (``csrc/kv_cache.cu``), both for head_dim 32 and 64;
 * MDL domain-aware attention and the task-query readout run the few-query kernel
   when both token counts are at most 64 (PyTorch SDPA beyond);
 * MixFormer / STCA single-query attention and the MDL-OneTrans sequence reader
@@ -44,6 +47,19 @@ def attention_preflight(config, device: torch.device | str | None = None) -> dic
     backend = config.runtime.kernel_backend
     if m.name in ("onetrans", "mdl_onetrans"):
         paths["mixed_causal"] = _fmha_check("OneTrans", int(m.token_dim), int(m.num_heads), problems, backend)
+        hd = int(m.token_dim) // max(1, int(m.num_heads))
+        if m.attention_window and backend != "torch":
+            from .window_attention import HEAD_DIMS
+
+            if hd in HEAD_DIMS:
+                paths["mixed_causal"] = f"tcgen05 windowed flash attention (head_dim {hd})"
+            else:
+                problems.append(f"OneTrans attention_window: the native kernels take head_dim {HEAD_DIMS}, not {hd}")
+        if m.request_cache_format == "4bit":
+            from .kv_cache import HEAD_DIMS as CACHE_DIMS
+
+            if hd not in CACHE_DIMS:
+                problems.append(f"OneTrans request_cache_format 4bit: head_dim {CACHE_DIMS}, not {hd}")
     for seq in config.sequences:
         if seq.encoder == "longer":
             d = int(seq.longer_dim)
