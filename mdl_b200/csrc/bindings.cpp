@@ -985,24 +985,64 @@ mdl::KvCache kv_cache_of(const at::Tensor& codes, const at::Tensor& scales, cons
   return c;
 }
 
-// [n, T, width] bf16 whose rows are read in 16-byte pieces
-const __nv_bfloat16* kv_rows(const at::Tensor& t, int64_t n, int64_t T, int64_t width, const mdl::KvCache&,
-                             const at::Device& dev, const char* name, long long* sb, long long* st) {
-  TORCH_CHECK(t.device() == dev && t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == n &&
-                  t.size(1) == T && t.size(2) == width && t.stride(2) == 1 && t.stride(0) % 8 == 0 &&
-                  t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must be bf16 [", n, ", ", T, ", ", width, "] with 16-byte aligned rows");
-  *sb = t.stride(0);
-  *st = t.stride(1);
-  return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr());
+std::string text(const char* s) { return s; }
+std::string text(int64_t n) { return std::to_string(n); }
+std::string text(const at::Device& d) { return d.str(); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
+std::string text(at::IntArrayRef sizes) {
+  std::string s = "(";
+  for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+  return s + ")";
+}
+template <typename... A>
+std::string message(const A&... a) {
+  std::string s;
+  ((s += text(a)), ...);
+  return s;
+}
+template <typename... A>
+[[noreturn]] void value_error(const A&... a) {
+  throw std::invalid_argument(message(a...));  // a ValueError in Python
+}
+template <typename... A>
+[[noreturn]] void type_error(const A&... a) {
+  PyErr_SetString(PyExc_TypeError, message(a...).c_str());
+  throw py::error_already_set();
 }
 
-const int* kv_index(const std::optional<at::Tensor>& t, int64_t n, const at::Device& dev, const char* name) {
-  if (!t.has_value() || !t->defined()) return nullptr;
-  TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() == n, name,
-              " must be contiguous int32 [", n, "]");
-  return t->data_ptr<int>();
+bool same_device(const at::Tensor& t, const at::Tensor& like) { return t.is_cuda() && t.get_device() == like.get_device(); }
+
+// [n, T, width] bf16 whose rows are read in 16-byte pieces; a copy where the strides do not allow it.
+at::Tensor kv_rows(const at::Tensor& t, int64_t n, int64_t T, int64_t width, const at::Tensor& codes, const char* name,
+                   long long* sb, long long* st) {
+  if (!same_device(t, codes)) value_error(name, " on ", t.device(), ", the cache on ", codes.device());
+  if (t.scalar_type() != at::kBFloat16) type_error(name, " must be bf16, not ", t.scalar_type());
+  if (t.dim() != 3 || t.size(0) != n || t.size(1) != T || t.size(2) != width)
+    value_error(name, " ", t.sizes(), ", expected [", n, ", ", T, ", ", width, "]");
+  if (at::GradMode::is_enabled() && t.requires_grad())
+    throw std::runtime_error("the key/value cache has no gradient: call it under torch.no_grad() or on detached tensors");
+  at::Tensor r = t;
+  const bool ok = t.stride(2) == 1 && t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 && t.stride(1) >= 0 &&
+                  t.stride(0) >= 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (!ok) r = t.contiguous();
+  if (reinterpret_cast<uintptr_t>(r.data_ptr()) % 16) r = r.clone();
+  *sb = r.stride(0);
+  *st = r.stride(1);
+  return r;
 }
+
+const __nv_bfloat16* bf16_ptr(const at::Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
+
+// [n] whole numbers as contiguous int32 (undefined: not given).
+at::Tensor kv_index(const std::optional<at::Tensor>& t, int64_t n, const at::Tensor& codes, const char* name) {
+  if (!t.has_value() || !t->defined()) return at::Tensor();
+  if (!at::isIntegralType(t->scalar_type(), false)) type_error(name, " holds whole numbers, not ", t->scalar_type());
+  if (t->dim() != 1 || t->size(0) != n) value_error(name, " ", t->sizes(), ", expected [", n, "]");
+  if (!same_device(*t, codes)) value_error(name, " on ", t->device(), ", the cache on ", codes.device());
+  return t->scalar_type() == at::kInt && t->is_contiguous() ? *t : t->to(at::kInt).contiguous();
+}
+
+const int* int_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
 
 void kv_write(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
               const at::Tensor& err, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& rows,
@@ -1010,15 +1050,21 @@ void kv_write(const at::Tensor& codes, const at::Tensor& scales, const at::Tenso
   c10::cuda::CUDAGuard guard(codes.device());
   mdl::KvWriteArgs a;
   a.c = kv_cache_of(codes, scales, table, lengths, err);
-  TORCH_CHECK(k.dim() == 3, "k must be [n, T, G * hd]");
+  if (k.dim() != 3) value_error("k ", k.sizes(), ", expected [rows, tokens, width]");
   const int64_t n = k.size(0), T = k.size(1), width = static_cast<int64_t>(a.c.G) * a.c.hd;
   TORCH_CHECK(T < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_write: sizes");
-  a.k = kv_rows(k, n, T, width, a.c, codes.device(), "k", &a.k_sb, &a.k_st);
-  a.v = kv_rows(v, n, T, width, a.c, codes.device(), "v", &a.v_sb, &a.v_st);
-  a.rows = kv_index(rows, n, codes.device(), "rows");
-  a.start = kv_index(start, n, codes.device(), "start");
-  a.kstart = kv_index(kstart, n, codes.device(), "kstart");
-  TORCH_CHECK(a.rows != nullptr || n <= a.c.R, "kv_write: more source rows than cache rows");
+  const at::Tensor kr = kv_rows(k, n, T, width, codes, "k", &a.k_sb, &a.k_st);
+  const at::Tensor vr = kv_rows(v, n, T, width, codes, "v", &a.v_sb, &a.v_st);
+  const at::Tensor ri = kv_index(rows, n, codes, "rows"), fi = kv_index(kstart, n, codes, "kstart");
+  at::Tensor si = kv_index(start, n, codes, "start");
+  if (!ri.defined() && n != a.c.R) value_error(n, " source rows for ", a.c.R, " cache rows: give rows");
+  // the kernel writes the lengths
+  if (si.defined() && si.storage().data_ptr().get() == lengths.storage().data_ptr().get()) si = si.clone();
+  a.k = bf16_ptr(kr);
+  a.v = bf16_ptr(vr);
+  a.rows = int_ptr(ri);
+  a.start = int_ptr(si);
+  a.kstart = int_ptr(fi);
   a.n = static_cast<int>(n);
   a.T = static_cast<int>(T);
   int launches = 0;
@@ -1026,53 +1072,59 @@ void kv_write(const at::Tensor& codes, const at::Tensor& scales, const at::Tenso
   g_launches += launches;
 }
 
-void kv_read(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
-             const at::Tensor& err, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& rows,
-             const std::optional<at::Tensor>& start) {
+std::pair<at::Tensor, at::Tensor> kv_read(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table,
+                                          const at::Tensor& lengths, const at::Tensor& err, int64_t count,
+                                          const std::optional<at::Tensor>& rows, const std::optional<at::Tensor>& start,
+                                          bool fp32) {
   c10::cuda::CUDAGuard guard(codes.device());
   mdl::KvReadArgs a;
   a.c = kv_cache_of(codes, scales, table, lengths, err);
-  TORCH_CHECK(k.device() == codes.device() && v.device() == codes.device() && k.is_contiguous() && v.is_contiguous() &&
-                  k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() &&
-                  k.size(2) == static_cast<int64_t>(a.c.G) * a.c.hd &&
-                  (k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat),
-              "kv_read: k and v must be contiguous bf16 or fp32 [n, count, G * hd]");
-  const int64_t n = k.size(0);
-  TORCH_CHECK(k.size(1) < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_read: sizes");
+  const int64_t n = rows.has_value() ? rows->size(0) : a.c.R;
+  if (count < 0) value_error("count ", count);
+  TORCH_CHECK(count < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_read: sizes");
+  const at::Tensor ri = kv_index(rows, n, codes, "rows"), si = kv_index(start, n, codes, "start");
+  const auto options = codes.options().dtype(fp32 ? at::kFloat : at::kBFloat16);
+  at::Tensor k = at::empty({n, count, static_cast<int64_t>(a.c.G) * a.c.hd}, options);
+  at::Tensor v = at::empty(k.sizes(), options);
   a.out_k = k.data_ptr();
   a.out_v = v.data_ptr();
-  a.fp32 = k.scalar_type() == at::kFloat;
-  a.rows = kv_index(rows, n, codes.device(), "rows");
-  a.start = kv_index(start, n, codes.device(), "start");
-  TORCH_CHECK(a.rows != nullptr || n <= a.c.R, "kv_read: more rows than the cache has");
+  a.fp32 = fp32;
+  a.rows = int_ptr(ri);
+  a.start = int_ptr(si);
   a.n = static_cast<int>(n);
-  a.count = static_cast<int>(k.size(1));
+  a.count = static_cast<int>(count);
   check(mdl::kv_read(a, stream_of(codes)), "kv_read");
   g_launches += 1;
+  return {k, v};
 }
 
-void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table, const at::Tensor& lengths,
-               const at::Tensor& err, const at::Tensor& q, const std::optional<at::Tensor>& k_new,
-               const std::optional<at::Tensor>& v_new, const std::optional<at::Tensor>& rows, const at::Tensor& out,
-               int64_t window, int64_t sinks, double scale) {
+at::Tensor kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& table,
+                     const at::Tensor& lengths, const at::Tensor& err, const at::Tensor& q,
+                     const std::optional<at::Tensor>& rows, const std::optional<at::Tensor>& k_new,
+                     const std::optional<at::Tensor>& v_new, int64_t window, int64_t sinks, double scale) {
   c10::cuda::CUDAGuard guard(codes.device());
   mdl::KvAttendArgs a;
   a.c = kv_cache_of(codes, scales, table, lengths, err);
-  TORCH_CHECK(q.dim() == 3 && q.size(2) % (static_cast<int64_t>(a.c.G) * a.c.hd) == 0 && q.size(2) > 0,
-              "q must be [B, N, H * hd] with H a multiple of the key heads");
-  const int64_t B = q.size(0), N = q.size(1), width = q.size(2), kw = static_cast<int64_t>(a.c.G) * a.c.hd;
+  const int64_t kw = static_cast<int64_t>(a.c.G) * a.c.hd;
+  if (q.dim() != 3 || q.size(2) == 0 || q.size(2) % kw)
+    value_error("q ", q.sizes(), ": the width must be a multiple of ", a.c.G, " key heads of ", a.c.hd);
+  if (window < 0 || sinks < 0) value_error("window ", window, " and sinks ", sinks, " must not be negative");
+  if (k_new.has_value() != v_new.has_value()) value_error("k_new and v_new come together");
+  const int64_t B = q.size(0), N = q.size(1), width = q.size(2);
   TORCH_CHECK(B < (int64_t{1} << 30) && N * width / a.c.hd < (int64_t{1} << 30), "kv_attend: sizes");
-  a.q = kv_rows(q, B, N, width, a.c, codes.device(), "q", &a.q_sb, &a.q_sn);
-  TORCH_CHECK(k_new.has_value() == v_new.has_value(), "k_new and v_new come together");
+  const at::Tensor qr = kv_rows(q, B, N, width, codes, "q", &a.q_sb, &a.q_sn);
+  at::Tensor kr, vr;
   if (k_new.has_value()) {
-    a.kn = kv_rows(*k_new, B, N, kw, a.c, codes.device(), "k_new", &a.kn_sb, &a.kn_sn);
-    a.vn = kv_rows(*v_new, B, N, kw, a.c, codes.device(), "v_new", &a.vn_sb, &a.vn_sn);
+    kr = kv_rows(*k_new, B, N, kw, codes, "k_new", &a.kn_sb, &a.kn_sn);
+    vr = kv_rows(*v_new, B, N, kw, codes, "v_new", &a.vn_sb, &a.vn_sn);
+    a.kn = bf16_ptr(kr);
+    a.vn = bf16_ptr(vr);
   }
-  a.rows = kv_index(rows, B, codes.device(), "rows");
-  TORCH_CHECK(a.rows != nullptr || B <= a.c.R, "kv_attend: more batch rows than cache rows");
-  TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.is_contiguous() &&
-                  out.sizes() == q.sizes(), "out must be contiguous bf16 like q");
-  TORCH_CHECK(window >= 0 && sinks >= 0, "window and sinks must not be negative");
+  const at::Tensor ri = kv_index(rows, B, codes, "rows");
+  if (!ri.defined() && B != a.c.R) value_error(B, " batch rows for ", a.c.R, " cache rows: give rows");
+  at::Tensor out = at::empty({B, N, width}, q.options());
+  a.q = bf16_ptr(qr);
+  a.rows = int_ptr(ri);
   a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   a.B = static_cast<int>(B);
   a.N = static_cast<int>(N);
@@ -1080,9 +1132,9 @@ void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tens
   // positions stay below 2^31: larger ones would see the same
   a.window = static_cast<int>(std::min<int64_t>(window, int64_t{1} << 30));
   a.sinks = static_cast<int>(std::min<int64_t>(sinks, int64_t{1} << 30));
-  a.scale = static_cast<float>(scale);
+  a.scale = scale != 0 ? static_cast<float>(scale) : 1.f / std::sqrt(static_cast<float>(a.c.hd));
   at::Tensor ws;
-  const long long need = mdl::kv_attend_workspace(a);
+  const long long need = B > 0 && N > 0 ? mdl::kv_attend_workspace(a) : 0;
   if (need > 0) {
     ws = at::empty({need}, q.options().dtype(at::kFloat));
     a.partial = ws.data_ptr<float>();
@@ -1090,6 +1142,7 @@ void kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at::Tens
   int launches = 0;
   check(mdl::kv_attend(a, stream_of(codes), &launches), "kv_attend");
   g_launches += launches;
+  return out;
 }
 
 // ------------------------------------------------------------------ windowed attention
@@ -1178,6 +1231,39 @@ at::Tensor window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, cons
   return dqkv;
 }
 
+// The differentiable operator: saves what the backward reads, off the interpreter's lock.
+struct WindowedAttention : public torch::autograd::Function<WindowedAttention> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv, const at::Tensor& kstart,
+                            int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale,
+                            const at::Tensor& err) {
+    const bool keep = qkv.requires_grad();
+    auto [out, out_lo, lse] = window_attn_fwd(qkv, kstart, H, G, Lq, window, sinks, scale, err, keep);
+    if (keep) {
+      ctx->save_for_backward({qkv, kstart, out, *out_lo, lse});
+      ctx->saved_data["err"] = err;
+      ctx->saved_data["args"] = std::vector<int64_t>{H, G, Lq, window, sinks};
+      ctx->saved_data["scale"] = scale;
+    }
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["args"].toIntVector();
+    at::Tensor dout = grads[0].to(at::kBFloat16).contiguous();
+    if (reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16) dout = dout.clone();
+    at::Tensor d = window_attn_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], dout, n[0], n[1], n[2], n[3], n[4],
+                                   ctx->saved_data["scale"].toDouble(), ctx->saved_data["err"].toTensor());
+    return {d, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor windowed_attention(const at::Tensor& qkv, const at::Tensor& kstart, int64_t H, int64_t G, int64_t Lq,
+                              int64_t window, int64_t sinks, double scale, const at::Tensor& err) {
+  return WindowedAttention::apply(qkv, kstart, H, G, Lq, window, sinks, scale, err);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1243,6 +1329,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("Lq"), py::arg("causal"), py::arg("scale"), py::arg("err") = py::none(), py::arg("ktail") = 0,
         py::arg("kexcl") = 0);
   m.def("position_add", &position_add);
+  m.def("windowed_attention", &windowed_attention);
   m.def("window_attn_fwd", &window_attn_fwd);
   m.def("window_attn_bwd", &window_attn_bwd);
   m.def("kv_write", &kv_write);

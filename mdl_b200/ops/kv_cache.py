@@ -116,44 +116,27 @@ class QuantizedKVCache:
 
 
 # ----------------------------------------------------------------------------- checks
+# (of the definitions on the CPU; the native entry points make the same ones)
 def _index(t: torch.Tensor | None, n: int, cache: QuantizedKVCache, name: str) -> torch.Tensor | None:
-    if t is None or (t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and t.device == cache.device
-                     and t.is_contiguous()):
-        return t
-    if t.dtype != torch.int32:
-        if t.is_floating_point() or t.dtype == torch.bool:
-            raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
-        t = t.to(torch.int32)
+    if t is None:
+        return None
+    if t.is_floating_point() or t.dtype == torch.bool:
+        raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
     if t.shape != (n,):
         raise ValueError(f"{name} {tuple(t.shape)}, expected ({n},)")
     if t.device != cache.device:
         raise ValueError(f"{name} on {t.device}, the cache on {cache.device}")
-    return t.contiguous()
+    return t
 
 
-def _tokens(t: torch.Tensor, width: int, cache: QuantizedKVCache, name: str) -> torch.Tensor:
-    """``[n, T, width]`` with a dense last dimension, 16-byte aligned rows on CUDA."""
-
+def _tokens(t: torch.Tensor, width: int, cache: QuantizedKVCache, name: str) -> None:
     if t.dim() != 3 or t.shape[2] != width:
         raise ValueError(f"{name} {tuple(t.shape)}, expected [rows, tokens, {width}]")
     if t.device != cache.device:
         raise ValueError(f"{name} on {t.device}, the cache on {cache.device}")
-    if t.device.type == "cuda":
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"{name} must be bf16, not {t.dtype}")
-        s0, s1, s2 = t.stride()
-        if s2 != 1 or s1 % 8 or s0 % 8 or s1 < 0 or s0 < 0 or t.data_ptr() % 16:
-            t = t.contiguous()
-            if t.data_ptr() % 16:
-                t = t.clone()
-    elif not t.is_floating_point():
+    if not t.is_floating_point():
         raise TypeError(f"{name} must be a floating type, not {t.dtype}")
-    return t
-
-
-def _no_grad(a: torch.Tensor, b: torch.Tensor | None, c: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
-                                    or (c is not None and c.requires_grad)):
+    if torch.is_grad_enabled() and t.requires_grad:
         raise RuntimeError("the key/value cache has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -205,24 +188,19 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, st
     the end of what was written."""
 
     with trace_range("mdl.kv_cache.write"):
+        if cache.err is not None:
+            ext().kv_write(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, k, v, rows, start, kstart)
+            return
         width = cache.kv_heads * cache.head_dim
-        _no_grad(k, v, None)
-        k, v = _tokens(k, width, cache, "k"), _tokens(v, width, cache, "v")
+        _tokens(k, width, cache, "k")
+        _tokens(v, width, cache, "v")
         n = k.shape[0]
         if v.shape != k.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
         if rows is None and n != cache.rows:
             raise ValueError(f"{n} source rows for {cache.rows} cache rows: give rows")
-        rows = _index(rows, n, cache, "rows")
-        kstart = _index(kstart, n, cache, "kstart")
-        start = _index(start, n, cache, "start")
-        if cache.device.type != "cuda":
-            kv_cache_write_reference(cache, k, v, start, kstart, rows)
-            return
-        if start is not None and start.untyped_storage().data_ptr() == cache.lengths.untyped_storage().data_ptr():
-            start = start.clone()  # the kernel writes the lengths
-        ext().kv_write(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, k, v, rows,
-                       start, kstart)
+        kv_cache_write_reference(cache, k, v, _index(start, n, cache, "start"), _index(kstart, n, cache, "kstart"),
+                                 _index(rows, n, cache, "rows"))
 
 
 # ----------------------------------------------------------------------------- read
@@ -234,30 +212,27 @@ def kv_cache_read(cache: QuantizedKVCache, count: int, start: torch.Tensor | Non
     length. fp32 holds them exactly; bf16 rounds once."""
 
     with trace_range("mdl.kv_cache.read"):
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise TypeError(f"the cache reads back bf16 or fp32, not {dtype}")
+        if cache.err is not None:
+            return ext().kv_read(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, count, rows, start,
+                                 dtype is torch.float32)
         if count < 0:
             raise ValueError(f"count {count}")
-        if dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"the cache reads back bf16 or fp32, not {dtype}")
         n = cache.rows if rows is None else rows.shape[0]
         rows = _index(rows, n, cache, "rows")
         start = _index(start, n, cache, "start")
         width = cache.kv_heads * cache.head_dim
-        if cache.device.type != "cuda":
-            r = (torch.arange(n) if rows is None else rows.long()).view(-1, 1)
-            pos = (0 if start is None else start.long().view(-1, 1)) + torch.arange(count)
-            if bool((pos < 0).any()):
-                raise ValueError("key/value cache: start outside the row")
-            live = pos < cache.lengths[r].long()
-            x = torch.zeros(n, count, cache.kv_heads, 2, cache.head_dim)
-            i, ti = live.expand(n, count).nonzero(as_tuple=True)
-            x[i, ti] = cache.values(r.expand(n, count)[i, ti], pos.expand(n, count)[i, ti])
-            x = x.to(dtype)
-            return x[..., 0, :].reshape(n, count, width), x[..., 1, :].reshape(n, count, width)
-        k = torch.empty(n, count, width, dtype=dtype, device=cache.device)
-        v = torch.empty_like(k)
-        ext().kv_read(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, k, v, rows,
-                      start)
-        return k, v
+        r = (torch.arange(n) if rows is None else rows.long()).view(-1, 1)
+        pos = (0 if start is None else start.long().view(-1, 1)) + torch.arange(count)
+        if bool((pos < 0).any()):
+            raise ValueError("key/value cache: start outside the row")
+        live = pos < cache.lengths[r].long()
+        x = torch.zeros(n, count, cache.kv_heads, 2, cache.head_dim)
+        i, ti = live.expand(n, count).nonzero(as_tuple=True)
+        x[i, ti] = cache.values(r.expand(n, count)[i, ti], pos.expand(n, count)[i, ti])
+        x = x.to(dtype)
+        return x[..., 0, :].reshape(n, count, width), x[..., 1, :].reshape(n, count, width)
 
 
 # ----------------------------------------------------------------------------- attend
@@ -314,26 +289,24 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKVCache, rows: torch.Tenso
     ``g * heads / kv_heads ..`` share key head ``g``. ``scale`` defaults to ``head_dim ** -0.5``."""
 
     with trace_range("mdl.attention.cached"):
+        if cache.err is not None:
+            return ext().kv_attend(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, q, rows, k_new,
+                                   v_new, window, sinks, scale or 0.0)
         G, hd = cache.kv_heads, cache.head_dim
         if q.dim() != 3 or q.shape[2] % (G * hd) or q.shape[2] == 0:
             raise ValueError(f"q {tuple(q.shape)}: the width must be a multiple of {G} key heads of {hd}")
-        _no_grad(q, k_new, v_new)
         if window < 0 or sinks < 0:
             raise ValueError(f"window {window} and sinks {sinks} must not be negative")
         if (k_new is None) != (v_new is None):
             raise ValueError("k_new and v_new come together")
         B, N, width = q.shape
-        q = _tokens(q, width, cache, "q")
+        _tokens(q, width, cache, "q")
         if rows is None and B != cache.rows:
             raise ValueError(f"{B} batch rows for {cache.rows} cache rows: give rows")
         rows = _index(rows, B, cache, "rows")
         if k_new is not None:
-            k_new, v_new = _tokens(k_new, G * hd, cache, "k_new"), _tokens(v_new, G * hd, cache, "v_new")
+            _tokens(k_new, G * hd, cache, "k_new")
+            _tokens(v_new, G * hd, cache, "v_new")
             if k_new.shape[:2] != (B, N) or v_new.shape[:2] != (B, N):
                 raise ValueError(f"k_new {tuple(k_new.shape)} and v_new {tuple(v_new.shape)} for {B} x {N} queries")
-        if cache.device.type != "cuda":
-            return cached_attention_reference(q, cache, rows, k_new, v_new, window, sinks, scale).to(q.dtype)
-        out = torch.empty(B, N, width, dtype=torch.bfloat16, device=q.device)
-        ext().kv_attend(cache.codes, cache.scales, cache.table, cache.lengths, cache.err, q, k_new,
-                        v_new, rows, out, int(window), int(sinks), float(scale) if scale else 1.0 / math.sqrt(hd))
-        return out
+        return cached_attention_reference(q, cache, rows, k_new, v_new, window, sinks, scale).to(q.dtype)

@@ -75,26 +75,6 @@ def window_attention_bwd(qkv, ks, out, out_lo, lse, dout, heads: int, kv_heads: 
                                  error_word(qkv.device))
 
 
-class WindowedAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, kstart, *args):
-        keep = ctx.needs_input_grad[0]
-        out, out_lo, lse = window_attention_fwd(qkv, kstart, *args, keep=keep)
-        if keep:
-            ctx.save_for_backward(qkv, kstart, out, out_lo, lse)
-            ctx.args = args
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        qkv, ks, out, out_lo, lse = ctx.saved_tensors
-        if dout.dtype is not torch.bfloat16 or not dout.is_contiguous():
-            dout = dout.to(torch.bfloat16).contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        return window_attention_bwd(qkv, ks, out, out_lo, lse, dout, *ctx.args), *([None] * 7)
-
-
 def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: int, window: int, sinks: int = 0,
                        kv_heads: int | None = None, scale: float | None = None) -> torch.Tensor:
     """See the module's text; ``scale`` defaults to ``head_dim ** -0.5``."""
@@ -132,5 +112,5 @@ def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: 
         ks = kstart
         if ks.dtype is not torch.int32 or not ks.is_contiguous():
             ks = ks.to(torch.int32).contiguous()
-        return WindowedAttentionFn.apply(qkv, ks, heads, G, lq, min(window, Lk), min(sinks, Lk),
-                                         float(scale) if scale else 1.0 / math.sqrt(hd))
+        return ext().windowed_attention(qkv, ks, heads, G, lq, min(window, Lk), min(sinks, Lk),
+                                        float(scale) if scale else 0.0, error_word(qkv.device))
