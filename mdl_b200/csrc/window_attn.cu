@@ -277,10 +277,10 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16* dst, int hd) {
 // Positions are relative to the first valid token.
 
 struct alignas(16) Item {
-  int h, b, kst, n;    // head, sample, first valid token, steps (-1: no more items)
-  int t, cs, k0, qf;   // tile; steps: cs from 0, then from k0 on (KEYS: cs a head, from k0); first query
-  int len;             // valid tokens
-  int j0, part, pad;   // first step, and slot of the partial sums (-1: none)
+  int n, t, cs, k0;       // steps (-1: no more items); tile; steps: cs from 0, then from k0 on (KEYS: cs a head, from k0)
+  int qf, len, j0, part;  // first query, valid tokens; first step, and slot of the partial sums (-1: none)
+  int h, b, kst, row0;    // head, sample, first valid token; query row of the tile's first row
+  long long out, lse;     // elements from the start of out (of dqkv in the backward) and of lse to that row
 };
 
 // Query steps of key tile t: from k0 on, cs a query head.
@@ -441,6 +441,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       const int slot = items % RECS, sq = items & 1;
       // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
       if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
+      w.it.row0 = it.kst + TILE * it.t - q0;
+      w.it.lse = (static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.row0;
+      w.it.out = ((static_cast<long long>(it.b) * p.Lq + it.row0) * p.H + it.h) * HD;
       if (lane == 0) {
         recs[slot] = it;
         mbar_arrive(&rec_full[slot]);
@@ -561,6 +564,7 @@ __global__ void __launch_bounds__(F_THREADS, 2)
     const int r = quarter * 32 + lane;
     constexpr int OC = HD / 2;
     const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int row_stride = p.H * HD;
     const uint32_t tS_own = base + half * 64, tP_own = base + 128 + half * 32, tO_own = base + 192 + half * OC;
     bool ok = true;
     int g = 0, items = 0;
@@ -570,15 +574,13 @@ __global__ void __launch_bounds__(F_THREADS, 2)
       const int k = items - 1, slot = k % RECS;
       const Item& it = recs[slot];
       const float l = sSum[((k & 1) * 2) * TILE + r] + sSum[((k & 1) * 2 + 1) * TILE + r];
-      const int qi = it.kst + TILE * it.t + r - (p.Lk - p.Lq);
-      const bool real = qi >= 0 && qi < p.Lq;
-      const long long row = static_cast<long long>(it.b) * p.Lq + qi;
-      const long long o = (row * p.H + it.h) * HD + half * OC;
-      if (real && half == 0)
-        p.lse[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + qi] = sRef[(k & 1) * TILE + r] + lg2(l);
+      const bool real = static_cast<unsigned>(it.row0 + r) < static_cast<unsigned>(p.Lq);
+      const long long o = it.out + r * row_stride;
+      const long long ls = it.lse + r;
       __syncwarp();
       if (lane == 0) mbar_arrive(&rec_empty[slot]);
-      const float inv = 1.f / l;
+      if (real && half == 0) p.lse[ls] = sRef[(k & 1) * TILE + r] + lg2(l);
+      const float inv = __fdividef(1.f, l);
 #pragma unroll
       for (int c = 0; c < OC / 16; ++c) {
         uint32_t ov[16];
@@ -594,10 +596,10 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          reinterpret_cast<uint4*>(p.out + o + c * 16)[e] =
+          reinterpret_cast<uint4*>(p.out + o + half * OC + c * 16)[e] =
               make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
           if (p.out_lo != nullptr)
-            reinterpret_cast<uint4*>(p.out_lo + o + c * 16)[e] =
+            reinterpret_cast<uint4*>(p.out_lo + o + half * OC + c * 16)[e] =
                 make_uint4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
         }
       }
@@ -608,9 +610,9 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         ok = false;
         break;
       }
-      const int n = recs[slot].n;
+      const int4 first = *reinterpret_cast<const int4*>(&recs[slot]);
+      const int n = first.x, t = first.y, cs = first.z, k0 = first.w;
       if (n < 0) break;
-      const int t = recs[slot].t, cs = recs[slot].cs, k0 = recs[slot].k0;
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < n; ++j, ++g) {
         if (!warp_wait(s_full, g & 1, p.err, abort_flag)) {
@@ -662,26 +664,26 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         row_max[half * TILE + r] = mx;
         pair_sync(1 + quarter);
         mx = fmaxf(mx, row_max[(half ^ 1) * TILE + r]);
-        if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        if (j == 0) {
+          m = mx;
+        } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float m_new = fmaxf(m, mx);
           const float alpha = m_new == -CUDART_INF_F ? 1.f : ex2(m - m_new);
           m = m_new;
           l *= alpha;
-          if (j > 0) {
-            if (!warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+          if (!warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < OC / 8; ++c) {  // few registers at a time: the scores are held
-              uint32_t ov[8];
-              tmem_ld8(tO_own + c * 8, ov);
-              tmem_wait_ld();
+          for (int c = 0; c < OC / 8; ++c) {  // few registers at a time: the scores are held
+            uint32_t ov[8];
+            tmem_ld8(tO_own + c * 8, ov);
+            tmem_wait_ld();
 #pragma unroll
-              for (int d = 0; d < 8; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha);
-              tmem_st8(tO_own + c * 8, ov);
-            }
+            for (int d = 0; d < 8; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha);
+            tmem_st8(tO_own + c * 8, ov);
           }
         }
         if (g > 0 && !warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {  // the last P was consumed
@@ -840,6 +842,9 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       const int slot = items % RECS;
       // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
       if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
+      w.it.row0 = ya - q0;
+      w.it.lse = (static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.row0;
+      w.it.out = (trow0 + ya) * width + (KEYS ? p.H + it.h : it.h) * HD;
       if (lane == 0) {
         recs[slot] = it;
         mbar_arrive(&rec_full[slot]);
@@ -1004,6 +1009,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS_own = tS + lane_off + 32 * half, tDP_own = tDP + lane_off + 32 * half;
     const uint32_t tP_own = tP + lane_off + PAIR_STEP * half, tDS_own = tDS + lane_off + PAIR_STEP * half;
+    const int row_stride = (p.H + 2 * p.G) * HD;
     bool ok = true;
     int items = 0, g = 0;
     // keys: dV or dK; queries: half of dQ
@@ -1017,9 +1023,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       const Item& it = recs[k % RECS];
       const int own = TILE * it.t + r;
       const bool store = own < it.len && (KEYS || own >= it.qf);
-      const int head = KEYS ? (half == 0 ? p.H + p.G + it.h : p.H + it.h) : it.h;
-      __nv_bfloat16* dst = p.dqkv + (static_cast<long long>(it.b) * p.Lk + it.kst + own) * (p.H + 2 * p.G) * HD +
-                           head * HD + col0;
+      __nv_bfloat16* dst = p.dqkv + it.out + r * row_stride + (KEYS && half == 0 ? p.G * HD : col0);
       const float f = (KEYS && half == 0) ? 1.f : p.scale;
       float4* sums = KEYS && it.part >= 0
                          ? reinterpret_cast<float4*>(p.partial + ((static_cast<long long>(it.part) * TILE + r) * 2 + half) * HD)
@@ -1054,17 +1058,19 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         ok = false;
         break;
       }
-      const Item& it = recs[slot];
-      const int n = it.n;
+      const Item& it = recs[slot];  // what only a mask or the item's ends need stays there
+      const int4 first = *reinterpret_cast<const int4*>(&it);
+      const int n = first.x, t = first.y, cs = first.z, k0 = first.w, own = TILE * t + r;
       if (n < 0) break;
-      const int cs = it.cs, k0 = it.k0, t = it.t, own = TILE * t + r;
       float row_lse = 0.f, row_d = 0.f;
       if constexpr (!KEYS) {
         // D of the row from dO (shared memory) and the output (16 bits: out + out_lo), half of
         // the head a warp; the output's loads are under way while the tile is waited for
         constexpr int V = HD / 16;  // 16-byte pieces of half a row
         const bool real = own >= it.qf && own < it.len;
-        const long long o = ((static_cast<long long>(it.b) * p.Lq + it.kst + own - q0) * p.H + it.h) * HD + half * (HD / 2);
+        const long long ls = recs[slot].lse + r;  // (sample, head, query row)
+        const long long o = ((static_cast<long long>(recs[slot].b) * p.Lq + recs[slot].row0 + r) * p.H + recs[slot].h) * HD +
+                            half * (HD / 2);
         uint4 hv[V], lv[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
@@ -1098,8 +1104,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         if (lane == 0) mbar_arrive(a_empty);
         pair_sync(1 + quarter);
         row_d = part[r] + part[TILE + r];
-        if (half == 0 && real)
-          p.dsum[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.kst + own - q0] = row_d;
+        if (half == 0 && real) p.dsum[ls] = row_d;
       }
       for (int j = 0, s_ = KEYS && it.j0 > 0 ? it.j0 % cs : 0; j < n; ++j, ++s_, ++g) {
         if (KEYS && s_ == cs) s_ = 0;
