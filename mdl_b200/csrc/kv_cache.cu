@@ -60,7 +60,9 @@ __device__ __forceinline__ long long slot_base(const KvCache& c, int pg, int g, 
 }
 
 // ============================================================================ write
-// A lane holds 16 values of a row, hd / 16 lanes the row.
+// A lane holds 16 values of a row, hd / 16 lanes the row: wide loads, a maximum of one or two
+// shuffles, and a store of 8 bytes. Bound by memory: 256 rows of up to 2,000 tokens, 8 heads of 32, K
+// and V: 104 us, 5.5 TB/s read and written (434,000 tokens of histories of unequal length).
 //
 // c = rint(x / s) without a division: x / s of two bf16 numbers is either a tie (an odd
 // multiple of 1/2) or at least 1/1020 away from one, and |x / s| <= 7.03 (up to 8-bit
@@ -197,7 +199,8 @@ __global__ void kv_length_kernel(KvWriteArgs a) {
 }
 
 // ============================================================================ read
-// Thread = one code word (8 values) of K and of V.
+// Thread = one code word (8 values) of K and of V. Bound by memory, the bf16 that it writes: 384
+// rows of up to 2,048 tokens, 8 heads of 32: 181 us, 5.5 TB/s read and written.
 template <int HD, bool F32>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chunk, int chunks) {
   constexpr int LPU = HD / 8;
@@ -268,6 +271,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 // operation), since the same shortcut over a long sum of keys would cancel. The scales enter
 // in fp32: s_k multiplies the scores, s_v the probabilities.
 //
+// Bound: the instructions that expand the codes (about 12 a key of 64 values and warp, with the
+// softmax's) and not memory, whose bytes are a quarter of bf16's. 24 single tokens over 131,071
+// keys, 8 query heads on 2 key heads of 64: 117 us, 3.2 TB/s of cache; 1,024 samples of 32
+// candidates, 8 heads of 32, window 512 of 2,000 keys: 173 us, 103 TFLOP/s; one token over 501
+// keys: 4.5 us.
 constexpr uint32_t kMagic = 0x43004300u;   // bf16 128, twice
 constexpr uint32_t kOffset = 0x43084308u;  // bf16 136, twice
 
@@ -371,6 +379,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     split = static_cast<int>(blockIdx.x - item * splits);
     part = split * WPI + warp;
     parts = splits * WPI;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join of the splits may take its place
   }
   const int qb = static_cast<int>(item % qblocks);
   const int g = static_cast<int>(item / qblocks % c.G);
@@ -551,7 +560,15 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
 #pragma unroll 1
   for (int i = part; i < total; i += parts) {
     const int k0 = step_key(i);
-    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], phase)) && !ring_wait(&full[st], phase, c.err)) break;
+    if (!__all_sync(0xffffffffu, mbar_try_wait(&full[st], phase)) && !ring_wait(&full[st], phase, c.err)) {
+      // the copies of the stages behind it land before the block may end
+      for (int s = 1; s < RING && i + s * parts < total; ++s) {
+        phase ^= st + 1 == RING ? 1 : 0;
+        st = st + 1 == RING ? 0 : st + 1;
+        ring_wait(&full[st], phase, c.err);
+      }
+      break;
+    }
     const uint8_t* sk = ring + st * STEP;
     const uint32_t* kw = reinterpret_cast<const uint32_t*>(sk) + row8 * (HD / 8) + t * KW;
     const uint32_t* vw = reinterpret_cast<const uint32_t*>(sk + KT * TILE_CODES) + t * (HD / 8) + (HD == 64 ? g8 : g8 >> 1);
@@ -914,13 +931,16 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   }
 }
 
-// Joins the splits: hd / 4 threads a query row.
+// Joins the splits, a warp a query row: lane s weighs split s (kMaxSplits is a warp), then hd / 4
+// lanes add up 4 dims each, in groups that share the splits. It is launched while the splits are
+// still being computed and waits for them in place.
+constexpr int kMaxSplits = 32;
+
 template <int HD>
 __global__ void __launch_bounds__(128) kv_combine_kernel(KvAttendArgs a, int qblocks, int splits, int cols) {
-  const int group = a.H / a.c.G, M = a.N * group;
-  const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long row = idx / (HD / 4);
-  const int d4 = static_cast<int>(idx % (HD / 4));
+  constexpr int LANES = HD / 4, GROUPS = 32 / LANES;
+  const int group = a.H / a.c.G, M = a.N * group, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= static_cast<long long>(a.B) * a.c.G * M) return;
   const int m = static_cast<int>(row % M);
   const long long bg = row / M;
@@ -928,20 +948,42 @@ __global__ void __launch_bounds__(128) kv_combine_kernel(KvAttendArgs a, int qbl
   const long long b = bg / a.c.G;
   const float* src = a.partial + ((bg * qblocks + m / cols) * splits * cols + m % cols) * (HD + 4);
   const long long step = static_cast<long long>(cols) * (HD + 4);
-  float top = -CUDART_INF_F;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, src[s * step + HD]);
-  const float use = top == -CUDART_INF_F ? 0.f : top;
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < splits; ++s) {
-    const float f = ex2(src[s * step + HD] - use);
-    const float4 y = *reinterpret_cast<const float4*>(src + s * step + 4 * d4);
-    sum = fmaf(src[s * step + HD + 1], f, sum);
-    acc.x = fmaf(y.x, f, acc.x);
-    acc.y = fmaf(y.y, f, acc.y);
-    acc.z = fmaf(y.z, f, acc.z);
-    acc.w = fmaf(y.w, f, acc.w);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float top = -CUDART_INF_F, sum = 0.f;
+  if (lane < splits) {
+    const float2 y = *reinterpret_cast<const float2*>(src + lane * step + HD);
+    top = y.x;
+    sum = y.y;
   }
+  const float own = top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f = ex2(own - (top == -CUDART_INF_F ? 0.f : top));
+  sum *= f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int d4 = lane % LANES, first = lane / LANES;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s0 = 0; s0 < splits; s0 += GROUPS) {
+    const int s = s0 + first;
+    const float w = __shfl_sync(0xffffffffu, f, s & 31);
+    if (s < splits) {
+      const float4 y = *reinterpret_cast<const float4*>(src + s * step + 4 * d4);
+      acc.x = fmaf(y.x, w, acc.x);
+      acc.y = fmaf(y.y, w, acc.y);
+      acc.z = fmaf(y.z, w, acc.z);
+      acc.w = fmaf(y.w, w, acc.w);
+    }
+  }
+#pragma unroll
+  for (int o = LANES; o < 32; o <<= 1) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+  }
+  if (first != 0) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   __nv_bfloat16* dst = a.out + (b * a.N + m / group) * a.H * HD + (g * group + m % group) * HD + 4 * d4;
   *reinterpret_cast<uint2*>(dst) =
@@ -971,10 +1013,24 @@ struct Plan {
   long long items;
 };
 
-// Query rows a block: 8, 16 or, of 32-wide heads, 32 (of 64-wide ones the accumulators of 32 rows
-// leave 8 warps a multiprocessor: 512 candidates of 32 tokens took 168 us instead of 76). One warp an item where the items alone fill the device and
-// each has few keys; else eight warps an item, and several blocks an item while the items
-// leave multiprocessors idle.
+// Query rows a block: the fewest of 8, 16 and (32-wide heads) 32 that hold an item's rows, so that
+// the codes are expanded once. 512 rows of 2,000 cached tokens, 8 heads of 32: 8 queries 113 us in
+// blocks of 8 (166 in 16, 254 in 32); 16 queries 167 us in 16 (207, 256); 32 queries 260 us in 32
+// (400, 324). 64-wide heads stay at 16: the accumulators of 32 rows leave 8 warps a
+// multiprocessor (512 candidates of 32 tokens: 168 us instead of 76).
+//
+// Warps an item, and blocks an item ("splits", joined by a second kernel): whatever has the lowest
+// cost, in keys that a warp passes while its multiprocessor is full. An item costs as much as 80
+// more keys with one warp and 400 with eight (which join in shared memory). With one warp an item
+// the uneven ends count as 1.5 more items, 5 % all told; eight warps of blocks of 32 rows take 35 %
+// longer (one block a multiprocessor). A multiprocessor with few warps is bound by their latency:
+// it counts as if it held 10.6 warps of an item each, or 1.5 blocks of eight.
+// Measured on single queries, 8 heads of 32, one warp an item | eight: 296 rows of 250 keys 12.6 |
+// 24.7 us, 1,000 keys 37.0 | 41.3, 4,000 keys 127 | 119; 64 rows of 1,000 keys 22.1 | 14.5; 32
+// queries a row, 512 rows of 8,000 keys 974 | 1,154. Splits 1 | 2 | 4 | 8 | 16 | 32: 1 row of
+// 32,000 keys 88 | 49 | 29 | 18 | 12 | 12 us; 16 rows of 2,000 keys 10 | 10 | 12 | 16 | 21 | 31,
+// of 32,000 keys 101 | 69 | 68 | 61 | 64 | 73. Over 130 such shapes the choice is 1.2 % slower than
+// the best on average, and by 2 us or 5 % at most.
 Plan plan_of(const KvAttendArgs& a) {
   Plan p;
   const int M = a.N * (a.H / a.c.G);
@@ -982,20 +1038,20 @@ Plan plan_of(const KvAttendArgs& a) {
   p.qblocks = (M + 8 * p.nt - 1) / (8 * p.nt);
   p.items = static_cast<long long>(a.B) * a.c.G * p.qblocks;
   const long long cap = static_cast<long long>(a.c.max_pages) << a.c.page_shift;
-  const long long keys = a.window > 0 ? std::min<long long>(cap, static_cast<long long>(a.window) + a.sinks) : cap;
+  const double keys =
+      static_cast<double>(a.window > 0 ? std::min<long long>(cap, static_cast<long long>(a.window) + a.sinks) : cap);
   const int sms = num_sms();
-  p.wpi = (p.items >= 16LL * sms && keys <= 4096) ? 1 : 8;
+  p.wpi = 1;
   p.splits = 1;
-  if (p.wpi == 8) {
-    // the least (waves of blocks) x (keys a block + what a block costs besides, as keys)
-    const long long slots = 3LL * sms, most = std::min<long long>(32, std::max<long long>(1, keys / 512));
-    double best = 0;
-    for (int n = 1; n <= most; ++n) {
-      const double cost = static_cast<double>((p.items * n + slots - 1) / slots) * (static_cast<double>(keys) / n + 1024);
-      if (n == 1 || cost < 0.98 * best) {
-        best = cost;
-        p.splits = n;
-      }
+  double best = std::max(10.6, 1.05 * (static_cast<double>(p.items) / sms + 1.5)) * (keys + 80);
+  const double slower = p.nt == 4 ? 1.35 : 1.0;
+  for (int n = 1; n <= kMaxSplits; ++n) {
+    const double busiest = static_cast<double>((p.items * n + sms - 1) / sms);  // blocks of a multiprocessor
+    const double cost = slower * std::max(1.5, busiest) * (keys / n + 400) + (n > 1 ? 1000 + 50 * n : 0);
+    if (cost < best) {
+      best = cost;
+      p.wpi = 8;
+      p.splits = n;
     }
   }
   return p;
@@ -1028,20 +1084,24 @@ cudaError_t launch_attend(const KvAttendArgs& a, const Plan& p, cudaStream_t str
 template <int HD>
 cudaError_t attend_hd(const KvAttendArgs& a, const Plan& p, cudaStream_t stream, int* launches) {
   cudaError_t e;
-  if (p.nt == 1) {
-    e = launch_attend<HD, 1>(a, p, stream);
-  } else if (HD == 64 || p.nt == 2) {
-    e = launch_attend<HD, 2>(a, p, stream);
-  } else {
-    if constexpr (HD == 32) e = launch_attend<HD, 4>(a, p, stream);
-  }
+  if (p.nt == 1) e = launch_attend<HD, 1>(a, p, stream);
+  else if (HD == 64 || p.nt == 2) e = launch_attend<HD, 2>(a, p, stream);
+  else e = launch_attend<HD, HD == 64 ? 2 : 4>(a, p, stream);
   *launches += 1;
   if (e != cudaSuccess || p.splits == 1) return e;
-  const long long threads = static_cast<long long>(a.B) * a.N * a.H * (HD / 4);
-  kv_combine_kernel<HD><<<static_cast<unsigned>((threads + 127) / 128), 128, 0, stream>>>(a, p.qblocks, p.splits,
-                                                                                         8 * p.nt);
+  const long long rows = static_cast<long long>(a.B) * a.N * a.H;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kv_combine_kernel<HD>, a, p.qblocks, p.splits, 8 * p.nt);
   *launches += 1;
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace
