@@ -1111,7 +1111,9 @@ at::Tensor kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at
   if (window < 0 || sinks < 0) value_error("window ", window, " and sinks ", sinks, " must not be negative");
   if (k_new.has_value() != v_new.has_value()) value_error("k_new and v_new come together");
   const int64_t B = q.size(0), N = q.size(1), width = q.size(2);
-  TORCH_CHECK(B < (int64_t{1} << 30) && N * width / a.c.hd < (int64_t{1} << 30), "kv_attend: sizes");
+  const int64_t capacity = static_cast<int64_t>(a.c.max_pages) << a.c.page_shift;
+  TORCH_CHECK(B < (int64_t{1} << 30) && N * width / a.c.hd < (int64_t{1} << 30) && capacity + N < (int64_t{1} << 30),
+              "kv_attend: sizes");
   const at::Tensor qr = kv_rows(q, B, N, width, codes, "q", &a.q_sb, &a.q_sn);
   at::Tensor kr, vr;
   if (k_new.has_value()) {
@@ -1129,7 +1131,7 @@ at::Tensor kv_attend(const at::Tensor& codes, const at::Tensor& scales, const at
   a.B = static_cast<int>(B);
   a.N = static_cast<int>(N);
   a.H = static_cast<int>(width / a.c.hd);
-  // positions stay below 2^31: larger ones would see the same
+  // positions stay below 2^30: larger ones would see the same
   a.window = static_cast<int>(std::min<int64_t>(window, int64_t{1} << 30));
   a.sinks = static_cast<int>(std::min<int64_t>(sinks, int64_t{1} << 30));
   a.scale = scale != 0 ? static_cast<float>(scale) : 1.f / std::sqrt(static_cast<float>(a.c.hd));

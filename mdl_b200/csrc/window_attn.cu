@@ -47,13 +47,16 @@ constexpr int BOX = 64;                 // rows of a TMA box, and of a step of t
 constexpr int TILE_BYTES = TILE * 128;  // 128-byte rows: 64 columns, the head's hd first
 constexpr float kLog2e = 1.4426950408889634f;
 
-constexpr int F_THREADS = 320, F_TMEM = 256;
-constexpr int RECS = 4;                         // item records in flight
-constexpr int TAIL = 512;                       // barriers and item records
-// Q[2] | K[2] | V[2] | row maxima and sums of the column halves, [2][2][128] each | references [2][128]
-constexpr int F_SMEM = 1024 + 6 * TILE_BYTES + 10 * TILE * 4 + TAIL;
-constexpr int B_THREADS = 320, B_TMEM = 256, B_STAGES = 4;
+constexpr int RECS = 4;                 // item records in flight
 constexpr int BOX_BYTES = BOX * 128;
+constexpr int TAIL = 512;               // barriers and item records of the backward
+constexpr int CHAINS = 2, F_THREADS = 384, F_TMEM = 256, F_STAGES = 2;
+constexpr int F_BARS = 9 + 2 * RECS + 2 * F_STAGES;
+// a chain: Q | K[2] | V[2]; then the item records and barriers of both chains
+constexpr int F_CHAIN = TILE_BYTES + 2 * F_STAGES * BOX_BYTES;
+constexpr int F_TAIL = 1024;
+constexpr int F_SMEM = 1024 + CHAINS * F_CHAIN + F_TAIL;
+constexpr int B_THREADS = 320, B_TMEM = 256, B_STAGES = 4;
 // stationary pair | streamed pair [4] | lse, D of the streamed rows [4][64] (or lse of the
 // stationary rows [128]) | halves of D [2][2][128] | tail
 constexpr int B_SMEM = 1024 + 2 * TILE_BYTES + 2 * B_STAGES * BOX_BYTES + 2 * B_STAGES * BOX * 4 + 4 * TILE * 4 + TAIL;
@@ -113,18 +116,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -174,7 +165,7 @@ __device__ __forceinline__ uint64_t desc_of(const void* base) { return make_smem
 __device__ __forceinline__ uint64_t desc_mn_of(const void* base) {
   return make_smem_desc(smem_u32(base), TILE_BYTES, 1024);
 }
-constexpr uint32_t K_STEP = 2, MN_STEP = 128, TILE_UNITS = TILE_BYTES / 16, BOX_UNITS = BOX_BYTES / 16;
+constexpr uint32_t K_STEP = 2, MN_STEP = 128, BOX_UNITS = BOX_BYTES / 16;
 
 // True on one lane of a converged warp, always the same one. The compiler knows that a single
 // lane runs what follows and keeps the operands of the tensor instructions in uniform registers.
@@ -190,10 +181,26 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 // A wait of the whole warp, with one outcome for all lanes (.sync.aligned code follows). The
 // loop of a wait that is not over at once stays out of line: the issuing warp shares its
 // scheduler with the computing ones, so that each instruction between two issues counts.
-__device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+__device__ __forceinline__ bool bar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, volatile int* abort_flag) {
   const uint64_t start = globaltimer_ns();
   for (uint32_t spins = 1;; ++spins) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, bar_try_wait(bar, parity))) return true;
     if ((spins & 255u) == 0) {
       const bool late = globaltimer_ns() - start > kWaitLimitNs;
       if (__any_sync(0xffffffffu, late || *abort_flag)) {
@@ -205,9 +212,20 @@ __device__ __noinline__ bool warp_wait_slow(uint64_t* bar, uint32_t parity, int*
   }
 }
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+// By shared-memory address: barriers at fixed distances then take one register for all.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, bar_try_wait(bar, parity))) return true;
   return warp_wait_slow(bar, parity, err, abort_flag);
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  return warp_wait(smem_u32(bar), parity, err, abort_flag);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // Pairs of fp32: one instruction for two columns.
@@ -297,7 +315,7 @@ __device__ __forceinline__ int step_row(int j, int cs, int k0) {
   return ROWS * (KEYS ? k0 + j : (j < cs ? j : k0 + j - cs));
 }
 
-// A block's items one after another (every gridDim.x-th). Only the loading warp walks them; it
+// The items of a block (of one of its chains in the forward) one after another, a fixed distance apart. Only the loading warp walks them; it
 // hands the others a record an item in shared memory, so that they carry neither the walk nor
 // its registers (kept beside 64 scores a thread they spilled, and the spills set the pace).
 // kstart of the next item is loaded an item ahead, and the digits are carried along.
@@ -307,9 +325,9 @@ struct Walk {
   int i;                // index within the pair (head, sample)
   int nh, nb, ni, nks;  // next item
 
-  __device__ __forceinline__ explicit Walk(const Params& p) {
-    nh = blockIdx.x % p.heads;
-    const int rest = blockIdx.x / p.heads;
+  __device__ __forceinline__ Walk(const Params& p, int first) {
+    nh = first % p.heads;
+    const int rest = first / p.heads;
     nb = rest % p.B;
     ni = rest / p.B;
     nks = ni < p.tiles ? __ldg(p.kstart + nb) : 0;
@@ -363,47 +381,50 @@ template <int HD>
 __global__ void __launch_bounds__(F_THREADS, 2)
     window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv,
                       const Params p) {
+  // 64-wide heads: P takes the place of half of S (64 | O 64 columns), and the next scores wait for
+  // the products; 32-wide ones have room beside it (S 64 | P 32 | O 32).
+  constexpr bool OVER = HD == 64;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* sQ = align1024(smem_raw);  // [2]
-  uint8_t* sK = sQ + 2 * TILE_BYTES;  // [2]
-  uint8_t* sV = sK + 2 * TILE_BYTES;  // [2]
-  float* sMax = reinterpret_cast<float*>(sV + 2 * TILE_BYTES);  // [2 steps][2 halves][128]
-  float* sSum = sMax + 4 * TILE;                                // [2 items][2 halves][128]
-  float* sRef = sSum + 4 * TILE;                                // [2 items][128]
-  Item* recs = reinterpret_cast<Item*>(sRef + 2 * TILE);        // [RECS]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(recs + RECS);
-  uint64_t* q_full = bars;        // [2]
-  uint64_t* q_empty = bars + 2;   // [2]
-  uint64_t* kv_full = bars + 4;   // [2]
-  uint64_t* kv_empty = bars + 6;  // [2]
-  uint64_t* s_full = bars + 12;
-  uint64_t* s_empty = bars + 13;
-  uint64_t* p_full = bars + 14;
-  uint64_t* pv_done = bars + 15;
-  uint64_t* done = bars + 16;
-  uint64_t* rec_full = bars + 17;   // [RECS]
-  uint64_t* rec_empty = bars + 21;  // [RECS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(RECS * sizeof(Item) + 26 * 8 <= TAIL, "records and barriers");
-
+  uint8_t* smem = align1024(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1);
+  const int chain = warp < 4 ? warp >> 1 : (warp - 4) >> 2;
+  uint8_t* sQ = smem + chain * F_CHAIN;
+  uint8_t* sK = sQ + TILE_BYTES;              // [F_STAGES]
+  uint8_t* sV = sK + F_STAGES * BOX_BYTES;    // [F_STAGES]
+  Item* recs = reinterpret_cast<Item*>(smem + CHAINS * F_CHAIN) + chain * RECS;
+  uint64_t* all_bars = reinterpret_cast<uint64_t*>(reinterpret_cast<Item*>(smem + CHAINS * F_CHAIN) + CHAINS * RECS);
+  uint64_t* bars = all_bars + chain * F_BARS;
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* s_full = bars + 2;
+  uint64_t* s_empty = bars + 3;
+  uint64_t* p_full = bars + 4;
+  uint64_t* pv_done = bars + 5;
+  uint64_t* done = bars + 6;
+  uint64_t* kv_full = bars + 7;                // [F_STAGES]
+  uint64_t* kv_empty = kv_full + F_STAGES;     // [F_STAGES]
+  uint64_t* rec_full = kv_empty + F_STAGES;    // [RECS]
+  uint64_t* rec_empty = rec_full + RECS;       // [RECS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_bars + CHAINS * F_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(CHAINS * (RECS * sizeof(Item) + F_BARS * 8) + 8 <= F_TAIL, "records and barriers");
+
+  if (threadIdx.x < 4 * 32 && (threadIdx.x & 63) == 0) {  // the first thread of each chain
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 4);
+    mbar_init(p_full, 4);
+    mbar_init(pv_done, 1);
+    mbar_init(done, 1);
+    for (int s = 0; s < F_STAGES; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
     }
     for (int s = 0; s < RECS; ++s) {
       mbar_init(&rec_full[s], 1);
-      mbar_init(&rec_empty[s], 9);  // the issuing warp and the softmax warps
+      mbar_init(&rec_empty[s], 5);  // the issuing warp and the softmax warps
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_empty, 8);
-    mbar_init(p_full, 8);
-    mbar_init(pv_done, 1);
-    mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -414,177 +435,189 @@ __global__ void __launch_bounds__(F_THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t tS = tmem, tP = tmem + 128, tO = tmem + 192;
+  const uint32_t tS = *tmem_slot + chain * 128;
+  const uint32_t tP = OVER ? tS + 32 : tS + 64, tO = OVER ? tS + 64 : tS + 96;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ walk and load
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_q);
-      tma_prefetch_desc(&tm_kv);
-    }
-    const int q0 = p.Lk - p.Lq;
-    int items = 0, g = 0;
-    bool ok = true;
-    Walk<false, TILE> w(p);
-    while (ok && w.next(p)) {
-      const Item& it = w.it;
-      // queries before the first valid token (a share of them per item)
-      const int pad = min(p.Lq, it.kst - q0);
-      for (int q = w.i * 32 + lane; q < pad; q += p.tiles * 32) {
-        const long long row = static_cast<long long>(it.b) * p.Lq + q;
-        zero_row(p.out + (row * p.H + it.h) * HD, HD);
-        if (p.out_lo != nullptr) zero_row(p.out_lo + (row * p.H + it.h) * HD, HD);
-        p.lse[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + q] = CUDART_INF_F;
-      }
-      if (it.n == 0) continue;
-      const int slot = items % RECS, sq = items & 1;
-      // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
-      if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) break;
-      w.it.row0 = it.kst + TILE * it.t - q0;
-      w.it.lse = (static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.row0;
-      w.it.out = ((static_cast<long long>(it.b) * p.Lq + it.row0) * p.H + it.h) * HD;
+  if (warp < 4) {
+    if ((warp & 1) == 0) {
+      // ---------------------------------------------------------- walk and load
       if (lane == 0) {
-        recs[slot] = it;
-        mbar_arrive(&rec_full[slot]);
+        tma_prefetch_desc(&tm_q);
+        tma_prefetch_desc(&tm_kv);
       }
-      __syncwarp();
-      const int kvh = it.h / (p.H / p.G);
-      if (!warp_wait(&q_empty[sq], ((items >> 1) + 1) & 1, p.err, abort_flag)) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&q_full[sq], TILE_BYTES);
-        load_tile(sQ + sq * TILE_BYTES, &tm_q, &q_full[sq], it.h * HD, it.kst + TILE * it.t - q0, it.b);
-      }
-      __syncwarp();
-      ++items;
-      for (int j = 0; j < it.n; ++j, ++g) {
-        const int st = g & 1, y = it.kst + step_row<false, TILE>(j, it.cs, it.k0);
-        if (!warp_wait(&kv_empty[st], ((g >> 1) + 1) & 1, p.err, abort_flag)) {
+      const int q0 = p.Lk - p.Lq;
+      int items = 0, g = 0;
+      bool ok = true;
+      Walk<false, BOX> w(p, chain * gridDim.x + blockIdx.x);
+      while (ok && w.next(p)) {
+        const Item& it = w.it;
+        // queries before the first valid token (a share of them per item)
+        const int pad = min(p.Lq, it.kst - q0);
+        for (int q = w.i * 32 + lane; q < pad; q += p.tiles * 32) {
+          const long long row = static_cast<long long>(it.b) * p.Lq + q;
+          zero_row(p.out + (row * p.H + it.h) * HD, HD);
+          if (p.out_lo != nullptr) zero_row(p.out_lo + (row * p.H + it.h) * HD, HD);
+          p.lse[(static_cast<long long>(it.b) * p.H + it.h) * p.Lq + q] = CUDART_INF_F;
+        }
+        if (it.n == 0) continue;
+        const int slot = items % RECS;
+        // parity of the previous use of a stage; a fresh barrier passes parity 1 at once
+        if (!warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        w.it.row0 = it.kst + TILE * it.t - q0;
+        w.it.lse = (static_cast<long long>(it.b) * p.H + it.h) * p.Lq + it.row0;
+        w.it.out = ((static_cast<long long>(it.b) * p.Lq + it.row0) * p.H + it.h) * HD;
+        if (lane == 0) {
+          recs[slot] = it;
+          mbar_arrive(&rec_full[slot]);
+        }
+        __syncwarp();
+        const int kvh = it.h / (p.H / p.G);
+        if (!warp_wait(q_empty, (items + 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
         if (lane == 0) {
-          mbar_arrive_expect_tx(&kv_full[st], 2 * TILE_BYTES);
-          load_tile(sK + st * TILE_BYTES, &tm_kv, &kv_full[st], (p.H + kvh) * HD, y, it.b);
-          load_tile(sV + st * TILE_BYTES, &tm_kv, &kv_full[st], (p.H + p.G + kvh) * HD, y, it.b);
+          mbar_arrive_expect_tx(q_full, TILE_BYTES);
+          load_tile(sQ, &tm_q, q_full, it.h * HD, it.row0, it.b);
         }
         __syncwarp();
+        ++items;
+        for (int j = 0; j < it.n; ++j, ++g) {
+          const int st = g % F_STAGES, y = it.kst + step_row<false, BOX>(j, it.cs, it.k0);
+          if (!warp_wait(&kv_empty[st], (g / F_STAGES + 1) & 1, p.err, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&kv_full[st], 2 * BOX_BYTES);
+            tma_load_3d(sK + st * BOX_BYTES, &tm_kv, &kv_full[st], (p.H + kvh) * HD, y, it.b);
+            tma_load_3d(sV + st * BOX_BYTES, &tm_kv, &kv_full[st], (p.H + p.G + kvh) * HD, y, it.b);
+          }
+          __syncwarp();
+        }
       }
-    }
-    const int slot = items % RECS;
-    if (ok && warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag) && lane == 0) {
-      recs[slot].n = -1;
-      mbar_arrive(&rec_full[slot]);
-    }
-    __syncwarp();
-    // every copy into this CTA's smem has landed before the CTA may exit
-    if (lane == 0) {
-      for (int j = max(0, items - 2); j < items; ++j) mbar_wait(&q_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
-      for (int j = max(0, g - 2); j < g; ++j) mbar_wait(&kv_full[j & 1], (j >> 1) & 1, nullptr, nullptr);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ issue
-    // The whole warp waits (uniform registers hold its counters and descriptors); lane 0
-    // issues. Scores run one step ahead of the products, across items.
-    constexpr uint32_t idesc_s = make_idesc_bf16(TILE, TILE, false, false);
-    constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, HD, false, true);
-    const uint64_t dQ = desc_of(sQ), dK = desc_of(sK), dV = desc_mn_of(sV);
-    int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the block
-    bool ok = true;
-    // steps of item `i`, -1 after the last
-    auto steps_of = [&](int i) -> int {
-      if (!warp_wait(&rec_full[i % RECS], (i / RECS) & 1, p.err, abort_flag)) {
-        ok = false;
-        return -1;
-      }
-      return __reduce_max_sync(0xffffffffu, recs[i % RECS].n);
-    };
-    auto issue_s = [&]() -> bool {
-      const int st = a_g & 1, sq = a_items & 1;
-      if ((a_j == 0 && !warp_wait(&q_full[sq], (a_items >> 1) & 1, p.err, abort_flag)) ||
-          !warp_wait(&kv_full[st], (a_g >> 1) & 1, p.err, abort_flag) ||
-          (a_g > 0 && !warp_wait(s_empty, (a_g - 1) & 1, p.err, abort_flag)))
-        return false;
-      tc_fence_after();
-      const uint64_t a = dQ + sq * TILE_UNITS, b = dK + st * TILE_UNITS;
-      const bool last = a_j + 1 == a_n;
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS, a + ks * K_STEP, b + ks * K_STEP, idesc_s, ks);
-        tc_commit(s_full);
-        if (last) tc_commit(&q_empty[sq]);
+      const int slot = items % RECS;
+      if (ok && warp_wait(&rec_empty[slot], (items / RECS + 1) & 1, p.err, abort_flag) && lane == 0) {
+        recs[slot].n = -1;
+        mbar_arrive(&rec_full[slot]);
       }
       __syncwarp();
-      ++a_g;
-      ++a_j;
-      if (last) {
-        a_j = 0;
-        a_n = steps_of(++a_items);
+      // every copy into this CTA's smem has landed before the CTA may exit
+      if (lane == 0) {
+        if (items > 0) mbar_wait(q_full, (items - 1) & 1, nullptr, nullptr);
+        for (int j = max(0, g - F_STAGES); j < g; ++j)
+          mbar_wait(&kv_full[j % F_STAGES], (j / F_STAGES) & 1, nullptr, nullptr);
       }
-      return ok;
-    };
-    a_n = steps_of(0);
-    int n = a_n, g = 0;
-    if (ok && a_n > 0) ok = issue_s();
-    for (int items = 0; ok && n > 0; ++items) {
-      for (int j = 0; j < n; ++j, ++g) {
-        const int st = g & 1;
-        if ((a_n > 0 && !issue_s()) || !warp_wait(p_full, g & 1, p.err, abort_flag)) {
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- issue
+      // The whole warp waits (uniform registers hold its counters and descriptors); one lane
+      // issues. Scores run one step ahead of the products, across items.
+      constexpr uint32_t idesc_s = make_idesc_bf16(TILE, BOX, false, false);
+      constexpr uint32_t idesc_pv = make_idesc_bf16(TILE, HD, false, true);
+      const uint64_t dQ = desc_of(sQ), dK = desc_of(sK), dV = desc_mn_of(sV);
+      int a_items = 0, a_j = 0, a_n = 0, a_g = 0;  // ahead: item, step, its steps, step of the chain
+      bool ok = true;
+      // steps of item `i`, -1 after the last
+      auto steps_of = [&](int i) -> int {
+        if (!warp_wait(&rec_full[i % RECS], (i / RECS) & 1, p.err, abort_flag)) {
           ok = false;
-          break;
+          return -1;
         }
+        return __reduce_max_sync(0xffffffffu, recs[i % RECS].n);
+      };
+      auto issue_s = [&]() -> bool {
+        const int st = a_g % F_STAGES;
+        if ((a_j == 0 && !warp_wait(q_full, a_items & 1, p.err, abort_flag)) ||
+            !warp_wait(&kv_full[st], (a_g / F_STAGES) & 1, p.err, abort_flag) ||
+            (!OVER && a_g > 0 && !warp_wait(s_empty, (a_g - 1) & 1, p.err, abort_flag)))
+          return false;
         tc_fence_after();
-        const uint64_t b = dV + st * TILE_UNITS;
-        const uint32_t acc = j > 0 ? 1u : 0u;
+        const uint64_t b = dK + st * BOX_UNITS;
+        const bool last = a_j + 1 == a_n;
         if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
-            tc_mma_bf16_ts(tO, tP + ks * 8, b + ks * MN_STEP, idesc_pv, ks > 0 ? 1u : acc);
-          tc_commit(pv_done);
-          tc_commit(&kv_empty[st]);
+          for (int ks = 0; ks < HD / 16; ++ks) tc_mma_bf16(tS, dQ + ks * K_STEP, b + ks * K_STEP, idesc_s, ks);
+          tc_commit(s_full);
+          if (last) tc_commit(q_empty);
         }
         __syncwarp();
+        ++a_g;
+        ++a_j;
+        if (last) {
+          a_j = 0;
+          a_n = steps_of(++a_items);
+        }
+        return ok;
+      };
+      a_n = steps_of(0);
+      int n = a_n, g = 0;
+      if (ok && a_n > 0) ok = issue_s();
+      for (int items = 0; ok && n > 0; ++items) {
+        for (int j = 0; j < n; ++j, ++g) {
+          const int st = g % F_STAGES;
+          if ((!OVER && a_n > 0 && !issue_s()) || !warp_wait(p_full, g & 1, p.err, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t b = dV + st * BOX_UNITS;
+          const uint32_t acc = j > 0 ? 1u : 0u;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < BOX / 16; ++ks)
+              tc_mma_bf16_ts(tO, tP + ks * 8, b + ks * MN_STEP, idesc_pv, ks > 0 ? 1u : acc);
+            tc_commit(pv_done);
+            tc_commit(&kv_empty[st]);
+          }
+          __syncwarp();
+          if (OVER && a_n > 0 && !issue_s()) {  // behind the products: the tensor pipe keeps their order
+            ok = false;
+            break;
+          }
+        }
+        if (!ok) break;
+        n = steps_of(items + 1);
+        if (elect_one()) mbar_arrive(&rec_empty[items % RECS]);
+        __syncwarp();
       }
-      if (!ok) break;
-      n = steps_of(items + 1);
-      if (elect_one()) mbar_arrive(&rec_empty[items % RECS]);
+      // all MMAs have finished before TMEM is released
+      if (elect_one()) {
+        tc_commit(done);
+        mbar_wait(done, 0, nullptr, nullptr);
+      }
       __syncwarp();
     }
-    // all MMAs have finished before TMEM is released
-    if (elect_one()) {
-      tc_commit(done);
-      mbar_wait(done, 0, nullptr, nullptr);
-    }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
-    // Two warps share 32 query rows, a half of the columns (of S and of O) each.
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    // Thread = query row.
+    const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    constexpr int OC = HD / 2;
-    const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int row_stride = p.H * HD;
-    const uint32_t tS_own = base + half * 64, tP_own = base + 128 + half * 32, tO_own = base + 192 + half * OC;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t bar = smem_u32(bars);
+    constexpr uint32_t S_FULL = 16, S_EMPTY = 24, P_FULL = 32, PV_DONE = 40, REC_FULL = 56 + 16 * F_STAGES,
+                       REC_EMPTY = REC_FULL + 8 * RECS;
     bool ok = true;
     int g = 0, items = 0;
-    // The output of item `items - 1`: written while the next item's first scores are
-    // exponentiated, when its last product has long finished.
-    auto write_out = [&]() {
-      const int k = items - 1, slot = k % RECS;
+    float m = 0.f, l = 0.f;  // reference and sum of the row
+    // The output of item `items - 1`, while the next item's first scores are computed.
+    auto write_out = [&](float ref, float sum) {
+      const int slot = (items - 1) % RECS;
       const Item& it = recs[slot];
-      const float l = sSum[((k & 1) * 2) * TILE + r] + sSum[((k & 1) * 2 + 1) * TILE + r];
       const bool real = static_cast<unsigned>(it.row0 + r) < static_cast<unsigned>(p.Lq);
-      const long long o = it.out + r * row_stride;
+      const long long o = it.out + static_cast<long long>(r) * (p.H * HD);
       const long long ls = it.lse + r;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&rec_empty[slot]);
-      if (real && half == 0) p.lse[ls] = sRef[(k & 1) * TILE + r] + lg2(l);
-      const float inv = __fdividef(1.f, l);
+      if (lane == 0) bar_arrive(bar + REC_EMPTY + 8 * slot);
+      if (real) p.lse[ls] = ref + lg2(sum);
+      const float inv = __fdividef(1.f, sum);
 #pragma unroll
-      for (int c = 0; c < OC / 16; ++c) {
+      for (int c = 0; c < HD / 16; ++c) {
         uint32_t ov[16];
-        tmem_ld16(tO_own + c * 16, ov);
+        tmem_ld16(tO + lanes + c * 16, ov);
         tmem_wait_ld();
         if (!real) continue;
         uint32_t hi[8];
@@ -596,112 +629,117 @@ __global__ void __launch_bounds__(F_THREADS, 2)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          reinterpret_cast<uint4*>(p.out + o + half * OC + c * 16)[e] =
+          reinterpret_cast<uint4*>(p.out + o + c * 16)[e] =
               make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
           if (p.out_lo != nullptr)
-            reinterpret_cast<uint4*>(p.out_lo + o + half * OC + c * 16)[e] =
+            reinterpret_cast<uint4*>(p.out_lo + o + c * 16)[e] =
                 make_uint4(ov[4 * e], ov[4 * e + 1], ov[4 * e + 2], ov[4 * e + 3]);
         }
       }
     };
     for (;; ++items) {
       const int slot = items % RECS;
-      if (!warp_wait(&rec_full[slot], (items / RECS) & 1, p.err, abort_flag)) {
+      if (!warp_wait(bar + REC_FULL + 8 * slot, (items / RECS) & 1, p.err, abort_flag)) {
         ok = false;
         break;
       }
       const int4 first = *reinterpret_cast<const int4*>(&recs[slot]);
       const int n = first.x, t = first.y, cs = first.z, k0 = first.w;
       if (n < 0) break;
-      float m = -CUDART_INF_F, l = 0.f;
-      for (int j = 0; j < n; ++j, ++g) {
-        if (!warp_wait(s_full, g & 1, p.err, abort_flag)) {
+      if (items > 0) {
+        if (!warp_wait(bar + PV_DONE, (g - 1) & 1, p.err, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t sr[64];
-        tmem_ld32(tS_own, sr);
-        tmem_ld32(tS_own + 32, sr + 32);
-        // Visible columns as two 32-column words: the diagonal, and what the window's lower edge
-        // cuts of tiles that are not all sinks. A word that is empty for the whole warp is not
-        // exponentiated; a full one needs no mask.
-        uint32_t vm[2] = {~0u, ~0u};
-        bool live[2] = {true, true}, part[2] = {false, false};
-        const int key0 = step_row<false, TILE>(j, cs, k0);
-        if (key0 == TILE * t || (TILE * t - key0 + TILE > p.window && key0 + TILE > p.sinks)) {
-          const int d = TILE * t + r - key0 - 64 * half;  // columns up to d are not in the future
-          const int lo = d - p.window + 1, sk = min(d, p.sinks - 1 - key0 - 64 * half);
+        write_out(m, l);
+      }
+      for (int j = 0; j < n; ++j, ++g) {
+        // Which of the step's two runs of 32 keys do these 32 queries see? None, all, or some.
+        const int row = TILE * t + 32 * quarter;  // the first query
+        const int key = step_row<false, BOX>(j, cs, k0);
+        bool live[2], part[2];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            vm[c] = range_bits(lo, d, c) | range_bits(0, sk, c);
-            live[c] = __any_sync(0xffffffffu, vm[c] != 0u);
-            part[c] = __any_sync(0xffffffffu, vm[c] != ~0u);
-          }
+        for (int c = 0; c < 2; ++c) {
+          const int lo = key + 32 * c, hi = lo + 31;
+          live[c] = lo <= row + 31 && (hi > row - p.window || lo < p.sinks);
+          part[c] = hi > row || (lo <= row + 31 - p.window && hi >= p.sinks);
         }
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty);
+        if (!warp_wait(bar + S_FULL, g & 1, p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        // The scores pass through registers 32 at a time, the first 32 twice (for the maximum and for
+        // the exponentials): all 64 would spill.
+        uint32_t sr[32];
+        auto load = [&](int c) {
+          tmem_ld32(tS + lanes + 32 * c, sr);
+          tmem_wait_ld();
+          if (part[c]) {
+            const int d = row + lane - key;  // keys up to d are not in the future
+            const uint32_t vm = range_bits(d - p.window + 1, d, c) | range_bits(0, min(d, p.sinks - 1 - key), c);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((vm >> k) & 1u)) sr[k] = __float_as_uint(-CUDART_INF_F);
+          }
+        };
         float mx = -CUDART_INF_F;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (!live[c]) continue;
-          if (part[c]) {
+          load(c);
+          float m2[2] = {__uint_as_float(sr[0]), __uint_as_float(sr[1])};
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!((vm[c] >> k) & 1u)) sr[32 * c + k] = __float_as_uint(-CUDART_INF_F);
+          for (int k = 2; k < 30; k += 4) {
+            m2[0] = max3(m2[0], __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+            m2[1] = max3(m2[1], __uint_as_float(sr[k + 2]), __uint_as_float(sr[k + 3]));
           }
-          float m4[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) m4[k] = __uint_as_float(sr[32 * c + k]);
-#pragma unroll
-          for (int k = 4; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(sr[32 * c + k]));
-          mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+          m2[0] = max3(m2[0], __uint_as_float(sr[30]), __uint_as_float(sr[31]));
+          mx = max3(mx, m2[0], m2[1]);
         }
         mx *= p.scale2;
-        float* row_max = sMax + (g & 1) * 2 * TILE;
-        row_max[half * TILE + r] = mx;
-        pair_sync(1 + quarter);
-        mx = fmaxf(mx, row_max[(half ^ 1) * TILE + r]);
+        if (g > 0 && !warp_wait(bar + PV_DONE, (g - 1) & 1, p.err, abort_flag)) {  // the last P was consumed
+          ok = false;
+          break;
+        }
+        tc_fence_after();
         if (j == 0) {
           m = mx;
+          l = 0.f;
         } else if (__any_sync(0xffffffffu, mx > m + 8.f)) {
           const float m_new = fmaxf(m, mx);
           const float alpha = m_new == -CUDART_INF_F ? 1.f : ex2(m - m_new);
           m = m_new;
           l *= alpha;
-          if (!warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < OC / 8; ++c) {  // few registers at a time: the scores are held
+          for (int c = 0; c < HD / 8; ++c) {  // few registers at a time: the scores are held
             uint32_t ov[8];
-            tmem_ld8(tO_own + c * 8, ov);
+            tmem_ld8(tO + lanes + c * 8, ov);
             tmem_wait_ld();
 #pragma unroll
             for (int d = 0; d < 8; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * alpha);
-            tmem_st8(tO_own + c * 8, ov);
+            tmem_st8(tO + lanes + c * 8, ov);
           }
         }
-        if (g > 0 && !warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {  // the last P was consumed
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (j == 0 && items > 0) write_out();
         const float m_use = m == -CUDART_INF_F ? 0.f : m;
         const F2 sc = {-p.scale2, -p.scale2}, mm = {m_use, m_use};
         F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 1; c >= 0; --c) {
           uint32_t pk[16];
+          if (c == 0) {
+            if (live[0] && live[1]) load(0);
+            if (!OVER) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive(bar + S_EMPTY);
+            }
+          }
           if (live[c]) {
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const F2 x = fma2(pair_of(sr + 32 * c + k), sc, mm);  // m - score; the sign is free in ex2
+              const F2 x = fma2(pair_of(sr + k), sc, mm);  // m - score; the sign is free in ex2
               const F2 e = {ex2(-x.x), ex2(-x.y)};
               sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
               pk[k / 2] = pack2(e.x, e.y);
@@ -710,31 +748,26 @@ __global__ void __launch_bounds__(F_THREADS, 2)
 #pragma unroll
             for (int k = 0; k < 16; ++k) pk[k] = 0u;
           }
-          tmem_st16(tP_own + 16 * c, pk);
+          tmem_st16(tP + lanes + 16 * c, pk);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) bar_arrive(bar + P_FULL);
       }
       if (!ok) break;
-      // Read by the other half after the pair's next barrier, which it passes only once it has
-      // read the item's before: two buffers do.
-      sSum[((items & 1) * 2 + half) * TILE + r] = l;
-      if (half == 0) sRef[(items & 1) * TILE + r] = m;
     }
-    if (ok && items > 0 && warp_wait(pv_done, (g - 1) & 1, p.err, abort_flag)) {
-      pair_sync(1 + quarter);
+    if (ok && items > 0 && warp_wait(bar + PV_DONE, (g - 1) & 1, p.err, abort_flag)) {
       tc_fence_after();
-      write_out();
+      write_out(m, l);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, F_TMEM);
+    tmem_dealloc(*tmem_slot, F_TMEM);
   }
 }
 
@@ -819,7 +852,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       tma_prefetch_desc(&tm_do);
     }
     bool ok = true;
-    Walk<KEYS, BOX> w(p);
+    Walk<KEYS, BOX> w(p, blockIdx.x);
     int items = 0, g = 0;
     const int width = (p.H + 2 * p.G) * HD;
     while (ok && w.next(p)) {
@@ -1264,7 +1297,7 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t W, uint64_t L, uin
 }
 
 // `heads` x B x `tiles` items over a grid of `grid` blocks.
-Params make_params(const WindowAttnArgs& a, int heads, int tiles, int grid) {
+Params make_params(const WindowAttnArgs& a, int heads, int tiles, int stride) {
   Params p;
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.out_lo = static_cast<__nv_bfloat16*>(a.out_lo);
@@ -1287,9 +1320,9 @@ Params make_params(const WindowAttnArgs& a, int heads, int tiles, int grid) {
   p.partial = a.partial;
   p.heads = heads;
   p.tiles = tiles;
-  p.dh = grid % heads;
-  p.db = grid / heads % a.B;
-  p.di = grid / heads / a.B;
+  p.dh = stride % heads;
+  p.db = stride / heads % a.B;
+  p.di = stride / heads / a.B;
   p.scale = a.scale;
   p.scale2 = a.scale * kLog2e;
   p.err = a.err;
@@ -1364,8 +1397,8 @@ cudaError_t fwd_hd(const WindowAttnArgs& a, cudaStream_t stream) {
   static std::atomic<bool> ready[kMaxDevices];
   const int dev = device_index();
   const int tiles = (a.Lq + TILE - 1) / TILE + 1;
-  const int grid = grid_of(a.H, a.B, tiles, 2LL * num_sms(dev));
-  const Params p = make_params(a, a.H, tiles, grid);
+  const int grid = grid_of(a.H, a.B, tiles, 2LL * num_sms(dev));  // the second chains start where the first ones end
+  const Params p = make_params(a, a.H, tiles, CHAINS * grid);
   const uint64_t W = static_cast<uint64_t>(a.H + 2 * a.G) * HD;
   const auto* base = static_cast<const __nv_bfloat16*>(a.qkv);
   CUtensorMap tq, tkv;

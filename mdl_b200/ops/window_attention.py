@@ -77,7 +77,7 @@ def window_attention_bwd(qkv, ks, out, out_lo, lse, dout, heads: int, kv_heads: 
 
 def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: int, window: int, sinks: int = 0,
                        kv_heads: int | None = None, scale: float | None = None) -> torch.Tensor:
-    """See the module's text; ``scale`` defaults to ``head_dim ** -0.5``."""
+    """See the module's text; ``scale`` (positive) defaults to ``head_dim ** -0.5``."""
 
     with trace_range("mdl.attention.windowed"):
         G = heads if kv_heads is None else kv_heads
@@ -90,6 +90,8 @@ def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: 
             raise ValueError(f"windowed attention: {lq} queries of {Lk} tokens")
         if window < 1 or sinks < 0:
             raise ValueError(f"windowed attention: window {window} must be positive, sinks {sinks} not negative")
+        if scale is not None and not 0.0 < scale < math.inf:
+            raise ValueError(f"windowed attention: scale {scale} must be positive")
         if kstart.shape != (B,) or kstart.is_floating_point() or kstart.dtype == torch.bool:
             raise ValueError(f"windowed attention: kstart {tuple(kstart.shape)} {kstart.dtype}, expected whole numbers "
                              f"({B},)")
@@ -113,4 +115,4 @@ def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: 
         if ks.dtype is not torch.int32 or not ks.is_contiguous():
             ks = ks.to(torch.int32).contiguous()
         return ext().windowed_attention(qkv, ks, heads, G, lq, min(window, Lk), min(sinks, Lk),
-                                        float(scale) if scale else 0.0, error_word(qkv.device))
+                                        scale or 0.0, error_word(qkv.device))

@@ -453,3 +453,12 @@ def test_quantize_rows_definition():
     assert s.tolist() == [1.0, 0.0]
     assert c.tolist() == [[7, 0, 0, 2, 2, -7, 0, 3], [0] * 8]
     assert math.isnan(float(quantize_rows(torch.tensor([[1.0, float("inf")]]))[1]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [0.0, -0.25, math.inf, math.nan])
+def test_scale_is_positive(device, scale):
+    cache = QuantizedKVCache(2, 16, 2, 32, device=device)
+    q = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError, match="scale"):
+        cached_attention(q, cache, scale=scale)

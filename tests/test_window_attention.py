@@ -317,3 +317,11 @@ def test_sinks_of_few_long_samples(B, Lk, lq, H, G, hd, window, sinks, kstart):
     (out, otol), (grad, gtol) = _exact(qkv, kstart, dout, H, G, lq, window, sinks)
     _close(o, out, otol)
     _close(dx, grad, gtol)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("scale", [0.0, -0.25, math.inf, math.nan])
+def test_scale_is_positive(device, scale):
+    qkv = torch.zeros(2, 16, 3 * 2 * 32, dtype=torch.bfloat16, device=device)
+    with pytest.raises(ValueError, match="scale"):
+        windowed_attention(qkv, torch.zeros(2, dtype=torch.int32, device=device), 2, 16, 4, scale=scale)
