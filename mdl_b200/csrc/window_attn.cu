@@ -197,7 +197,7 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, volatile int* abort_flag) {
+__device__ __forceinline__ bool warp_wait_held(uint32_t bar, uint32_t parity, int* err, volatile int* abort_flag) {
   const uint64_t start = globaltimer_ns();
   for (uint32_t spins = 1;; ++spins) {
     if (__all_sync(0xffffffffu, bar_try_wait(bar, parity))) return true;
@@ -210,6 +210,10 @@ __device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* 
       }
     }
   }
+}
+
+__device__ __noinline__ bool warp_wait_slow(uint32_t bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  return warp_wait_held(bar, parity, err, abort_flag);
 }
 
 // By shared-memory address: barriers at fixed distances then take one register for all.
@@ -1043,15 +1047,18 @@ __global__ void __launch_bounds__(B_THREADS, 2)
     const uint32_t tS_own = tS + lane_off + 32 * half, tDP_own = tDP + lane_off + 32 * half;
     const uint32_t tP_own = tP + lane_off + PAIR_STEP * half, tDS_own = tDS + lane_off + PAIR_STEP * half;
     const int row_stride = (p.H + 2 * p.G) * HD;
+    const uint32_t bar = smem_u32(bars);
+    constexpr uint32_t A_FULL = 0, A_EMPTY = 8, B_FULL = 16, S_FULL = 80, S_EMPTY = 88, P_FULL = 96, P_EMPTY = 104,
+                       ACC_FULL = 112, ACC_EMPTY = 120, REC_FULL = 136, REC_EMPTY = REC_FULL + 8 * RECS;
     bool ok = true;
     int items = 0, g = 0;
     // keys: dV or dK; queries: half of dQ
     constexpr int COLS = KEYS ? HD : HD / 2;
     const int col0 = KEYS ? 0 : half * COLS;
     const uint32_t tAcc_own = (KEYS && half == 0 ? tAcc0 : tAcc1) + lane_off + col0;
-    // Gradients of item k: written while its successor's first step is under way.
+    // Gradients of item k: written once its successor's first scores are there.
     auto write_grad = [&](int k) -> bool {
-      if (!warp_wait(acc_full, k & 1, p.err, abort_flag)) return false;
+      if (!warp_wait(bar + ACC_FULL, k & 1, p.err, abort_flag)) return false;
       tc_fence_after();
       const Item& it = recs[k % RECS];
       const int own = TILE * it.t + r;
@@ -1062,7 +1069,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
                          ? reinterpret_cast<float4*>(p.partial + ((static_cast<long long>(it.part) * TILE + r) * 2 + half) * HD)
                          : nullptr;
 #pragma unroll
-      for (int e = 0; e < COLS / 8; ++e) {  // few registers at a time: the scores are held
+      for (int e = 0; e < COLS / 8; ++e) {
         uint32_t gr[8], y[4];
         tmem_ld8(tAcc_own + 8 * e, gr);
         tmem_wait_ld();
@@ -1080,14 +1087,14 @@ __global__ void __launch_bounds__(B_THREADS, 2)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(acc_empty);
-        mbar_arrive(&rec_empty[k % RECS]);
+        bar_arrive(bar + ACC_EMPTY);
+        bar_arrive(bar + REC_EMPTY + 8 * (k % RECS));
       }
       return true;
     };
     for (;; ++items) {
       const int slot = items % RECS;
-      if (!warp_wait(&rec_full[slot], (items / RECS) & 1, p.err, abort_flag)) {
+      if (!warp_wait(bar + REC_FULL + 8 * slot, (items / RECS) & 1, p.err, abort_flag)) {
         ok = false;
         break;
       }
@@ -1104,37 +1111,41 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         const long long ls = recs[slot].lse + r;  // (sample, head, query row)
         const long long o = ((static_cast<long long>(recs[slot].b) * p.Lq + recs[slot].row0 + r) * p.H + recs[slot].h) * HD +
                             half * (HD / 2);
-        uint4 hv[V], lv[V];
-#pragma unroll
-        for (int c = 0; c < V; ++c) {
-          hv[c] = lv[c] = make_uint4(0, 0, 0, 0);
-          if (real) {
-            hv[c] = __ldg(reinterpret_cast<const uint4*>(p.out + o) + c);
-            lv[c] = __ldg(reinterpret_cast<const uint4*>(p.out_lo + o) + c);
-          }
-        }
-        if (!warp_wait(a_full, items & 1, p.err, abort_flag)) {
-          ok = false;
-          break;
-        }
-        row_lse = sLse[r];
         const uint8_t* go = sA2 + r * 128;
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-          const uint4 gv = *reinterpret_cast<const uint4*>(go + ((half * V + c) ^ (r & 7)) * 16);
-          const uint32_t e[4] = {gv.x, gv.y, gv.z, gv.w}, a[4] = {hv[c].x, hv[c].y, hv[c].z, hv[c].w},
-                         z[4] = {lv[c].x, lv[c].y, lv[c].z, lv[c].w};
+        for (int v = 0; v < V; v += 2) {
+          uint4 hv[2], lv[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            row_d = fmaf(__uint_as_float(a[i] << 16) + __uint_as_float(z[i] << 16), __uint_as_float(e[i] << 16), row_d);
-            row_d = fmaf(__uint_as_float(a[i] & 0xFFFF0000u) + __uint_as_float(z[i] & 0xFFFF0000u),
-                         __uint_as_float(e[i] & 0xFFFF0000u), row_d);
+          for (int c = 0; c < 2; ++c) {
+            hv[c] = lv[c] = make_uint4(0, 0, 0, 0);
+            if (real) {
+              hv[c] = __ldg(reinterpret_cast<const uint4*>(p.out + o) + v + c);
+              lv[c] = __ldg(reinterpret_cast<const uint4*>(p.out_lo + o) + v + c);
+            }
+          }
+          if (v == 0 && !warp_wait_held(bar + A_FULL, items & 1, p.err, abort_flag)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint4 gv = *reinterpret_cast<const uint4*>(go + ((half * V + v + c) ^ (r & 7)) * 16);
+            const uint32_t e[4] = {gv.x, gv.y, gv.z, gv.w}, a[4] = {hv[c].x, hv[c].y, hv[c].z, hv[c].w},
+                           z[4] = {lv[c].x, lv[c].y, lv[c].z, lv[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              row_d = fmaf(__uint_as_float(a[i] << 16) + __uint_as_float(z[i] << 16), __uint_as_float(e[i] << 16), row_d);
+              row_d = fmaf(__uint_as_float(a[i] & 0xFFFF0000u) + __uint_as_float(z[i] & 0xFFFF0000u),
+                           __uint_as_float(e[i] & 0xFFFF0000u), row_d);
+            }
           }
         }
+        if (!ok) break;
+        row_lse = sLse[r];
         float* part = sHalf + (items & 1) * 2 * TILE;
         part[half * TILE + r] = row_d;
         __syncwarp();
-        if (lane == 0) mbar_arrive(a_empty);
+        if (lane == 0) bar_arrive(bar + A_EMPTY);
         pair_sync(1 + quarter);
         row_d = part[r] + part[TILE + r];
         if (half == 0 && real) p.dsum[ls] = row_d;
@@ -1143,57 +1154,55 @@ __global__ void __launch_bounds__(B_THREADS, 2)
         if (KEYS && s_ == cs) s_ = 0;
         const int st = g % B_STAGES;
         const int c0 = step_row<KEYS, BOX>(s_, cs, k0) + 32 * half;  // this warp's first column
-        if ((KEYS && !warp_wait(&b_full[st], (g / B_STAGES) & 1, p.err, abort_flag)) ||
-            !warp_wait(s_full, g & 1, p.err, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        uint32_t s[32], dp[32];
-        tmem_ld32(tS_own, s);
-        tmem_ld32(tDP_own, dp);
-        // visible columns of this row (see the forward)
-        const int r0 = TILE * t + 32 * quarter;  // this warp's first row
-        uint32_t vm = ~0u;
+        // Which of the 32 x 32 scores of this warp are visible? None, all, or some (see the forward).
+        const int r0 = TILE * t + 32 * quarter;  // its first row
+        bool live, part;
         if constexpr (KEYS) {
-          const bool whole = c0 >= r0 + 31 && c0 >= it.qf && c0 + 32 <= it.len &&
-                             (r0 + 32 <= p.sinks || c0 + 32 - r0 <= p.window);
-          if (!whole) {
+          live = c0 + 31 >= max(r0, it.qf) && c0 < it.len && (r0 < p.sinks || c0 < r0 + 31 + p.window);
+          part = c0 < r0 + 31 || c0 < it.qf || c0 + 32 > it.len || (r0 + 32 > p.sinks && c0 + 32 - r0 > p.window);
+        } else {
+          live = c0 <= min(r0 + 31, it.len - 1) && r0 + 31 >= it.qf && (c0 < p.sinks || c0 + 31 > r0 - p.window);
+          part = c0 + 31 > r0 || r0 < it.qf || r0 + 32 > it.len || (c0 + 32 > p.sinks && r0 + 32 - c0 > p.window);
+        }
+        uint32_t vm = ~0u;
+        if (part) {
+          if constexpr (KEYS) {
             const int hi = own < p.sinks ? it.len - 1 : min(it.len - 1, own + p.window - 1);
             vm = range_bits(max(own, it.qf) - c0, hi - c0, 0);
-          }
-        } else {
-          const bool whole = c0 + 31 <= r0 && r0 >= it.qf && r0 + 32 <= it.len &&
-                             (c0 + 32 <= p.sinks || r0 + 32 - c0 <= p.window);
-          if (!whole) {
+          } else {
             const int d = own >= it.qf && own < it.len ? own - c0 : -1;
             vm = range_bits(d - p.window + 1, d, 0) | range_bits(0, min(d, p.sinks - 1 - c0), 0);
           }
         }
-        const bool live = __any_sync(0xffffffffu, vm != 0u), part = __any_sync(0xffffffffu, vm != ~0u);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty);
-        const float4* lse4 = reinterpret_cast<const float4*>(sLse + st * BOX + 32 * half);
-        const float4* d4 = reinterpret_cast<const float4*>(sD + st * BOX + 32 * half);
-        const F2 sc = {-p.scale2, -p.scale2}, minus = {-1.f, -1.f};
-        if ((j == 0 && items > 0 && !write_grad(items - 1)) ||
-            (g > 0 && !warp_wait(p_empty, (g - 1) & 1, p.err, abort_flag))) {
+        if ((KEYS && !warp_wait(bar + B_FULL + 8 * st, (g / B_STAGES) & 1, p.err, abort_flag)) ||
+            !warp_wait(bar + S_FULL, g & 1, p.err, abort_flag) || (j == 0 && items > 0 && !write_grad(items - 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const float4* lse4 = reinterpret_cast<const float4*>(sLse + st * BOX + 32 * half);
+        const float4* d4 = reinterpret_cast<const float4*>(sD + st * BOX + 32 * half);
+        const F2 sc = {-p.scale2, -p.scale2}, minus = {-1.f, -1.f};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 16 columns at a time, stored as they are done: few registers
-          uint32_t pk[8], dk[8];
+        for (int c = 0; c < 2; ++c) {  // 16 columns at a time: few registers
+          uint32_t s[16], dp[16], pk[8], dk[8];
+          if (live) {
+            tmem_ld16(tS_own + 16 * c, s);
+            tmem_ld16(tDP_own + 16 * c, dp);
+            tmem_wait_ld();
+          }
+          if (c == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar + S_EMPTY);
+          }
           if (live) {
 #pragma unroll
-            for (int k = 16 * c; k < 16 * c + 16; k += 4) {
+            for (int k = 0; k < 16; k += 4) {
               float4 lv = make_float4(row_lse, row_lse, row_lse, row_lse), dv = make_float4(row_d, row_d, row_d, row_d);
               if constexpr (KEYS) {
-                lv = lse4[k / 4];
-                dv = d4[k / 4];
+                lv = lse4[4 * c + k / 4];
+                dv = d4[4 * c + k / 4];
               }
 #pragma unroll
               for (int e = 0; e < 4; e += 2) {
@@ -1201,25 +1210,33 @@ __global__ void __launch_bounds__(B_THREADS, 2)
                 const F2 x = fma2(pair_of(s + i), sc, e == 0 ? F2{lv.x, lv.y} : F2{lv.z, lv.w});  // lse - score
                 F2 pr = {ex2(-x.x), ex2(-x.y)};
                 if (part) {
-                  if (!((vm >> i) & 1u)) pr.x = 0.f;
-                  if (!((vm >> (i + 1)) & 1u)) pr.y = 0.f;
+                  if (!((vm >> (16 * c + i)) & 1u)) pr.x = 0.f;
+                  if (!((vm >> (16 * c + i + 1)) & 1u)) pr.y = 0.f;
                 }
                 const F2 ds = mul2(pr, fma2(e == 0 ? F2{dv.x, dv.y} : F2{dv.z, dv.w}, minus, pair_of(dp + i)));
-                if constexpr (KEYS) pk[(i - 16 * c) / 2] = pack2(pr.x, pr.y);
-                dk[(i - 16 * c) / 2] = pack2(ds.x, ds.y);
+                if constexpr (KEYS) pk[i / 2] = pack2(pr.x, pr.y);
+                dk[i / 2] = pack2(ds.x, ds.y);
               }
             }
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) pk[k] = dk[k] = 0u;
           }
+          if (c == 0) {  // the last step's P and dS were consumed
+            if (g > 0 && !warp_wait_held(bar + P_EMPTY, (g - 1) & 1, p.err, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
           if constexpr (KEYS) tmem_st8(tP_own + 8 * c, pk);
           tmem_st8(tDS_own + 8 * c, dk);
         }
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) bar_arrive(bar + P_FULL);
       }
       if (!ok) break;
     }
