@@ -1017,6 +1017,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
             const uint32_t off = (ks >> 1) * PAIR_STEP + (ks & 1) * 8;
             if constexpr (KEYS) tc_mma_bf16_ts(tAcc0, tP + off, b2 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
             tc_mma_bf16_ts(tAcc1, tDS + off, b1 + ks * MN_STEP, idesc_acc, ks > 0 ? 1u : acc);
+            if constexpr (!KEYS) tc_mma_bf16_ts(tAcc1, tP + off, b1 + ks * MN_STEP, idesc_acc, 1u);
           }
           tc_commit(p_empty);
           tc_commit(&b_empty[st]);
@@ -1214,8 +1215,14 @@ __global__ void __launch_bounds__(B_THREADS, 2)
                   if (!((vm >> (16 * c + i + 1)) & 1u)) pr.y = 0.f;
                 }
                 const F2 ds = mul2(pr, fma2(e == 0 ? F2{dv.x, dv.y} : F2{dv.z, dv.w}, minus, pair_of(dp + i)));
-                if constexpr (KEYS) pk[i / 2] = pack2(pr.x, pr.y);
-                dk[i / 2] = pack2(ds.x, ds.y);
+                const uint32_t hi = pack2(ds.x, ds.y);
+                dk[i / 2] = hi;
+                if constexpr (KEYS) {
+                  pk[i / 2] = pack2(pr.x, pr.y);
+                } else {  // what rounding took off dS
+                  const F2 lo = add2(ds, {-__uint_as_float(hi << 16), -__uint_as_float(hi & 0xFFFF0000u)});
+                  pk[i / 2] = pack2(lo.x, lo.y);
+                }
               }
             }
           } else {
@@ -1229,7 +1236,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
             }
             tc_fence_after();
           }
-          if constexpr (KEYS) tmem_st8(tP_own + 8 * c, pk);
+          tmem_st8(tP_own + 8 * c, pk);
           tmem_st8(tDS_own + 8 * c, dk);
         }
         if (!ok) break;
