@@ -6,15 +6,20 @@
 // that the window's lower edge cuts need a mask. A query tile visits the tiles of the sinks and
 // then those of its window, so the cost grows with the window and not with the history.
 //
-// Forward (320 threads, two persistent CTAs an SM, 256 TMEM columns each: S 128, P 64, O 64).
-// Work item = sample, head, query tile.
-//   warp 0     walks the items; TMA: Q, K and V tiles into two-stage rings
-//   warp 1     issues: S = Q K^T; O += P V with P as the A operand straight from TMEM
-//   warps 2-9  softmax, two warps a set of 32 query rows: P = exp2(S * c - m) as bf16 into
-//              TMEM. m is a reference that moves only when a score passes it by more than 8
-//              (exp2 of the excess stays below 256), so O is rarely rescaled, and is read once.
-// S of the next tile, of the next item too, is issued as soon as the softmax holds the present
-// one in registers.
+// Forward (384 threads, two persistent CTAs an SM, each with two chains that share nothing but the
+// CTA's 256 TMEM columns). Work item = sample, head, query tile; a step = 64 of its keys. A chain:
+//   one warp    walks the items; TMA: Q, and K and V into two-stage rings
+//   one warp    issues: S = Q K^T; O += P V with P as the A operand straight from TMEM
+//   four warps  softmax, a thread a query row: P = exp2(S * c - m) as bf16 into TMEM. m is a
+//               reference that moves only when a score passes it by more than 8 (exp2 of the
+//               excess stays below 256), so O is rarely rescaled, and is read once.
+// S of the next step, of the next item too, is issued as soon as the softmax has read the present
+// one. Bound by latency and issue: a chain's steps follow one another, so four chains an SM fill
+// its schedulers to a half (the exponentials' unit to a half too, the tensor pipe to 4 %, L2 to
+// 41 %). Two chains an SM of 128-key steps, two warps a set of rows, were 736 us where these are
+// 462, largely for the registers that the scores took then. Measured: 1,024 samples of up to 544
+// tokens, 8 heads of 32, window 128 + 4: 462 us; 64 of 2,000, window 256 + 8: 150 us; 2 of 8,191, 4
+// heads of 64, window 1,024 + 16: 43 us, 240 TFLOP/s.
 //
 // Backward, two launches of one kernel (320 threads, two persistent CTAs an SM): a stationary
 // tile of 128 rows meets a stream of 64-row tiles,
@@ -24,7 +29,13 @@
 //                       heads that share the key head follow one another)
 // Recomputing S and dP in the second launch costs two products more than one launch that adds
 // dQ to memory would, and needs no fp32 buffer, no clearing, no atomics: every sum has one
-// owner and one order.
+// owner and one order. Bound like the forward (schedulers 44 to 50 %, L2 33 %). Measured, queries |
+// keys: 661 | 700 us on the first of the shapes above, 52 | 70 us on the last.
+//
+// Rounding to bf16: P and dS are the A operands of products with bf16 tiles, which tcgen05 takes
+// in one type only. Each costs a product's result 0.0017 of its norm, as much as rounding the result
+// itself does. dS of dQ is held as two bf16 terms (16 bits), which the queries' launch has room for.
+// Sums, references, lse and D are fp32, O reaches D as out + out_lo (16 bits).
 //
 // Every wait is bounded (error word + abort flag) and every role drains what it has in flight
 // before the CTA exits.
@@ -43,7 +54,7 @@ namespace mdl {
 namespace {
 
 constexpr int TILE = 128;               // rows of a tile
-constexpr int BOX = 64;                 // rows of a TMA box, and of a step of the backward
+constexpr int BOX = 64;                 // rows of a TMA box, and of a step
 constexpr int TILE_BYTES = TILE * 128;  // 128-byte rows: 64 columns, the head's hd first
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -51,7 +62,7 @@ constexpr int RECS = 4;                 // item records in flight
 constexpr int BOX_BYTES = BOX * 128;
 constexpr int TAIL = 512;               // barriers and item records of the backward
 constexpr int CHAINS = 2, F_THREADS = 384, F_TMEM = 256, F_STAGES = 2;
-constexpr int F_BARS = 9 + 2 * RECS + 2 * F_STAGES;
+constexpr int F_BARS = 7 + 2 * RECS + 2 * F_STAGES;
 // a chain: Q | K[2] | V[2]; then the item records and barriers of both chains
 constexpr int F_CHAIN = TILE_BYTES + 2 * F_STAGES * BOX_BYTES;
 constexpr int F_TAIL = 1024;
@@ -72,7 +83,7 @@ struct Params {
   float* dsum;
   int B, H, G, Lk, Lq, hd, window, sinks;
   int heads, tiles;  // work items = (head, sample, tile index): heads x B x tiles
-  int dh, db, di;    // gridDim.x items further on, in these digits
+  int dh, db, di;    // an item and the next of its block (forward: chain), in these digits
   // key tiles: the first `stiles` (those with sinks) come in `parts` items of `psteps` steps each,
   // whose sums go to `partial` (parts == 1: like any other tile)
   int stiles, parts, psteps;
@@ -1258,7 +1269,7 @@ __global__ void __launch_bounds__(B_THREADS, 2)
 }
 
 // dV and dK of the sinks' tiles from their parts, in the parts' order. JOIN_ROWS rows a block;
-// a thread = four neighbouring elements.
+// a thread = four neighbouring elements. Bound by its launch: 8 tiles of 8 parts, 64-wide heads: 3.6 us.
 constexpr int JOIN_ROWS = 8;
 template <int HD>
 __global__ void __launch_bounds__(128) window_join_kernel(const Params p) {
@@ -1388,9 +1399,12 @@ cudaError_t allow_smem(K kern, int bytes, std::atomic<bool>* done) {
   return e;
 }
 
-// How the sinks' key tiles are cut. Every query sees them, so with few samples and a long history
-// one of them would be the critical path: 2 samples of 8,191 tokens, 4 heads, took 223 us for the
-// launch, 128 steps in one block where the average was 35. Parts of about half the average load.
+// How the sinks' key tiles are cut. Every query sees them, so that with few samples and a long
+// history one of them is the critical path: from three quarters of a block's average load on it
+// comes in parts of about half that load, joined by a second kernel. Backward of 2 samples of 8,191
+// tokens, 8 query heads on 2 key heads of 64, window 128 + 4: 751 us in one piece, 116 in 33; of 8
+// samples, 4 heads, window 1,024 + 16 (0.95 of the load): 563 and 497; of 16 samples of 2,000, 8
+// heads of 32, window 256 + 8 (0.54 of the load): 159, and 169 in two.
 struct Cut {
   int stiles = 0, parts = 1, psteps = 1;
 };
@@ -1406,7 +1420,7 @@ Cut cut_of(const WindowAttnArgs& a) {
   const long long load = total / (2LL * num_sms(device_index())) + 1;
   const long long steps = std::max<long long>(16, load / 2);
   const long long parts = (most + steps - 1) / steps;
-  if (most <= load || parts < 2) return c;
+  if (4 * most <= 3 * load || parts < 2) return c;
   c.parts = static_cast<int>(parts);
   c.psteps = static_cast<int>(steps);
   return c;
