@@ -462,3 +462,33 @@ def test_scale_is_positive(device, scale):
     q = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device=device)
     with pytest.raises(ValueError, match="scale"):
         cached_attention(q, cache, scale=scale)
+
+
+@GPU
+def test_split_calls_that_follow_one_another():
+    """The join of a row's parts starts while they are computed: calls in a row on one stream, and
+    captured ones, give what single calls give."""
+
+    G, hd, T, H = 2, 64, 30000, 8
+    cache = _shuffled(1, T, G, hd, 64, "cuda")
+    k, v = _kv(1, T, G, hd, "cuda", 7)
+    kv_cache_write(cache, k, v)
+    g = torch.Generator().manual_seed(2)
+    qs = [torch.randn(1, 1, H * hd, generator=g).bfloat16().cuda() for _ in range(8)]
+    single = []
+    for q in qs:
+        single.append(cached_attention(q, cache))
+        torch.cuda.synchronize()
+    row = [cached_attention(q, cache) for q in qs]
+    for a, b in zip(single, row):
+        assert torch.equal(a, b)
+    inputs = [torch.zeros_like(qs[0]) for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [cached_attention(q, cache) for q in inputs]
+    for i in range(0, 8, 2):
+        for t, q in zip(inputs, qs[i:i + 2]):
+            t.copy_(q)
+        graph.replay()
+        assert torch.equal(outs[0], single[i]) and torch.equal(outs[1], single[i + 1])
+    _check_errors("cuda")
