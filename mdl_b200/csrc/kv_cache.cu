@@ -62,7 +62,7 @@ __device__ __forceinline__ long long slot_base(const KvCache& c, int pg, int g, 
 // ============================================================================ write
 // A lane holds 16 values of a row, hd / 16 lanes the row: wide loads, a maximum of one or two
 // shuffles, and a store of 8 bytes. Bound by memory: 256 rows of up to 2,000 tokens, 8 heads of 32, K
-// and V: 104 us, 5.5 TB/s read and written (434,000 tokens of histories of unequal length).
+// and V: 102 us, 5.6 TB/s read and written (434,000 tokens of histories of unequal length).
 //
 // c = rint(x / s) without a division: x / s of two bf16 numbers is either a tie (an odd
 // multiple of 1/2) or at least 1/1020 away from one, and |x / s| <= 7.03 (up to 8-bit
@@ -149,11 +149,22 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int c
   const int sub = threadIdx.x % LPU;
   const __nv_bfloat16* kb = a.k + i * a.k_sb + sub * 16;
   const __nv_bfloat16* vb = a.v + i * a.v_sb + sub * 16;
-  for (int base = 0; base < units; base += kThreads / LPU) {  // whole warps stay together: shuffles below
-    const int u = base + threadIdx.x / LPU;
+  // unit u = slow * inner + fast, carried along
+  constexpr int UNITS = kThreads / LPU;
+  const int inner = token_fast ? nt : c.G, ds = UNITS / inner, df = UNITS % inner;
+  int u = threadIdx.x / LPU, slow = u / inner, fast = u % inner;
+  auto next = [&]() {
+    u += UNITS;
+    slow += ds;
+    fast += df;
+    if (fast >= inner) {
+      fast -= inner;
+      ++slow;
+    }
+  };
+  for (int base = 0; base < units; base += UNITS, next()) {  // whole warps stay together: shuffles below
     const bool live = u < units;
-    const int q = token_fast ? u / nt : u / c.G, rem = u - q * (token_fast ? nt : c.G);
-    const int g = token_fast ? q : rem, t = t0 + (token_fast ? rem : q);
+    const int g = token_fast ? slow : fast, t = t0 + (token_fast ? fast : slow);
     const int pos = start + t - first;
     const bool in = live && t >= first;
     uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
@@ -198,12 +209,35 @@ __global__ void kv_length_kernel(KvWriteArgs a) {
   c.lengths[r] = min(start + a.T - first, cap);
 }
 
+// ============================================================================ codes
+// Codes to bf16 pairs: (w >> 4i) & 0x000F000F | 0x4300_4300 is the exact bf16 pair
+// (128 + nibble i, 128 + nibble i + 4) = 136 + c.
+constexpr uint32_t kMagic = 0x43004300u;   // bf16 128, twice
+constexpr uint32_t kOffset = 0x43084308u;  // bf16 136, twice
+
+// (w & 0x000F000F) | magic in one instruction: it takes one immediate, so the magic number has to
+// sit in a register (`magic`, which the compiler does not see through).
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(d) : "r"(w), "r"(magic));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t code_pair_signed(uint32_t w, uint32_t magic) {
+  const uint32_t u = code_pair(w, magic), o = kOffset;
+  const __nv_bfloat162 r =
+      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&o));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // ============================================================================ read
-// Thread = one code word (8 values) of K and of V. Bound by memory, the bf16 that it writes: 384
-// rows of up to 2,048 tokens, 8 heads of 32: 181 us, 5.5 TB/s read and written.
+// Thread = one code word (8 values) of K and of V, units by token, then head: a warp reads a dense
+// run of a page. Bound by memory, the bf16 that it writes: 384 rows of up to 2,048 tokens, 8 heads of
+// 32: 167 us, 6.0 TB/s read and written (182 us where each nibble was converted by itself, 222
+// million conversions on a unit that does 16 a cycle).
 template <int HD, bool F32>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chunk, int chunks) {
-  constexpr int LPU = HD / 8;
+  constexpr int LPU = HD / 8, UNITS = kThreads / LPU;  // units a pass
   const KvCache& c = a.c;
   const int i = blockIdx.x / chunks;
   const int r = row_of(c, a.rows, i);
@@ -212,13 +246,13 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
   const int start = a.start != nullptr ? a.start[i] : 0;
   if (start < 0 && threadIdx.x == 0) record_error(c.err, MDL_ERR_BAD_INDEX);
   const int t0 = (blockIdx.x - i * chunks) * chunk, nt = min(chunk, a.count - t0);
-  const int units = nt * c.G;
-  const int sub = threadIdx.x % LPU;
-  for (int u = threadIdx.x / LPU; u < units; u += kThreads / LPU) {
-    const int g = u / nt, t = t0 + u % nt;
-    const long long pos = static_cast<long long>(start) + t;
-    uint32_t w[2] = {0x88888888u, 0x88888888u};
-    float s[2] = {0.f, 0.f};
+  const int sub = threadIdx.x % LPU, u = threadIdx.x / LPU;
+  const int dg = UNITS / nt, dt = UNITS % nt;
+  uint32_t magic;
+  asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(kMagic));
+  for (int g = u / nt, t = u % nt; g < c.G;) {
+    const long long pos = static_cast<long long>(start) + t0 + t;
+    uint32_t w[2] = {0x88888888u, 0x88888888u}, sc = 0;
     if (pos >= 0 && pos < len) {
       const int pg = page_of(c, r, static_cast<int>(pos));
       if (pg >= 0) {
@@ -226,26 +260,39 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
         const long long b = slot_base(c, pg, g, 0) + slot;
         w[0] = reinterpret_cast<const uint32_t*>(c.codes)[b * LPU + sub];
         w[1] = reinterpret_cast<const uint32_t*>(c.codes)[(b + (1ll << c.page_shift)) * LPU + sub];
-        const uint32_t sc = reinterpret_cast<const uint32_t*>(c.scales)[scale_index(c, pg, g, static_cast<int>(pos))];
-        s[0] = bf16_lo(sc);
-        s[1] = bf16_hi(sc);
+        sc = reinterpret_cast<const uint32_t*>(c.scales)[scale_index(c, pg, g, static_cast<int>(pos))];
       }
     }
-    const long long off = (static_cast<long long>(i) * a.count + t) * (c.G * HD) + g * HD + sub * 8;
+    const long long off = (static_cast<long long>(i) * a.count + t0 + t) * (c.G * HD) + g * HD + sub * 8;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      float x[8];
+      uint32_t p[4];  // values (j, j + 4), exact
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[kv] * static_cast<float>(static_cast<int>((w[kv] >> (4 * e)) & 15u) - 8);
+      for (int j = 0; j < 4; ++j) p[j] = code_pair_signed(w[kv] >> (4 * j), magic);
       void* out = kv ? a.out_v : a.out_k;
       if constexpr (F32) {
+        const float s = kv ? bf16_hi(sc) : bf16_lo(sc);
         float4* d = reinterpret_cast<float4*>(static_cast<float*>(out) + off);
-        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        d[0] = make_float4(s * bf16_lo(p[0]), s * bf16_lo(p[1]), s * bf16_lo(p[2]), s * bf16_lo(p[3]));
+        d[1] = make_float4(s * bf16_hi(p[0]), s * bf16_hi(p[1]), s * bf16_hi(p[2]), s * bf16_hi(p[3]));
       } else {
+        const uint32_t ss = __byte_perm(sc, sc, kv ? 0x3232 : 0x1010);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // s * c, rounded once
+          const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&p[j]),
+                                           *reinterpret_cast<const __nv_bfloat162*>(&ss));
+          p[j] = *reinterpret_cast<const uint32_t*>(&x);
+        }
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + off) =
-            make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
+                       __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
       }
+    }
+    g += dg;
+    t += dt;
+    if (t >= nt) {
+      t -= nt;
+      ++g;
     }
   }
 }
@@ -265,8 +312,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 // of a request do not fill that, and the kernel is bound by the expansion of the codes and
 // by memory, not by the products.
 //
-// Codes to bf16: (w >> 4i) & 0x000F000F | 0x4300_4300 is the exact bf16 pair (128 + nibble i,
-// 128 + nibble i + 4) = 136 + c. K uses it as it is: S = q . (136 + c) - 136 * sum(q), the
+// The codes enter as code_pair gives them, 136 + c. K uses it as it is: S = q . (136 + c) - 136 * sum(q), the
 // second term being the accumulator's initial value. V subtracts 136 (one packed, exact
 // operation), since the same shortcut over a long sum of keys would cancel. The scales enter
 // in fp32: s_k multiplies the scores, s_v the probabilities.
@@ -276,24 +322,6 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 // keys, 8 query heads on 2 key heads of 64: 117 us, 3.2 TB/s of cache; 1,024 samples of 32
 // candidates, 8 heads of 32, window 512 of 2,000 keys: 173 us, 103 TFLOP/s; one token over 501
 // keys: 4.5 us.
-constexpr uint32_t kMagic = 0x43004300u;   // bf16 128, twice
-constexpr uint32_t kOffset = 0x43084308u;  // bf16 136, twice
-
-// (w & 0x000F000F) | magic in one instruction: it takes one immediate, so the magic number has to
-// sit in a register (`magic`, which the compiler does not see through).
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t magic) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(d) : "r"(w), "r"(magic));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t code_pair_signed(uint32_t w, uint32_t magic) {
-  const uint32_t u = code_pair(w, magic), o = kOffset;
-  const __nv_bfloat162 r =
-      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&o));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, float c0, float c1, float c2, float c3) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -1106,16 +1134,24 @@ cudaError_t attend_hd(const KvAttendArgs& a, const Plan& p, cudaStream_t stream,
 
 }  // namespace
 
+// Tokens a block of a write or a read: 64, or 16 where that leaves multiprocessors without one. 3 rows
+// of 777 tokens, 4 heads of 64 (39 blocks of 64): read 8.4 us, with 16 tokens 4.4, written 9.8 and
+// 7.2; 37 rows of 1,237 tokens, 3 heads of 32 (740 blocks): read 8.5, with 16 tokens 10.5, written 14.2
+// and 17.4.
+static int chunk_of(int rows, int tokens) {
+  return static_cast<long long>(rows) * ((tokens + 63) / 64) < num_sms() ? 16 : 64;
+}
+
 cudaError_t kv_write(const KvWriteArgs& a, cudaStream_t stream, int* launches) {
   if (a.n == 0) return cudaSuccess;
-  constexpr int kChunk = 64;
-  const int chunks = std::max(1, (a.T + kChunk - 1) / kChunk);
+  const int chunk = a.T > 64 ? chunk_of(a.n, a.T) : 64;  // one block a row sets the length by itself
+  const int chunks = std::max(1, (a.T + chunk - 1) / chunk);
   if (static_cast<long long>(chunks) * a.n > 0x7fffffffLL) return cudaErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(chunks) * a.n;
   if (a.c.hd == 64)
-    kv_write_kernel<64><<<grid, kThreads, 0, stream>>>(a, kChunk, chunks);
+    kv_write_kernel<64><<<grid, kThreads, 0, stream>>>(a, chunk, chunks);
   else
-    kv_write_kernel<32><<<grid, kThreads, 0, stream>>>(a, kChunk, chunks);
+    kv_write_kernel<32><<<grid, kThreads, 0, stream>>>(a, chunk, chunks);
   *launches += 1;
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || chunks == 1) return e;
@@ -1126,13 +1162,12 @@ cudaError_t kv_write(const KvWriteArgs& a, cudaStream_t stream, int* launches) {
 
 cudaError_t kv_read(const KvReadArgs& a, cudaStream_t stream) {
   if (a.n == 0 || a.count == 0) return cudaSuccess;
-  constexpr int kChunk = 64;
-  const int chunks = (a.count + kChunk - 1) / kChunk;
+  const int chunk = chunk_of(a.n, a.count), chunks = (a.count + chunk - 1) / chunk;
   if (static_cast<long long>(chunks) * a.n > 0x7fffffffLL) return cudaErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(chunks) * a.n;
   auto kern = a.c.hd == 64 ? (a.fp32 ? kv_read_kernel<64, true> : kv_read_kernel<64, false>)
                            : (a.fp32 ? kv_read_kernel<32, true> : kv_read_kernel<32, false>);
-  kern<<<grid, kThreads, 0, stream>>>(a, kChunk, chunks);
+  kern<<<grid, kThreads, 0, stream>>>(a, chunk, chunks);
   return cudaGetLastError();
 }
 
