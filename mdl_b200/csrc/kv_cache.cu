@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 //
 // Bound: the instructions that expand the codes (about 12 a key of 64 values and warp, with the
 // softmax's) and not memory, whose bytes are a quarter of bf16's. 24 single tokens over 131,071
-// keys, 8 query heads on 2 key heads of 64: 117 us, 3.2 TB/s of cache; 1,024 samples of 32
+// keys, 8 query heads on 2 key heads of 64: 121 us, 3.5 TB/s of cache; 1,024 samples of 32
 // candidates, 8 heads of 32, window 512 of 2,000 keys: 166 us, 108 TFLOP/s; one token over 501
 // keys: 4.5 us.
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -382,10 +382,13 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return d;
 }
 
-// Blocks an SM that the registers have to allow: the kernel hides its latencies with warps.
+// Blocks an SM that the registers have to allow: the kernel hides its latencies with warps, up to
+// where it spills. 8 query rows a block: 32-wide heads with one warp an item, 256 rows of 2,000 keys:
+// five blocks 63 us, six (spilling) 67, seven 83; 64-wide ones with eight warps: two blocks 121 us
+// for 24 rows of 131,071 keys and 48 for 256 of 2,000, three (spilling) 127 and 46.
 template <int HD, int NT, int WPI>
 constexpr int min_blocks() {
-  return WPI == 1 ? (NT == 1 ? (HD == 64 ? 5 : 6) : (NT == 2 ? 4 : 3)) : (NT == 1 ? 3 : (NT == 2 ? 2 : 1));
+  return WPI == 1 ? (NT == 1 ? 5 : (NT == 2 ? 4 : 3)) : (NT == 1 ? (HD == 64 ? 2 : 3) : (NT == 2 ? 2 : 1));
 }
 template <int NT>
 constexpr int tiles_a_step() { return NT == 1 ? 4 : 2; }
