@@ -15,8 +15,8 @@
 //               excess stays below 256), so O is rarely rescaled, and is read once.
 // S of the next step, of the next item too, is issued as soon as the softmax has read the present
 // one. Bound by latency and issue: a chain's steps follow one another, so four chains an SM fill
-// its schedulers to a half (the exponentials' unit to a half too, the tensor pipe to 4 %, L2 to
-// 41 %). Two chains an SM of 128-key steps, two warps a set of rows, were 736 us where these are
+// its schedulers to a half (the ALUs to 42 %, the exponentials' unit to 31 %, the tensor pipe to
+// 11 %, L2 to 42 %). Two chains an SM of 128-key steps, two warps a set of rows, were 736 us where these are
 // 462, largely for the registers that the scores took then. Measured: 1,024 samples of up to 544
 // tokens, 8 heads of 32, window 128 + 4: 462 us; 64 of 2,000, window 256 + 8: 150 us; 2 of 8,191, 4
 // heads of 64, window 1,024 + 16: 43 us, 240 TFLOP/s.
@@ -29,7 +29,7 @@
 //                       heads that share the key head follow one another)
 // Recomputing S and dP in the second launch costs two products more than one launch that adds
 // dQ to memory would, and needs no fp32 buffer, no clearing, no atomics: every sum has one
-// owner and one order. Bound like the forward (schedulers 44 to 50 %, L2 33 %). Measured, queries |
+// owner and one order. Bound like the forward (schedulers 44 to 54 %, L2 33 %). Measured, queries |
 // keys: 661 | 700 us on the first of the shapes above, 52 | 70 us on the last.
 //
 // Rounding to bf16: P and dS are the A operands of products with bf16 tiles, which tcgen05 takes
