@@ -286,7 +286,9 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKVCache, rows: torch.Tenso
     cache), or, with fresh keys ``k_new, v_new [B, N, kv_heads * head_dim]`` that are not in the
     cache, at ``length + n``. It sees the positions up to its own: all of them (``window`` 0),
     or the last ``window`` and the first ``sinks``; a query that sees none gives zero. Heads
-    ``g * heads / kv_heads ..`` share key head ``g``. ``scale`` (positive) defaults to ``head_dim ** -0.5``."""
+    ``g * heads / kv_heads ..`` share key head ``g``. ``scale`` (positive) defaults to ``head_dim ** -0.5``.
+    On the GPU an infinity or a NaN in a cached token reaches only the queries that see it; one in
+    ``v_new`` may reach every query of its batch row."""
 
     with trace_range("mdl.attention.cached"):
         if scale is not None and not 0.0 < scale < math.inf:

@@ -15,7 +15,9 @@ tokens stay visible because a softmax trained with a window parks weight on them
 * the queries are the last ``lq`` tokens; padding is a per-sample prefix (``kstart``), is
   never read, and its queries give zero;
 * returns ``[B, lq, heads * head_dim]``; the gradient of a shared key head sums over the
-  query heads that share it.
+  query heads that share it;
+* an infinity or a NaN in a valid token may reach every query of its sample, also those that
+  do not see the token (a weight of zero times it is a NaN).
 
 CUDA: the tcgen05 kernels of ``csrc/window_attn.cu`` (bf16, head widths 32 and 64), forward
 and backward without atomics. CPU: the same contract in fp32 PyTorch.
