@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   if (hi > 0) {
     const int end = (hi + CH - 1) / CH;
     if (W > 0) {
-      cw = max(0, qmin - W + 1) / CH;
+      cw = min(max(0, qmin - W + 1) / CH, end);  // the window of late fresh tokens lies past the row
       cs = min((min(S, hi) + CH - 1) / CH, cw);
     }
     total = cs + end - cw;

@@ -492,3 +492,39 @@ def test_split_calls_that_follow_one_another():
         graph.replay()
         assert torch.equal(outs[0], single[i]) and torch.equal(outs[1], single[i + 1])
     _check_errors("cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("H,G", [(2, 2), (2, 1)])
+@pytest.mark.parametrize("N,window,sinks", [(40, 1, 4), (64, 1, 4), (64, 8, 4), (96, 8, 4), (100, 32, 70), (128, 48, 4)])
+def test_candidates_whose_window_has_left_the_cache(device, hd, H, G, N, window, sinks):
+    """More fresh tokens than the window: the later queries see the sinks alone of the cache."""
+
+    _attend_case(device, [31, 32, 64, 96, 100, 128, 3], N, H, G, hd, window, sinks, True, rows=[2, 0, 1, 3, 6, 5, 4])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("N,window,sinks", [(40, 1, 4), (100, 32, 4), (128, 48, 4)])
+def test_candidates_far_past_long_rows(device, N, window, sinks):
+    for hd in (32, 64):
+        _attend_case(device, [1920, 1984, 2000], N, 1, 1, hd, window, sinks, True)
+
+
+@GPU
+def test_many_candidates_whose_window_has_left_the_cache():
+    """The same with one warp an item: as many candidates as fill the device."""
+
+    lengths, N, H, hd = [32, 64, 100, 333], 40, 4, 32
+    R, B, T = len(lengths), 700, max(lengths)
+    cache = _shuffled(R, T, H, hd, 64, "cuda")
+    k, v = _kv(R, T, H, hd, "cuda", 2)
+    kv_cache_write(cache, k, v, start=_int([0] * R, "cuda"), kstart=_int([T - x for x in lengths], "cuda"))
+    g = torch.Generator().manual_seed(1)
+    q, kn, vn = torch.randn(B, N, 3 * H * hd, generator=g).bfloat16().cuda().chunk(3, -1)
+    rows = torch.randint(0, R, (B,), generator=g).int().cuda()
+    got = cached_attention(q, cache, rows=rows, k_new=kn, v_new=vn, window=1, sinks=4)
+    ref = cached_attention_reference(q, cache, rows, kn, vn, 1, 4)
+    # |o| <= max |v| of what is seen: unit-normal values stay below 6
+    assert (got.float() - ref).abs().max() <= 1.05 * 2.0 ** -7 * 6
+    _check_errors("cuda")
