@@ -402,7 +402,7 @@ constexpr int ring_steps() { return HD == 64 ? 2 : 3; }
 template <int HD, int NT, int WPI>
 constexpr int attend_smem() {
   constexpr int warps = WPI == 1 ? 4 : WPI;
-  constexpr int ring = warps * ring_steps<HD>() * (step_bytes<HD, NT>() + 8);
+  constexpr int ring = warps * ring_steps<HD>() * (step_bytes<HD, NT>() + 8) + warps * 4;
   constexpr int join = WPI == 1 ? 0 : WPI * 8 * NT * (HD + 6) * 4;
   return ring > join ? ring : join;
 }
@@ -418,6 +418,17 @@ __device__ __forceinline__ void bulk_copy(uint8_t* dst, const void* src, uint32_
 // The rest of a wait that is not over at once; the same outcome on every lane.
 __device__ __noinline__ bool ring_wait(uint64_t* bar, uint32_t parity, int* err) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, nullptr));
+}
+
+// Bit j: the 16-key tile at k0 + 16 j (below len) lies in a page outside the cache. Out of line: it
+// is looked at only once a page has been found missing.
+__device__ __noinline__ uint32_t missing_tiles(const KvCache& c, const int* table, int k0, int len, int tiles) {
+  uint32_t gone = 0;
+  for (int j = 0; j < tiles && k0 + 16 * j < len; ++j) {
+    const int q = __ldg(table + ((k0 + 16 * j) >> c.page_shift));
+    if (static_cast<unsigned>(q) >= static_cast<unsigned>(c.num_pages)) gone |= 1u << j;
+  }
+  return gone;
 }
 
 template <int HD, int NT, int WPI>
@@ -550,6 +561,13 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   constexpr int WARPS = WPI == 1 ? 4 : WPI;
   uint8_t* ring = sm_ring + warp * RING * STEP;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm_ring + WARPS * RING * STEP) + warp * RING;
+  // Steps from all_lo + 1 (or up to S) to all_hi are visible to every query of the block. Once the warp
+  // has met a page outside the cache, none is: every step is masked, by another look at the table. (In
+  // shared memory: as a register that changes it made the kernels spill.)
+  constexpr int BAD_PAGE = -0x7fffffff - 1;
+  volatile int* all_hi = reinterpret_cast<volatile int*>(sm_ring + WARPS * RING * (STEP + 8)) + warp;
+  *all_hi = min(len, qmin + 1) - CH;
+  const int all_lo = W > 0 ? qmax - W : -1, all_sink = S - CH;
   if (lane == 0) {
     for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1);
     fence_barrier_init();
@@ -570,6 +588,7 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     const int q = __ldg(table + (k0 >> c.page_shift));
     if (static_cast<unsigned>(q) < static_cast<unsigned>(c.num_pages)) return q;
     record_error(c.err, MDL_ERR_BAD_INDEX);
+    *all_hi = BAD_PAGE;  // page 0 is copied in its place and hidden
     return 0;
   };
   auto pages = [&](int i) {
@@ -617,8 +636,6 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
     fetch(part + s * parts, s);
   }
   pages(part + RING * parts);
-  // steps from all_lo + 1 (or up to S) to all_hi are visible to every query of the block
-  const int all_hi = min(len, qmin + 1) - CH, all_lo = W > 0 ? qmax - W : -1, all_sink = S - CH;
   int st = 0;
   uint32_t phase = 0;
 #pragma unroll 1
@@ -684,15 +701,16 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
       }
     }
     // every key of the step visible to every query of the block?
-    const bool whole = k0 <= all_hi && (k0 > all_lo || k0 <= all_sink);
+    const bool whole = k0 <= *all_hi && (k0 > all_lo || k0 <= all_sink);
     if (!whole) {
+      const uint32_t gone = *all_hi == BAD_PAGE ? missing_tiles(c, table, k0, len, KT) : 0u;
       uint32_t reach[KT][2];  // a key is visible to the queries less than this far on
 #pragma unroll
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int kp = k0 + 16 * j + 8 * h + row8;
-          reach[j][h] = kp >= len ? 0u : (W == 0 || kp < S ? 0x80000000u : static_cast<uint32_t>(W));
+          reach[j][h] = kp >= len || (gone >> j & 1u) != 0 ? 0u : (W == 0 || kp < S ? 0x80000000u : static_cast<uint32_t>(W));
         }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)

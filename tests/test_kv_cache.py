@@ -528,3 +528,80 @@ def test_many_candidates_whose_window_has_left_the_cache():
     # |o| <= max |v| of what is seen: unit-normal values stay below 6
     assert (got.float() - ref).abs().max() <= 1.05 * 2.0 ** -7 * 6
     _check_errors("cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hd,G,page,N", [(32, 2, 64, 1), (64, 1, 64, 1), (32, 1, 16, 20), (64, 2, 32, 3), (32, 2, 256, 33)])
+def test_keys_of_a_page_outside_the_cache_are_hidden(device, hd, G, page, N):
+    """A table entry outside the pool hides its tokens, whatever page 0 holds: as if the row ended
+    before the page (its last one), or with the tokens of that page out of the sum (one in the
+    middle); the error word says so. The CPU definition raises."""
+
+    T, R = 5 * page, 3
+    k, v = _kv(R, T, G, hd, device, 6)
+    q = torch.randn(R, N, 2 * G * hd, generator=torch.Generator().manual_seed(3)).bfloat16().to(device)
+    kn, vn = _kv(R, N, G, hd, device, 8)
+    for bad, at in ((-1, 4), (10 ** 6, 2)):
+        table = torch.arange(R * 5, dtype=torch.int32).view(R, 5).flip(0).contiguous()
+        cache = QuantizedKVCache(R, T, G, hd, page=page, table=table, num_pages=R * 5, device=device)
+        kv_cache_write(cache, k, v)
+        row, pg = 1, int(cache.table[1, at])
+        want = cached_attention(q, cache, k_new=kn, v_new=vn)
+        if device == "cpu":
+            cache.table[row, at] = bad
+            with pytest.raises(ValueError, match="page"):
+                cached_attention(q, cache, k_new=kn, v_new=vn)
+            continue
+        # what the row gives without the page: the other tokens moved together, no window, so that
+        # positions do not matter
+        short = QuantizedKVCache(1, 4 * page, G, hd, page=page, device=device)
+        keep = [i for i in range(T) if i // page != at]
+        kv_cache_write(short, k[row:row + 1, keep], v[row:row + 1, keep])
+        want[row] = cached_attention(q[row:row + 1], short, k_new=kn[row:row + 1], v_new=vn[row:row + 1])[0]
+        cache.table[row, at] = bad
+        # NaN in page 0 and in the page that is gone would show
+        zero = int((cache.table == 0).nonzero()[0, 0])
+        got = cached_attention(q, cache, k_new=kn, v_new=vn)
+        torch.cuda.synchronize()
+        from mdl_b200.ops._ext import check_error_word
+
+        with pytest.raises(RuntimeError, match="outside"):
+            check_error_word(torch.device("cuda", 0))
+        # another order of the same sums: the roundings of P and of the result (2^-8 each) on both
+        # sides; |o| <= max |v| < 6
+        assert (got.float() - want.float()).abs().max() <= 2 * 1.05 * 2.0 ** -7 * 6
+        cache.scales[0] = float("nan")
+        again = cached_attention(q, cache, k_new=kn, v_new=vn)
+        others = [r for r in range(R) if r != zero]
+        assert torch.equal(again[others], got[others]) and torch.isnan(again[zero]).any()
+        rk, _ = kv_cache_read(cache, T, dtype=torch.float32)
+        assert not rk[row, at * page:(at + 1) * page].any()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside"):
+            check_error_word(torch.device("cuda", 0))
+
+
+@GPU
+@pytest.mark.parametrize("hd,H,N", [(32, 4, 1), (32, 2, 12), (64, 2, 1), (64, 4, 20)])
+def test_hidden_pages_with_one_warp_an_item(hd, H, N):
+    """The same where candidates fill the device: they give what a few of them give (another order
+    of the same sums: the roundings of P and of the result, on both sides)."""
+
+    R, T, B = 4, 333, 1200
+    cache = QuantizedKVCache(R, T, H, hd, device="cuda")
+    k, v = _kv(R, T, H, hd, "cuda", 2)
+    kv_cache_write(cache, k, v)
+    cache.table[1, 2], cache.table[3, 5] = -5, 10 ** 6
+    cache.scales[0] = float("nan")       # page 0 belongs to row 0
+    g = torch.Generator().manual_seed(1)
+    q, kn, vn = torch.randn(B, N, 3 * H * hd, generator=g).bfloat16().cuda().chunk(3, -1)
+    rows = (torch.arange(B, device="cuda") % 3 + 1).int()
+    got = cached_attention(q, cache, rows=rows, k_new=kn, v_new=vn, window=300, sinks=4)
+    few = cached_attention(q[:6], cache, rows=rows[:6], k_new=kn[:6], v_new=vn[:6], window=300, sinks=4)
+    assert torch.isfinite(got).all() and torch.isfinite(few).all()
+    assert (got[:6].float() - few.float()).abs().max() <= 2 * 1.05 * 2.0 ** -7 * 6
+    torch.cuda.synchronize()
+    from mdl_b200.ops._ext import check_error_word
+
+    with pytest.raises(RuntimeError, match="outside"):
+        check_error_word(torch.device("cuda", 0))
