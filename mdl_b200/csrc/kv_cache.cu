@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int c
   for (int base = 0; base < units; base += UNITS, next()) {  // whole warps stay together: shuffles below
     const bool live = u < units;
     const int g = token_fast ? slow : fast, t = t0 + (token_fast ? fast : slow);
-    const int pos = start + t - first;
-    const bool in = live && t >= first;
+    const int at = t - first;  // behind start
+    const bool in = live && at >= 0;
     uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
     int pg = -1;
     if (in) {
@@ -209,12 +209,14 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int c
       k1 = kp[1];
       v0 = vp[0];
       v1 = vp[1];
-      if (pos >= cap) record_error(c.err, MDL_ERR_CAPACITY);
-      else pg = page_of(c, r, pos);
+      // compared like this, since start + at may pass 32 bits in a long row
+      if (at >= cap - start) record_error(c.err, MDL_ERR_CAPACITY);
+      else pg = page_of(c, r, start + at);
     }
     uint16_t ks, vs;
     const uint2 kc = quantise16<HD>(k0, k1, ks), vc = quantise16<HD>(v0, v1, vs);
     if (pg < 0) continue;
+    const int pos = start + at;
     const long long bk = slot_base(c, pg, g, 0) + (pos & ((1 << c.page_shift) - 1));
     const long long bv = bk + (1ll << c.page_shift);
     reinterpret_cast<uint2*>(c.codes)[bk * LPU + sub] = kc;
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvWriteArgs a, int c
   // only the single block of a row may write the length that its threads read above
   if (chunks == 1) {
     __syncthreads();
-    if (threadIdx.x == 0) c.lengths[r] = min(start + a.T - first, cap);
+    if (threadIdx.x == 0) c.lengths[r] = start + min(a.T - first, cap - start);
   }
 }
 
@@ -239,7 +241,7 @@ __global__ void kv_length_kernel(KvWriteArgs a) {
   const int first = a.kstart != nullptr ? min(max(a.kstart[i], 0), a.T) : 0;
   const int start = a.start != nullptr ? a.start[i] : c.lengths[r];
   if (start < 0 || start > cap) return;
-  c.lengths[r] = min(start + a.T - first, cap);
+  c.lengths[r] = start + min(a.T - first, cap - start);
 }
 
 // ============================================================================ codes

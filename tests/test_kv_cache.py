@@ -605,3 +605,31 @@ def test_hidden_pages_with_one_warp_an_item(hd, H, N):
 
     with pytest.raises(RuntimeError, match="outside"):
         check_error_word(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [2, 2 ** 20 + 70])
+def test_write_at_the_end_of_a_row_of_two_billion_positions(device, T):
+    """Positions past the capacity that 32 bits cannot hold are past the capacity too."""
+
+    page = 2 ** 20
+    per = 2 ** 31 // page - 1
+    table = torch.zeros(1, per, dtype=torch.int32)
+    cache = QuantizedKVCache(1, per * page, 1, 32, page=page, table=table, num_pages=1, device=device)
+    k, v = _kv(1, 1, 1, 32, device)
+    k, v = k.expand(1, T, 32), v.expand(1, T, 32)
+    start = _int([cache.capacity - 1], device)
+    if device == "cpu":
+        with pytest.raises(ValueError, match="full"):
+            kv_cache_write(cache, k, v, start=start)
+        return
+    kv_cache_write(cache, k, v, start=start)
+    torch.cuda.synchronize()
+    from mdl_b200.ops._ext import check_error_word
+
+    with pytest.raises(RuntimeError, match="overflow"):
+        check_error_word(torch.device("cuda", 0))
+    assert cache.lengths.tolist() == [cache.capacity]
+    got, _ = kv_cache_read(cache, 1, start=start, dtype=torch.float32)
+    assert torch.equal(got[0, 0].double(), _round4(k[0, :1])[0])
+    _check_errors(device)
