@@ -129,6 +129,13 @@ def _index(t: torch.Tensor | None, n: int, cache: QuantizedKVCache, name: str) -
     return t
 
 
+def _rows(t: torch.Tensor | None, n: int, cache: QuantizedKVCache) -> torch.Tensor | None:
+    t = _index(t, n, cache, "rows")
+    if t is not None and bool(((t < 0) | (t >= cache.rows)).any()):
+        raise IndexError(f"key/value cache: rows outside the cache's {cache.rows}")
+    return t
+
+
 def _tokens(t: torch.Tensor, width: int, cache: QuantizedKVCache, name: str) -> None:
     if t.dim() != 3 or t.shape[2] != width:
         raise ValueError(f"{name} {tuple(t.shape)}, expected [rows, tokens, {width}]")
@@ -200,7 +207,7 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, st
         if rows is None and n != cache.rows:
             raise ValueError(f"{n} source rows for {cache.rows} cache rows: give rows")
         kv_cache_write_reference(cache, k, v, _index(start, n, cache, "start"), _index(kstart, n, cache, "kstart"),
-                                 _index(rows, n, cache, "rows"))
+                                 _rows(rows, n, cache))
 
 
 # ----------------------------------------------------------------------------- read
@@ -220,7 +227,7 @@ def kv_cache_read(cache: QuantizedKVCache, count: int, start: torch.Tensor | Non
         if count < 0:
             raise ValueError(f"count {count}")
         n = cache.rows if rows is None else rows.shape[0]
-        rows = _index(rows, n, cache, "rows")
+        rows = _rows(rows, n, cache)
         start = _index(start, n, cache, "start")
         width = cache.kv_heads * cache.head_dim
         r = (torch.arange(n) if rows is None else rows.long()).view(-1, 1)
@@ -307,7 +314,7 @@ def cached_attention(q: torch.Tensor, cache: QuantizedKVCache, rows: torch.Tenso
         _tokens(q, width, cache, "q")
         if rows is None and B != cache.rows:
             raise ValueError(f"{B} batch rows for {cache.rows} cache rows: give rows")
-        rows = _index(rows, B, cache, "rows")
+        rows = _rows(rows, B, cache)
         if k_new is not None:
             _tokens(k_new, G * hd, cache, "k_new")
             _tokens(v_new, G * hd, cache, "v_new")

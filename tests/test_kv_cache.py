@@ -633,3 +633,29 @@ def test_write_at_the_end_of_a_row_of_two_billion_positions(device, T):
     got, _ = kv_cache_read(cache, 1, start=start, dtype=torch.float32)
     assert torch.equal(got[0, 0].double(), _round4(k[0, :1])[0])
     _check_errors(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_negative_rows_are_outside(device):
+    """Row -1 is no row, not the last one."""
+
+    cache = QuantizedKVCache(2, 32, 1, 32, device=device)
+    k, v = _kv(2, 4, 1, 32, device)
+    kv_cache_write(cache, k, v)
+    q = torch.ones(1, 1, 32, dtype=torch.bfloat16, device=device)
+    for call in (lambda: kv_cache_write(cache, k[:1], v[:1], rows=_int([-1], device)),
+                 lambda: kv_cache_read(cache, 4, rows=_int([-1], device)),
+                 lambda: cached_attention(q, cache, rows=_int([-1], device))):
+        if device == "cpu":
+            with pytest.raises(IndexError):
+                call()
+        else:
+            from mdl_b200.ops._ext import check_error_word
+
+            out = call()
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="outside"):
+                check_error_word(torch.device("cuda", 0))
+            if out is not None:
+                assert not any(x.any() for x in (out if isinstance(out, tuple) else (out,)))
+        assert cache.lengths.tolist() == [4, 4]
