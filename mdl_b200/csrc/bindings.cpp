@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -1033,13 +1034,16 @@ at::Tensor kv_rows(const at::Tensor& t, int64_t n, int64_t T, int64_t width, con
 
 const __nv_bfloat16* bf16_ptr(const at::Tensor& t) { return reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()); }
 
-// [n] whole numbers as contiguous int32 (undefined: not given).
+// [n] whole numbers as contiguous int32 (undefined: not given). Wider ones are clamped first: past
+// 32 bits they lie outside any cache, on either side, and must not wrap into it.
 at::Tensor kv_index(const std::optional<at::Tensor>& t, int64_t n, const at::Tensor& codes, const char* name) {
   if (!t.has_value() || !t->defined()) return at::Tensor();
   if (!at::isIntegralType(t->scalar_type(), false)) type_error(name, " holds whole numbers, not ", t->scalar_type());
   if (t->dim() != 1 || t->size(0) != n) value_error(name, " ", t->sizes(), ", expected [", n, "]");
   if (!same_device(*t, codes)) value_error(name, " on ", t->device(), ", the cache on ", codes.device());
-  return t->scalar_type() == at::kInt && t->is_contiguous() ? *t : t->to(at::kInt).contiguous();
+  if (t->scalar_type() == at::kInt) return t->contiguous();
+  const at::Tensor wide = t->element_size() >= 4 ? t->to(at::kLong).clamp(INT32_MIN, INT32_MAX) : *t;
+  return wide.to(at::kInt).contiguous();
 }
 
 const int* int_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }

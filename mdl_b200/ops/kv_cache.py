@@ -70,6 +70,8 @@ class QuantizedKVCache:
                 raise ValueError(f"key/value cache: table {tuple(table.shape)}, expected {(rows, per_row)}")
             if table.is_floating_point():
                 raise TypeError("key/value cache: the page table holds whole numbers")
+            if table.dtype is not torch.int32:  # past 32 bits: outside any cache, not wrapped into it
+                table = table.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
             table = table.to(device=device, dtype=torch.int32).contiguous()
         self.rows, self.kv_heads, self.head_dim, self.page = rows, kv_heads, head_dim, page
         self.num_pages, self.device = num_pages, device

@@ -659,3 +659,49 @@ def test_negative_rows_are_outside(device):
             if out is not None:
                 assert not any(x.any() for x in (out if isinstance(out, tuple) else (out,)))
         assert cache.lengths.tolist() == [4, 4]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_indexes_past_32_bits_do_not_wrap(device):
+    """64-bit rows, starts and pages that 32 bits would turn into valid ones are outside."""
+
+    big = 2 ** 32
+    cache = QuantizedKVCache(2, 32, 1, 32, page=16, device=device)
+    k, v = _kv(2, 4, 1, 32, device)
+    kv_cache_write(cache, k, v)
+    held = kv_cache_read(cache, 32, dtype=torch.float32)[0].clone()
+    wide = lambda *x: torch.tensor(x, dtype=torch.int64, device=device)
+    q = torch.ones(1, 1, 32, dtype=torch.bfloat16, device=device)
+    calls = [lambda: kv_cache_write(cache, k[:1], v[:1], rows=wide(big + 1)),
+             lambda: kv_cache_write(cache, k, v, start=wide(big, big + 2)),
+             lambda: kv_cache_write(cache, k[:1], v[:1], rows=wide(-big)),
+             lambda: kv_cache_read(cache, 4, rows=wide(big)),
+             lambda: kv_cache_read(cache, 4, start=wide(-big, -big)),
+             lambda: cached_attention(q, cache, rows=wide(big + 1))]
+    for call in calls:
+        if device == "cpu":
+            with pytest.raises((ValueError, IndexError)):
+                call()
+        else:
+            from mdl_b200.ops._ext import check_error_word
+
+            out = call()
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="outside"):
+                check_error_word(torch.device("cuda", 0))
+            if out is not None:
+                assert not any(x.any() for x in (out if isinstance(out, tuple) else (out,)))
+        assert cache.lengths.tolist() == [4, 4]
+        assert torch.equal(kv_cache_read(cache, 32, dtype=torch.float32)[0], held)
+    # padding past the last token is all of it, before the first is none
+    kv_cache_write(cache, k, v, start=wide(0, 0), kstart=wide(big, -big))
+    assert cache.lengths.tolist() == [0, 4]
+    paged = QuantizedKVCache(1, 32, 1, 32, page=16, table=torch.tensor([[big, big + 1]]), num_pages=2, device=device)
+    if device == "cpu":
+        with pytest.raises(ValueError, match="page"):
+            kv_cache_write(paged, k[:1], v[:1])
+    else:
+        kv_cache_write(paged, k[:1], v[:1])
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside"):
+            check_error_word(torch.device("cuda", 0))
