@@ -114,7 +114,8 @@ def windowed_attention(qkv: torch.Tensor, kstart: torch.Tensor, heads: int, lq: 
             if qkv.data_ptr() % 16:
                 qkv = qkv.clone()
         ks = kstart
-        if ks.dtype is not torch.int32 or not ks.is_contiguous():
-            ks = ks.to(torch.int32).contiguous()
+        if ks.dtype is not torch.int32:
+            ks = ks.to(torch.int64).clamp(0, Lk).to(torch.int32)  # what lies past 32 bits must not wrap
+        ks = ks.contiguous()
         return ext().windowed_attention(qkv, ks, heads, G, lq, min(window, Lk), min(sinks, Lk),
                                         scale or 0.0, error_word(qkv.device))

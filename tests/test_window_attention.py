@@ -325,3 +325,14 @@ def test_scale_is_positive(device, scale):
     qkv = torch.zeros(2, 16, 3 * 2 * 32, dtype=torch.bfloat16, device=device)
     with pytest.raises(ValueError, match="scale"):
         windowed_attention(qkv, torch.zeros(2, dtype=torch.int32, device=device), 2, 16, 4, scale=scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_starts_past_32_bits_do_not_wrap(device):
+    """A 64-bit start past the sample's end is all padding, one far below 0 is none."""
+
+    qkv, _ = _inputs(3, 50, 50, 2, 2, 32, device)
+    x = qkv if device == "cuda" else qkv.float()
+    got = windowed_attention(x, torch.tensor([2 ** 32, -2 ** 32 + 7, 5], device=device), 2, 50, 9, 1)
+    want = windowed_attention(x, torch.tensor([50, 0, 5], device=device), 2, 50, 9, 1)
+    assert torch.equal(got, want) and not got[0].any() and got[1, 0].any()
