@@ -92,12 +92,15 @@ class QuantizedKVCache:
         return self.codes.numel() + 2 * self.scales.numel()
 
     def reset(self, rows: torch.Tensor | None = None) -> None:
-        """Empties the cache, or only ``rows``."""
+        """Empties the cache, or only ``rows`` (whole numbers)."""
 
         if rows is None:
             self.lengths.zero_()
-        else:
-            self.lengths[rows.long()] = 0
+            return
+        rows = rows.reshape(-1).to(self.device)
+        none = torch.empty(rows.shape[0], 0, self.kv_heads * self.head_dim, dtype=torch.bfloat16, device=self.device)
+        # nothing written from position 0: rows outside the cache are met like those of any write
+        kv_cache_write(self, none, none, start=torch.zeros_like(rows, dtype=torch.int32), rows=rows)
 
     # ------------------------------------------------------------------ definition in PyTorch
     def _slots(self, rows: torch.Tensor, pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -705,3 +705,33 @@ def test_indexes_past_32_bits_do_not_wrap(device):
         torch.cuda.synchronize()
         with pytest.raises(RuntimeError, match="outside"):
             check_error_word(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_reset_of_rows_outside_the_cache(device):
+    """On CUDA they are skipped and recorded, on the CPU refused; no valid row is emptied for them."""
+
+    cache = QuantizedKVCache(4, 32, 1, 32, device=device)
+    k, v = _kv(4, 3, 1, 32, device)
+    kv_cache_write(cache, k, v)
+    for rows in ([4], [-1], [1, 2 ** 40]):
+        rows = torch.tensor(rows, device=device)
+        if device == "cpu":
+            with pytest.raises(IndexError):
+                cache.reset(rows)
+            assert cache.lengths.tolist() == [3, 3, 3, 3]
+            continue
+        from mdl_b200.ops._ext import check_error_word
+
+        cache.reset(rows)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="outside"):
+            check_error_word(torch.device("cuda", 0))
+        assert cache.lengths.tolist() == [3, 3 if len(rows) == 1 else 0, 3, 3]
+    cache.reset(torch.tensor([[3, 0], [3, 3]], dtype=torch.int16))     # any shape, from the host too
+    assert cache.lengths.tolist()[0] == 0 and cache.lengths.tolist()[3] == 0
+    cache.reset(torch.tensor([], dtype=torch.int64, device=device))
+    assert cache.lengths.tolist()[2] == 3
+    with pytest.raises(TypeError):
+        cache.reset(torch.tensor([True, False, True, False], device=device))
+    _check_errors(device)
