@@ -1059,11 +1059,12 @@ void kv_write(const at::Tensor& codes, const at::Tensor& scales, const at::Tenso
   TORCH_CHECK(T < (int64_t{1} << 30) && n < (int64_t{1} << 30), "kv_write: sizes");
   const at::Tensor kr = kv_rows(k, n, T, width, codes, "k", &a.k_sb, &a.k_st);
   const at::Tensor vr = kv_rows(v, n, T, width, codes, "v", &a.v_sb, &a.v_st);
-  const at::Tensor ri = kv_index(rows, n, codes, "rows"), fi = kv_index(kstart, n, codes, "kstart");
-  at::Tensor si = kv_index(start, n, codes, "start");
+  at::Tensor ri = kv_index(rows, n, codes, "rows"), si = kv_index(start, n, codes, "start"),
+             fi = kv_index(kstart, n, codes, "kstart");
   if (!ri.defined() && n != a.c.R) value_error(n, " source rows for ", a.c.R, " cache rows: give rows");
-  // the kernel writes the lengths
-  if (si.defined() && si.storage().data_ptr().get() == lengths.storage().data_ptr().get()) si = si.clone();
+  // the kernel writes the lengths while other blocks read these
+  for (at::Tensor* t : {&ri, &si, &fi})
+    if (t->defined() && t->storage().data_ptr().get() == lengths.storage().data_ptr().get()) *t = t->clone();
   a.k = bf16_ptr(kr);
   a.v = bf16_ptr(vr);
   a.rows = int_ptr(ri);

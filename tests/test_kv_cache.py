@@ -735,3 +735,18 @@ def test_reset_of_rows_outside_the_cache(device):
     with pytest.raises(TypeError):
         cache.reset(torch.tensor([True, False, True, False], device=device))
     _check_errors(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_indexes_may_lie_in_the_lengths_memory(device):
+    """kstart read from the lengths that the write replaces, rows in another order."""
+
+    R, T = 4096, 6
+    cache = QuantizedKVCache(R, 16, 1, 32, page=16, device=device)
+    first = torch.arange(R, dtype=torch.int32) % 5
+    cache.lengths.copy_(first)
+    k, v = _kv(R, T, 1, 32, device)
+    rows = torch.arange(R - 1, -1, -1, dtype=torch.int32, device=device)
+    kv_cache_write(cache, k, v, start=torch.zeros(R, dtype=torch.int32, device=device), kstart=cache.lengths, rows=rows)
+    assert torch.equal(cache.lengths.cpu(), (T - first).flip(0))
+    _check_errors(device)
