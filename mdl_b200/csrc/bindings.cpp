@@ -973,7 +973,7 @@ mdl::KvCache kv_cache_of(const at::Tensor& codes, const at::Tensor& scales, cons
   while ((int64_t{1} << c.page_shift) < page) ++c.page_shift;
   c.hd = static_cast<int>(codes.size(4) * 2);
   TORCH_CHECK(c.hd == 32 || c.hd == 64, "head width must be 32 or 64");
-  TORCH_CHECK(codes.size(0) >= 1 && table.size(1) >= 1 && table.size(1) * page < (int64_t{1} << 31), "cache sizes");
+  TORCH_CHECK((codes.size(0) >= 1 || table.size(1) == 0) && table.size(1) * page < (int64_t{1} << 31), "cache sizes");
   c.codes = codes.data_ptr<uint8_t>();
   c.scales = reinterpret_cast<__nv_bfloat16*>(scales.data_ptr());
   c.table = table.data_ptr<int>();

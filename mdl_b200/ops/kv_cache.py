@@ -40,13 +40,13 @@ class QuantizedKVCache:
     ``table [rows, ceil(max_tokens / page)]`` (int32) names the page of each run of
     ``page`` positions; by default row ``r`` owns pages ``r * per_row ..``. A table with
     fewer pages than that (``num_pages``) is the caller's to fill before it writes. A page
-    may be shared between rows that only read it."""
+    may be shared between rows that only read it. ``max_tokens`` 0: rows that hold nothing."""
 
     def __init__(self, rows: int, max_tokens: int, kv_heads: int, head_dim: int, page: int = 64,
                  table: torch.Tensor | None = None, num_pages: int | None = None, device=None) -> None:
-        if rows < 1 or max_tokens < 1 or kv_heads < 1:
-            raise ValueError(f"key/value cache: rows {rows}, max_tokens {max_tokens} and kv_heads {kv_heads} must be "
-                             "positive")
+        if rows < 1 or max_tokens < 0 or kv_heads < 1:
+            raise ValueError(f"key/value cache: rows {rows} and kv_heads {kv_heads} must be positive, max_tokens "
+                             f"{max_tokens} not negative")
         if head_dim not in HEAD_DIMS:
             raise NotImplementedError(f"key/value cache: head width {head_dim}, the cache takes {HEAD_DIMS}")
         if page < 16 or page & (page - 1):
@@ -59,7 +59,7 @@ class QuantizedKVCache:
             device = torch.device("cuda", torch.cuda.current_device())
         if num_pages is None:
             num_pages = rows * per_row
-        if num_pages < 1:
+        if num_pages < min(per_row, 1):
             raise ValueError(f"key/value cache: num_pages {num_pages}")
         if table is None:
             if num_pages < rows * per_row:

@@ -750,3 +750,31 @@ def test_indexes_may_lie_in_the_lengths_memory(device):
     kv_cache_write(cache, k, v, start=torch.zeros(R, dtype=torch.int32, device=device), kstart=cache.lengths, rows=rows)
     assert torch.equal(cache.lengths.cpu(), (T - first).flip(0))
     _check_errors(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_empty_cache(device):
+    """Rows of no positions: nothing is held, candidates see their own tokens alone."""
+
+    cache = QuantizedKVCache(2, 0, 1, 32, device=device)
+    assert cache.capacity == 0 and cache.nbytes == 0
+    k, v = _kv(2, 3, 1, 32, device)
+    kv_cache_write(cache, k[:, :0], v[:, :0])
+    rk, rv = kv_cache_read(cache, 2)
+    assert rk.shape == (2, 2, 32) and not rk.any() and not rv.any()
+    assert not cached_attention(k, cache).any()
+    other = QuantizedKVCache(2, 5, 1, 32, device=device)
+    assert torch.equal(cached_attention(k, cache, k_new=k, v_new=v), cached_attention(k, other, k_new=k, v_new=v))
+    _check_errors(device)
+    if device == "cpu":
+        with pytest.raises(ValueError, match="full"):
+            kv_cache_write(cache, k, v)
+    else:
+        from mdl_b200.ops._ext import check_error_word
+
+        kv_cache_write(cache, k, v)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="overflow"):
+            check_error_word(torch.device("cuda", 0))
+    with pytest.raises(ValueError):
+        QuantizedKVCache(2, -1, 1, 32, device=device)

@@ -142,3 +142,37 @@ def test_four_bit_request_cache(device, window, sinks, heads):
     if device == "cuda":
         torch.cuda.synchronize()
         check_error_word(0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (5, 2)])
+def test_four_bit_request_cache_of_a_pyramid_that_halves_to_nothing(device, window, sinks):
+    """Layers that keep no sequence token have an empty cache: candidates see their own tokens
+    alone. Against a full cache of the values that the 4-bit one stands for, as above."""
+
+    m, spec = _config(seq_len=16, layers=6, min_len=3, pyramid_round_to=1, pyramid_halve_every=1,
+                      attention_window=window, attention_sinks=sinks, request_cache_format="4bit")
+    cfg = app_config_from_mapping(m)
+    torch.manual_seed(0)
+    model = build_model(cfg, device=device, base_seed=1).eval()
+    assert model.query_counts[-2:] == [0, 0]
+    rb = _requests(SyntheticGenerator(model.encoder.batch_plan, spec).batch(12), cfg, 12, 4).to(device)
+    with torch.no_grad():
+        cache = model.precompute_request_cache(rb)
+        scores = model.forward_with_cache(rb, cache)
+        layers = []
+        for s_in, (kv, kst) in zip([16, *model.query_counts], cache["layers"]):
+            k, v = kv_cache_read(kv, s_in, dtype=torch.float32)
+            back = torch.zeros(k.shape[0], s_in, 2 * k.shape[2], device=k.device)
+            for r in range(k.shape[0]):
+                n = int(kv.lengths[r])
+                assert n == s_in - int(kst[r])
+                back[r, s_in - n:] = torch.cat([k[r, :n], v[r, :n]], -1)
+            layers.append((back, kst))
+        assert cache["layers"][-1][0].nbytes == 0
+        want = model.forward_with_cache(rb, {**cache, "layers": layers})
+    tol = 1e-4 if device == "cpu" else 6e-2
+    torch.testing.assert_close(scores, want, atol=tol, rtol=tol)
+    if device == "cuda":
+        torch.cuda.synchronize()
+        check_error_word(0)
