@@ -730,9 +730,10 @@ class OneTransModel(nn.Module):
             xn = _rms_reference(S, layer.norm1, self.eps)
             kv = xn @ layer.wqkv_s[D:].t() + layer.bqkv_s[D:]                   # [R, s_in, 2D]
             if four_bits:
-                cache = QuantizedKVCache(R, s_in, self.attn_heads, self.head_dim, device=kv.device)
-                kv = kv.to(torch.bfloat16)
-                kv_cache_write(cache, kv[..., :D], kv[..., D:], kstart=kst)
+                cache = QuantizedKVCache(max(R, 1), s_in, self.attn_heads, self.head_dim, device=kv.device)
+                if R > 0:  # a batch may hold no request
+                    kv = kv.to(torch.bfloat16)
+                    kv_cache_write(cache, kv[..., :D], kv[..., D:], kstart=kst)
                 layers.append((cache, kst))
             else:
                 layers.append((kv, kst))

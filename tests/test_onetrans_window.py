@@ -176,3 +176,18 @@ def test_four_bit_request_cache_of_a_pyramid_that_halves_to_nothing(device, wind
     if device == "cuda":
         torch.cuda.synchronize()
         check_error_word(0)
+
+
+@pytest.mark.parametrize("fmt", ["full", "4bit"])
+def test_request_cache_of_no_requests(fmt):
+    m, spec = _config(min_len=3, request_cache_format=fmt)
+    cfg = app_config_from_mapping(m)
+    model = build_model(cfg, device="cpu", base_seed=1).eval()
+    rb = _requests(SyntheticGenerator(model.encoder.batch_plan, spec).batch(4), cfg, 4, 2)
+    seq = rb.sequences["behavior"]
+    none = {"ids": seq["ids"][:, :0], "lengths": seq["lengths"][:0], "row_indices": seq["row_indices"][:0]}
+    rb.sequences["behavior"] = none
+    cache = model.precompute_request_cache(rb)
+    assert len(cache["layers"]) == 3 and cache["kstart"].shape == (0,)
+    if fmt == "4bit":
+        assert not any(kv.lengths.any() for kv, _ in cache["layers"])
