@@ -22,7 +22,7 @@ readout is ``_mdl_logits`` over the final NS tokens and the domain tokens,
 read by one task head per task.
 
 CUDA: the backbone is the OneTrans CUDA path (tcgen05 GEMMs writing the token
-buffer, tcgen05 flash attention); every per-token FFN and projector is a
+buffer, its attention kernels); every per-token FFN and projector is a
 grouped tcgen05 GEMM pair reading the NS rows of the token buffer in place,
 and attention over the NS tokens is the few-query kernel. CPU: the fp32
 PyTorch definitions of both.
@@ -86,9 +86,7 @@ class MDLOneTransModel(MDLDomainMixin, OneTransModel):
             seq_in = grad_ready(seq_in, hooks, nl + 1)
             if self.ns_mode != "auto_split":
                 ns_in = self.ns_tokens(ns_in).to(torch.bfloat16)
-            if self.head_dim != 32:
-                raise NotImplementedError(f"OneTrans head_dim {self.head_dim}: the tcgen05 attention kernels take "
-                                          "head_dim 32 (set runtime.kernel_backend: torch for this model)")
+            self._check_head_dim()
             if self.multi:
                 X = OneTransAssembleFn.apply(seq_in.to(torch.bfloat16), ns_in, kstart, self, L)
             else:

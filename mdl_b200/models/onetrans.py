@@ -624,6 +624,12 @@ class OneTransModel(nn.Module):
             return self._forward_cuda(seq_in, ns_in, kstart, batch, task_scale)
         return self.forward_reference(seq_in, ns_in, kstart, batch, task_scale)
 
+    def _check_head_dim(self) -> None:
+        native_dims = WINDOW_HEAD_DIMS if self.window else NATIVE_HEAD_DIMS
+        if self.head_dim not in native_dims:
+            raise NotImplementedError(f"OneTrans head_dim {self.head_dim}: the native attention kernels take "
+                                      f"{native_dims} (set runtime.kernel_backend: torch for this model)")
+
     def _forward_cuda(self, seq_in, ns_in, kstart, batch, task_scale):
         from ..ops.dense import grad_ready
 
@@ -632,10 +638,7 @@ class OneTransModel(nn.Module):
         seq_in = grad_ready(seq_in, hooks, nl + 1)
         if self.ns_mode != "auto_split":
             ns_in = self.ns_tokens(ns_in).to(torch.bfloat16)
-        native_dims = WINDOW_HEAD_DIMS if self.window else NATIVE_HEAD_DIMS
-        if self.head_dim not in native_dims:
-            raise NotImplementedError(f"OneTrans head_dim {self.head_dim}: the native attention kernels take "
-                                      f"{native_dims} (set runtime.kernel_backend: torch for this model)")
+        self._check_head_dim()
         if self.multi:
             X = OneTransAssembleFn.apply(seq_in.to(torch.bfloat16), ns_in, kstart, self, self.L)
         else:

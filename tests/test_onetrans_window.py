@@ -191,3 +191,41 @@ def test_request_cache_of_no_requests(fmt):
     assert len(cache["layers"]) == 3 and cache["kstart"].shape == (0,)
     if fmt == "4bit":
         assert not any(kv.lengths.any() for kv, _ in cache["layers"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model", [dict(heads=1, attention_window=9, attention_sinks=2), dict(heads=1), dict(heads=8)])
+def test_mdl_onetrans_takes_the_head_widths_that_preflight_promises(model):
+    """64-wide heads, with a window and without, and 8-wide ones: a step against the CPU definition,
+    with the tolerances of the 32-wide one."""
+
+    model = dict(model)
+    heads = model.pop("heads")
+    m, spec = scaled_config(4, 1e-4, num_fields=12, batch=64, seq_len=40, num_layers=3, mdl=True)
+    m["model"].update({"hidden_dim": 128, "token_dim": 64, "num_heads": heads, "num_ns_tokens": 4,
+                       "task_head_hidden_dim": 64, "pyramid_round_to": 8, **model})
+    m["training"].update({"lr_warmup_steps": 0, "dense_optimizer": "adam", "lr_dense": 1e-3})
+    spec.sequences["behavior"].min_len = 10
+    cfg = app_config_from_mapping(m)
+    attention_preflight(cfg, "cuda")
+    torch.manual_seed(0)
+    cpu_model = build_model(cfg, device="cpu", base_seed=1)
+    gpu_model = build_model(cfg, device="cuda", base_seed=1)
+    gpu_model.load_state_dict({k: v.cuda() for k, v in cpu_model.state_dict().items()})
+    gpu_model.store.slab.copy_(cpu_model.store.slab)
+    cpu_tr = Trainer(cfg, cpu_model, device=torch.device("cpu"))
+    gpu_tr = Trainer(cfg, gpu_model, device=torch.device("cuda"))
+    batch = SyntheticGenerator(cpu_model.encoder.batch_plan, spec).batch(64)
+    out_c = cpu_tr.forward_backward(batch)
+    out_g = gpu_tr.forward_backward(batch.to("cuda"))
+    torch.cuda.synchronize()
+    check_error_word(0)
+    torch.testing.assert_close(out_g["logits"].cpu(), out_c["logits"].detach(), atol=6e-2, rtol=6e-2)
+    gc, gg = cpu_tr.dense.grad, gpu_tr.dense.grad.cpu()
+    scale = gc.norm().item()
+    for name in cpu_tr.dense.names:
+        o = cpu_tr.dense.offsets[name]
+        n = cpu_tr.dense.params[name].numel()
+        ref, got = gc[o:o + n], gg[o:o + n]
+        err = (ref - got).norm().item()
+        assert err <= 0.1 * ref.norm().item() + 2e-3 * scale, (name, err, ref.norm().item())
