@@ -1242,8 +1242,7 @@ at::Tensor window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, cons
 struct WindowedAttention : public torch::autograd::Function<WindowedAttention> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv, const at::Tensor& kstart,
                             int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks, double scale,
-                            const at::Tensor& err) {
-    const bool keep = qkv.requires_grad();
+                            const at::Tensor& err, bool keep) {
     auto [out, out_lo, lse] = window_attn_fwd(qkv, kstart, H, G, Lq, window, sinks, scale, err, keep);
     if (keep) {
       ctx->save_for_backward({qkv, kstart, out, *out_lo, lse});
@@ -1262,13 +1261,15 @@ struct WindowedAttention : public torch::autograd::Function<WindowedAttention> {
     at::Tensor d = window_attn_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], dout, n[0], n[1], n[2], n[3], n[4],
                                    ctx->saved_data["scale"].toDouble(), ctx->saved_data["err"].toTensor());
     return {d, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+            at::Tensor(), at::Tensor()};
   }
 };
 
 at::Tensor windowed_attention(const at::Tensor& qkv, const at::Tensor& kstart, int64_t H, int64_t G, int64_t Lq,
                               int64_t window, int64_t sinks, double scale, const at::Tensor& err) {
-  return WindowedAttention::apply(qkv, kstart, H, G, Lq, window, sinks, scale, err);
+  // asked here: inside apply the gradient mode is always off
+  const bool keep = at::GradMode::is_enabled() && qkv.requires_grad();
+  return WindowedAttention::apply(qkv, kstart, H, G, Lq, window, sinks, scale, err, keep);
 }
 
 }  // namespace

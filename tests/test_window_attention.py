@@ -336,3 +336,24 @@ def test_starts_past_32_bits_do_not_wrap(device):
     got = windowed_attention(x, torch.tensor([2 ** 32, -2 ** 32 + 7, 5], device=device), 2, 50, 9, 1)
     want = windowed_attention(x, torch.tensor([50, 0, 5], device=device), 2, 50, 9, 1)
     assert torch.equal(got, want) and not got[0].any() and got[1, 0].any()
+
+
+@GPU
+def test_forward_without_a_gradient_keeps_nothing_for_one():
+    """Under no_grad a forward takes its output and the log-sum-exp, and no more."""
+
+    B, L, H, hd = 64, 512, 8, 32
+    qkv, _ = _inputs(B, L, L, H, H, hd, "cuda")
+    ks = torch.zeros(B, dtype=torch.int32, device="cuda")
+    out_bytes, lse_bytes = 2 * B * L * H * hd, 4 * B * L * H
+    for leaf in (qkv, qkv.clone().requires_grad_()):
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                windowed_attention(leaf, ks, H, L, 50, 2)
+                torch.cuda.synchronize()
+                torch.cuda.reset_peak_memory_stats()
+                before = torch.cuda.memory_allocated()
+                out = windowed_attention(leaf, ks, H, L, 50, 2)
+                assert torch.cuda.max_memory_allocated() - before <= out_bytes + lse_bytes + 4096
+                assert not out.requires_grad
+                del out
