@@ -170,7 +170,8 @@ class OneTransLayerFn(torch.autograd.Function):
                    3 * D)
         ks = kstart.to(torch.int32).contiguous()
         if layer.window:
-            att, att_lo, lse = window_attention_fwd(qkv, ks, heads, heads, Lq, layer.window, layer.sinks)
+            att, att_lo, lse = window_attention_fwd(qkv, ks, heads, heads, Lq, layer.window, layer.sinks,
+                                                    keep=ctx.needs_input_grad[0])
         else:
             att = torch.empty(B, Lq, D, dtype=torch.bfloat16, device=dev)
             att_lo = None

@@ -229,3 +229,31 @@ def test_mdl_onetrans_takes_the_head_widths_that_preflight_promises(model):
         ref, got = gc[o:o + n], gg[o:o + n]
         err = (ref - got).norm().item()
         assert err <= 0.1 * ref.norm().item() + 2e-3 * scale, (name, err, ref.norm().item())
+
+
+@pytest.mark.gpu
+def test_evaluation_keeps_nothing_for_a_backward(monkeypatch):
+    from mdl_b200.models import onetrans
+
+    kept = []
+    native = onetrans.window_attention_fwd
+
+    def spy(*args, **kw):
+        res = native(*args, **kw)
+        kept.append(res[1] is not None)
+        return res
+
+    monkeypatch.setattr(onetrans, "window_attention_fwd", spy)
+    m, spec = _config(attention_window=9, attention_sinks=2)
+    cfg = app_config_from_mapping(m)
+    torch.manual_seed(0)
+    model = build_model(cfg, device="cuda", base_seed=1)
+    trainer = Trainer(cfg, model, device=torch.device("cuda"))
+    batch = SyntheticGenerator(model.encoder.batch_plan, spec).batch(16).to("cuda")
+    with torch.no_grad():
+        scores = model(batch)["logits"].float()
+    assert kept == [False] * 3
+    kept.clear()
+    trained = trainer.forward_backward(batch)["logits"].float()
+    assert kept == [True] * 3
+    assert torch.equal(scores, trained.detach())
