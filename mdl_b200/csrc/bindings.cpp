@@ -1238,6 +1238,20 @@ at::Tensor window_attn_bwd(const at::Tensor& qkv, const at::Tensor& kstart, cons
   return dqkv;
 }
 
+// The gradient where the graph of a gradient is asked for: it has no derivative of its own, and
+// says so once one is wanted, instead of leaving its terms out.
+struct WindowedAttentionGrad : public torch::autograd::Function<WindowedAttentionGrad> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& qkv, const at::Tensor& kstart,
+                            const at::Tensor& out, const at::Tensor& out_lo, const at::Tensor& lse,
+                            const at::Tensor& dout, int64_t H, int64_t G, int64_t Lq, int64_t window, int64_t sinks,
+                            double scale, const at::Tensor& err) {
+    return window_attn_bwd(qkv, kstart, out, out_lo, lse, dout, H, G, Lq, window, sinks, scale, err);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    throw std::runtime_error("windowed attention: the CUDA kernels have no second derivative");
+  }
+};
+
 // The differentiable operator: saves what the backward reads, off the interpreter's lock.
 struct WindowedAttention : public torch::autograd::Function<WindowedAttention> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv, const at::Tensor& kstart,
@@ -1258,8 +1272,13 @@ struct WindowedAttention : public torch::autograd::Function<WindowedAttention> {
     const auto n = ctx->saved_data["args"].toIntVector();
     at::Tensor dout = grads[0].to(at::kBFloat16).contiguous();
     if (reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16) dout = dout.clone();
-    at::Tensor d = window_attn_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], dout, n[0], n[1], n[2], n[3], n[4],
-                                   ctx->saved_data["scale"].toDouble(), ctx->saved_data["err"].toTensor());
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const at::Tensor err = ctx->saved_data["err"].toTensor();
+    at::Tensor d = at::GradMode::is_enabled()
+                       ? WindowedAttentionGrad::apply(saved[0], saved[1], saved[2], saved[3], saved[4], dout, n[0], n[1],
+                                                      n[2], n[3], n[4], scale, err)
+                       : window_attn_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], dout, n[0], n[1], n[2], n[3],
+                                         n[4], scale, err);
     return {d, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
             at::Tensor(), at::Tensor()};
   }

@@ -20,7 +20,7 @@ tokens stay visible because a softmax trained with a window parks weight on them
   do not see the token (a weight of zero times it is a NaN).
 
 CUDA: the tcgen05 kernels of ``csrc/window_attn.cu`` (bf16, head widths 32 and 64), forward
-and backward without atomics. CPU: the same contract in fp32 PyTorch.
+and backward without atomics; a second derivative is refused. CPU: the same contract in fp32 PyTorch.
 """
 
 from __future__ import annotations

@@ -357,3 +357,26 @@ def test_forward_without_a_gradient_keeps_nothing_for_one():
                 assert torch.cuda.max_memory_allocated() - before <= out_bytes + lse_bytes + 4096
                 assert not out.requires_grad
                 del out
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_second_derivative_is_right_or_refused(device):
+    """The CPU definition has one; the kernels refuse it instead of leaving its terms out."""
+
+    qkv, dout = _inputs(1, 20, 20, 1, 1, 32, device)
+    ks = torch.zeros(1, dtype=torch.int32, device=device)
+    x = (qkv if device == "cuda" else qkv.float()).clone().requires_grad_()
+    out = windowed_attention(x, ks, 1, 20, 7, 1)
+    (dx,) = torch.autograd.grad(out, x, dout.to(out.dtype), create_graph=True)
+    assert dx.requires_grad
+    total = out.float().sum() + dx.float().square().sum()
+    if device == "cuda":
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(total, x)
+    else:
+        assert torch.isfinite(torch.autograd.grad(total, x)[0]).all()
+    # a first derivative in which it has no part stays possible
+    out = windowed_attention(x, ks, 1, 20, 7, 1)
+    (dx,) = torch.autograd.grad(out, x, dout.to(out.dtype), create_graph=True)
+    want = torch.autograd.grad(windowed_attention(x, ks, 1, 20, 7, 1), x, dout.to(out.dtype))[0]
+    assert torch.equal(dx.detach(), want)
