@@ -380,3 +380,71 @@ def test_a_second_derivative_is_right_or_refused(device):
     (dx,) = torch.autograd.grad(out, x, dout.to(out.dtype), create_graph=True)
     want = torch.autograd.grad(windowed_attention(x, ks, 1, 20, 7, 1), x, dout.to(out.dtype))[0]
     assert torch.equal(dx.detach(), want)
+
+
+def _rounded_gradients(q, k, v, do, seen):
+    """dQ and dK of one head in 64 bits: exact, with the kernels' roundings (P of the output and the
+    keys' dS to bf16, D from the output in two bf16 terms, the queries' dS in two), with D from the
+    rounded output, and with the queries' dS in one term."""
+
+    def bf(x):
+        return x.float().bfloat16().double()
+
+    scale = q.shape[1] ** -0.5
+    s = (q @ k.T * scale).masked_fill(~seen, -math.inf)
+    p, dp = torch.softmax(s, -1), do @ v.T
+    e = torch.exp(s - s.amax(-1, keepdim=True))
+    o = (bf(e) @ v) / e.sum(-1, keepdim=True)
+    high = bf(o)
+
+    def grads(d, terms):
+        ds = p * (dp - d)
+        hi = bf(ds)
+        return bf(scale * (hi + bf(ds - hi) if terms == 2 else hi) @ k), bf(scale * hi.T @ q)
+
+    def row_sum(x):
+        return (do * x).sum(-1, keepdim=True)
+
+    exact = p * (dp - row_sum(p @ v))
+    return {"exact": (scale * exact @ k, scale * exact.T @ q), "kernel": grads(row_sum(high + bf(o - high)), 2),
+            "rounded output": grads(row_sum(high), 2), "one term": grads(row_sum(high + bf(o - high)), 1)}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("gain,lost", [(2.0, "rounded output"), (0.5, "one term")])
+def test_gradient_keeps_its_second_terms(device, hd, gain, lost):
+    """The norm of the error of dQ (for D: of dK too) is that of the kernels' roundings, computed in 64
+    bits, and not that of a form which has lost the output's low part or the queries' second term of
+    dS. The limit is the geometric mean of the two, which are at least 1.2 apart for these inputs."""
+
+    L, H, window, sinks = 400, 2, 64, 2
+    g = torch.Generator().manual_seed(0)
+    qkv = torch.randn(1, L, 3 * H * hd, generator=g)
+    qkv[..., :2 * H * hd] *= gain
+    qkv = qkv.bfloat16()
+    dout = torch.randn(1, L, H * hd, generator=g).bfloat16()
+    i, j = torch.arange(L).view(-1, 1), torch.arange(L).view(1, -1)
+    seen = (j <= i) & ((i - j < window) | (j < sinks))
+    x = qkv[0].double().view(L, 3 * H, hd)
+    heads = [_rounded_gradients(x[:, h], x[:, H + h], x[:, 2 * H + h], dout[0].double().view(L, H, hd)[:, h], seen)
+             for h in range(H)]
+    forms = {name: [torch.cat([f[name][n] for f in heads], -1) for n in (0, 1)] for name in heads[0]}
+
+    def error(form, n):
+        return float((form[n] - forms["exact"][n]).norm() / forms["exact"][n].norm())
+
+    if device == "cuda":
+        leaf = qkv.cuda().requires_grad_()
+        out = windowed_attention(leaf, torch.zeros(1, dtype=torch.int32, device="cuda"), H, L, window, sinks)
+        (dx,) = torch.autograd.grad(out, leaf, dout.cuda())
+        dx = dx[0].double().cpu()
+        got = [dx[:, :H * hd], dx[:, H * hd:2 * H * hd]]
+    for n in ((0, 1) if lost == "rounded output" else (0,)):
+        now, without = error(forms["kernel"], n), error(forms[lost], n)
+        assert without > 1.2 * now
+        limit = math.sqrt(now * without)
+        if device == "cuda":
+            assert error(got, n) <= limit, (error(got, n), now, without)
+        else:
+            assert now <= limit < without
