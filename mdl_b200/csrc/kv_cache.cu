@@ -395,18 +395,23 @@ constexpr int min_blocks() {
 }
 template <int NT>
 constexpr int tiles_a_step() { return NT == 1 ? 4 : 2; }
-// Shared memory: a warp's ring of steps (K codes | V codes | scales), then their barriers; the
-// join of eight warps takes the same space afterwards.
+// Shared memory: the warps' rings of steps (K codes | V codes | scales), whose space the join of eight
+// warps takes afterwards; behind both the rings' barriers and a word a warp. The barriers keep a place of
+// their own: a barrier that lanes have waited on may still be written when the wait is over, and with the
+// join's maxima there (more than 8 query rows a block of 64-wide heads) some of these were lost.
 template <int HD, int NT>
 constexpr int step_bytes() { return 16 * tiles_a_step<NT>() * (HD + 4); }
 template <int HD>
 constexpr int ring_steps() { return HD == 64 ? 2 : 3; }
 template <int HD, int NT, int WPI>
-constexpr int attend_smem() {
-  constexpr int warps = WPI == 1 ? 4 : WPI;
-  constexpr int ring = warps * ring_steps<HD>() * (step_bytes<HD, NT>() + 8) + warps * 4;
+constexpr int attend_data() {
+  constexpr int ring = (WPI == 1 ? 4 : WPI) * ring_steps<HD>() * step_bytes<HD, NT>();
   constexpr int join = WPI == 1 ? 0 : WPI * 8 * NT * (HD + 6) * 4;
   return ring > join ? ring : join;
+}
+template <int HD, int NT, int WPI>
+constexpr int attend_smem() {
+  return attend_data<HD, NT, WPI>() + (WPI == 1 ? 4 : WPI) * (8 * ring_steps<HD>() + 4);
 }
 
 // Bulk copy into this CTA's shared memory, 16-byte aligned, counted on `bar`.
@@ -559,15 +564,17 @@ __global__ void __launch_bounds__(WPI == 1 ? 128 : 32 * WPI, min_blocks<HD, NT, 
   // A ring of steps in shared memory, filled by bulk copies: enough bytes under way to cover
   // the memory latency without registers for them.
   constexpr int RING = ring_steps<HD>(), STEP = step_bytes<HD, NT>(), TILE_CODES = 16 * HD / 2;
+  constexpr int BARS = attend_data<HD, NT, WPI>();
+  static_assert(BARS % 8 == 0, "barriers");
   extern __shared__ __align__(128) uint8_t sm_ring[];
   constexpr int WARPS = WPI == 1 ? 4 : WPI;
   uint8_t* ring = sm_ring + warp * RING * STEP;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ring + WARPS * RING * STEP) + warp * RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ring + BARS) + warp * RING;
   // Steps from all_lo + 1 (or up to S) to all_hi are visible to every query of the block. Once the warp
   // has met a page outside the cache, none is: every step is masked, by another look at the table. (In
   // shared memory: as a register that changes it made the kernels spill.)
   constexpr int BAD_PAGE = -0x7fffffff - 1;
-  volatile int* all_hi = reinterpret_cast<volatile int*>(sm_ring + WARPS * RING * (STEP + 8)) + warp;
+  volatile int* all_hi = reinterpret_cast<volatile int*>(sm_ring + BARS + WARPS * RING * 8) + warp;
   *all_hi = min(len, qmin + 1) - CH;
   const int all_lo = W > 0 ? qmax - W : -1, all_sink = S - CH;
   if (lane == 0) {

@@ -778,3 +778,31 @@ def test_an_empty_cache(device):
             check_error_word(torch.device("cuda", 0))
     with pytest.raises(ValueError):
         QuantizedKVCache(2, -1, 1, 32, device=device)
+
+
+@GPU
+@pytest.mark.parametrize("hd,H,G,B,N,lengths,fresh", [
+    (64, 10, 5, 4, 142, [405, 0, 273, 405], False), (64, 1, 1, 600, 10, [47, 0, 47, 20], True),
+    (64, 15, 5, 5, 133, [2645, 0, 472, 90], True), (64, 8, 8, 40, 16, [700, 1], True),
+    (32, 4, 4, 30, 32, [900, 64], True), (32, 8, 2, 60, 4, [1500, 33], False),
+])
+def test_repeated_calls_of_more_blocks_than_the_device_holds(hd, H, G, B, N, lengths, fresh):
+    """Blocks that follow one another on a multiprocessor join their warps in shared memory: every
+    call gives the same, near the fp32 definition."""
+
+    R, T = len(lengths), max(lengths)
+    cache = _shuffled(R, T, G, hd, 256, "cuda")
+    k, v = _kv(R, T, G, hd, "cuda", 11)
+    kv_cache_write(cache, k, v, start=_int([0] * R, "cuda"), kstart=_int([T - x for x in lengths], "cuda"))
+    g = torch.Generator().manual_seed(12)
+    q, kn, vn = torch.randn(B, N, (H + 2 * G) * hd, generator=g).bfloat16().cuda().split([H * hd, G * hd, G * hd], -1)
+    rows = torch.randint(0, R, (B,), generator=g).int().cuda()
+    if not fresh:
+        kn = vn = None
+    outs = [cached_attention(q, cache, rows=rows, k_new=kn, v_new=vn) for _ in range(60)]
+    ref = cached_attention_reference(q, cache, rows, kn, vn)
+    # |o| <= max |v| of what is seen: unit-normal values stay below 6
+    assert (outs[0].float() - ref).abs().max() <= 1.05 * 2.0 ** -7 * 6
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+    _check_errors("cuda")
