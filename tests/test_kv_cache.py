@@ -806,3 +806,66 @@ def test_repeated_calls_of_more_blocks_than_the_device_holds(hd, H, G, B, N, len
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
     _check_errors("cuda")
+
+
+@GPU
+@pytest.mark.parametrize("hd,G,page", [(32, 8, 64), (64, 1, 256)])
+def test_offsets_past_32_bits(hd, G, page):
+    """Rows whose pages lie at both ends of a pool of more than 2^32 bytes of codes, and an output of
+    more than 2^31 elements."""
+
+    per, T = 5, 5 * page - 3
+    num = 2 ** 32 // (G * page * hd) + 2 * per
+    table = torch.stack([torch.arange(per), torch.arange(num - per, num), torch.arange(num - 2 * per, num - per)]).int()
+    big = QuantizedKVCache(3, T, G, hd, page=page, table=table, num_pages=num, device="cuda")
+    assert big.codes.numel() > 2 ** 32
+    small = QuantizedKVCache(3, T, G, hd, page=page, device="cuda")
+    k, v = _kv(3, T, G, hd, "cuda", 3)
+    q = torch.randn(3, 2, 2 * G * hd, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    for c in (big, small):
+        kv_cache_write(c, k, v)
+    assert torch.equal(big.lengths, small.lengths)
+    for a, b in zip(kv_cache_read(big, T), kv_cache_read(small, T)):
+        assert torch.equal(a, b)
+    for window, sinks in ((0, 0), (50, 3)):
+        assert torch.equal(cached_attention(q, big, window=window, sinks=sinks),
+                           cached_attention(q, small, window=window, sinks=sinks))
+    del big
+    n = 2 ** 31 // (T * G * hd) + 2
+    rows = torch.zeros(n, dtype=torch.int32, device="cuda")
+    rows[-1] = 2
+    rk, rv = kv_cache_read(small, T, rows=rows)
+    assert rk.numel() > 2 ** 31
+    for got, want in ((rk, kv_cache_read(small, T)[0]), (rv, kv_cache_read(small, T)[1])):
+        assert torch.equal(got[-1], want[2]) and torch.equal(got[-2], want[0])
+    _check_errors("cuda")
+
+
+@GPU
+def test_sources_and_queries_past_32_bits():
+    """Tokens, queries and outputs of more than 2^31 elements."""
+
+    G, hd, R = 2, 32, 6
+    T = 2 ** 31 // (R * G * hd) // 8 + 9
+    wide = torch.zeros(R, T, 8, G * hd, dtype=torch.bfloat16, device="cuda")
+    assert wide.numel() > 2 ** 31
+    k, v = wide[:, :, 7], wide[:, :, 0]       # token strides of 8 rows
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k[:, -300:].normal_(generator=g)
+    v[:, -300:].normal_(generator=g)
+    cache = QuantizedKVCache(R, 300, G, hd, device="cuda")
+    kv_cache_write(cache, k, v, kstart=_int([T - 300] * R, "cuda"))
+    got, _ = kv_cache_read(cache, 300, dtype=torch.float32)
+    want = _round4(k[:, -300:].reshape(R, 300, G, hd)).view(R, 300, G * hd)
+    assert torch.equal(got.double(), want)
+    del wide, k, v
+    B, N, H = 2 ** 31 // (64 * 16 * hd) + 3, 64, 16
+    q = torch.zeros(B, N, H * hd, dtype=torch.bfloat16, device="cuda")
+    assert q.numel() > 2 ** 31
+    q[-2:].normal_(generator=g)
+    rows = (torch.arange(B, device="cuda") % R).int()
+    out = cached_attention(q, cache, rows=rows)
+    few = cached_attention(q[-2:], cache, rows=rows[-2:])
+    # another order of the same sums (see above); |v| < 6
+    assert (out[-2:].float() - few.float()).abs().max() <= 2 * 1.05 * 2.0 ** -7 * 6
+    _check_errors("cuda")

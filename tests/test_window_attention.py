@@ -448,3 +448,25 @@ def test_gradient_keeps_its_second_terms(device, hd, gain, lost):
             assert error(got, n) <= limit, (error(got, n), now, without)
         else:
             assert now <= limit < without
+
+
+@GPU
+def test_more_elements_than_32_bits_count():
+    """2,800 samples of 1,024 tokens: the last of them as by itself."""
+
+    B, L, H, hd, window, sinks = 2800, 1024, 8, 32, 60, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.zeros(B, L, 3 * H * hd, dtype=torch.bfloat16, device="cuda")
+    dout = torch.zeros(B, L, H * hd, dtype=torch.bfloat16, device="cuda")
+    assert qkv.numel() > 2 ** 31
+    qkv[-1:].normal_(generator=g)
+    dout[-1:].normal_(generator=g)
+    ks = torch.full((B,), 5, dtype=torch.int32, device="cuda")
+    x = qkv.requires_grad_()
+    o = windowed_attention(x, ks, H, L, window, sinks)
+    (dx,) = torch.autograd.grad(o, x, dout)
+    (out, otol), (grad, gtol) = _exact(qkv[-1:].detach(), [5], dout[-1:], H, H, L, window, sinks)
+    _close(o[-1:], out, otol)
+    _close(dx[-1:], grad, gtol)
+    assert not o[:-1].any() and not dx[:-1].any()
+    _errors()
