@@ -67,7 +67,8 @@ def error_word(device: torch.device | int) -> torch.Tensor:
         index = torch.cuda.current_device()
     word = _ERROR_WORDS.get(index)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        with torch.inference_mode(False):  # it outlives the mode in which it is first needed
+            word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
         _ERROR_WORDS[index] = word
     return word
 

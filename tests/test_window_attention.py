@@ -470,3 +470,21 @@ def test_more_elements_than_32_bits_count():
     _close(dx[-1:], grad, gtol)
     assert not o[:-1].any() and not dx[:-1].any()
     _errors()
+
+
+@GPU
+def test_error_word_first_used_in_inference_mode(monkeypatch):
+    """The device's error word can be cleared afterwards, outside the mode."""
+
+    from mdl_b200.ops import _ext
+
+    monkeypatch.setattr(_ext, "_ERROR_WORDS", {})
+    qkv = torch.zeros(1, 16, 96, dtype=torch.bfloat16, device="cuda")
+    with torch.inference_mode():
+        windowed_attention(qkv, torch.zeros(1, dtype=torch.int32, device="cuda"), 1, 16, 4)
+    word = _ext.error_word(qkv.device)
+    torch.cuda.synchronize()
+    word.fill_(8)
+    with pytest.raises(RuntimeError, match="outside"):
+        _ext.check_error_word(qkv.device)
+    assert int(word) == 0
