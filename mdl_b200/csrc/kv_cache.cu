@@ -345,18 +345,18 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvReadArgs a, int chu
 // instead of 16 rows are padding), and the codes, expanded in registers, are the A operand of
 // both products. tcgen05 needs 128 rows (and its operands in shared memory): the few queries
 // of a request do not fill that, and the kernel is bound by the expansion of the codes and
-// by memory, not by the products.
+// its latency, not by the products.
 //
 // The codes enter as code_pair gives them, 136 + c. K uses it as it is: S = q . (136 + c) - 136 * sum(q), the
 // second term being the accumulator's initial value. V subtracts 136 (one packed, exact
 // operation), since the same shortcut over a long sum of keys would cancel. The scales enter
 // in fp32: s_k multiplies the scores, s_v the probabilities.
 //
-// Bound: the instructions that expand the codes (about 12 a key of 64 values and warp, with the
-// softmax's) and not memory, whose bytes are a quarter of bf16's. 24 single tokens over 131,071
-// keys, 8 query heads on 2 key heads of 64: 121 us, 3.5 TB/s of cache; 1,024 samples of 32
-// candidates, 8 heads of 32, window 512 of 2,000 keys: 166 us, 108 TFLOP/s; one token over 501
-// keys: 4.5 us.
+// Bound by the latency of a step (expand, product, maximum, exponentials, product follow one another,
+// with 8 to 16 warps a multiprocessor to hide it): issue slots are 56 % busy, the pipe that expands the
+// codes 44 to 55 %, DRAM 4 to 40 %. 24 single tokens over 131,071 keys, 8 query heads on 2 key heads of
+// 64: 119 us, 3.6 TB/s of cache; 1,024 samples of 32 candidates, 8 heads of 32, window 512 of 2,000
+// keys: 165 us, 108 TFLOP/s; one token over 501 keys: 4.6 us.
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, float c0, float c1, float c2, float c3) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -386,9 +386,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Blocks an SM that the registers have to allow: the kernel hides its latencies with warps, up to
-// where it spills. 8 query rows a block: 32-wide heads with one warp an item, 256 rows of 2,000 keys:
-// five blocks 63 us, six (spilling) 67, seven 83; 64-wide ones with eight warps: two blocks 121 us
-// for 24 rows of 131,071 keys and 48 for 256 of 2,000, three (spilling) 127 and 46.
+// where it spills much. 8 query rows a block: 32-wide heads with one warp an item, 256 rows of 2,000
+// keys: five blocks 62 us, six (spilling) 67, seven 83; 64-wide ones with one warp, 4 heads: five blocks
+// (8 bytes spilled) 52 us for 2,000 rows of 300 keys and 75 for 1,000 of 1,000, four (none) 53 and 74;
+// with eight warps: two blocks 121 us for 24 rows of 131,071 keys and 48 for 256 of 2,000, three
+// (spilling) 127 and 46.
 template <int HD, int NT, int WPI>
 constexpr int min_blocks() {
   return WPI == 1 ? (NT == 1 ? 5 : (NT == 2 ? 4 : 3)) : (NT == 1 ? (HD == 64 ? 2 : 3) : (NT == 2 ? 2 : 1));
@@ -1122,6 +1124,10 @@ struct Plan {
 // 32,000 keys 88 | 49 | 29 | 18 | 12 | 12 us; 16 rows of 2,000 keys 10 | 10 | 12 | 16 | 21 | 31,
 // of 32,000 keys 101 | 69 | 68 | 61 | 64 | 73. Over 130 such shapes the choice is 1.2 % slower than
 // the best on average, and by 2 us or 5 % at most.
+//
+// The lengths are on the device, so that keys are counted by the capacity (or the window): rows that fill
+// little of it are split like full ones. 16 rows of 500 tokens, 8 heads of 32: 9.7 us with room for 512,
+// 14.9 with room for 131,072; 256 rows 19.1 and 25.4.
 Plan plan_of(const KvAttendArgs& a) {
   Plan p;
   const int M = a.N * (a.H / a.c.G);

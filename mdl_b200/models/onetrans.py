@@ -708,7 +708,9 @@ class OneTransModel(nn.Module):
         keys and their padding count; candidates then run only their NS tokens. Rows are the
         requests of the sequence payload (``row_indices``; one per row without it). With
         ``model.request_cache_format: 4bit`` a layer's K/V are a ``QuantizedKVCache``
-        (``head_dim + 4`` bytes a token and head instead of ``8 * head_dim``)."""
+        (``head_dim + 4`` bytes a token and head instead of ``8 * head_dim``). The layers run
+        their fp32 PyTorch definition, on CUDA too: the scores take ``4 * heads * s * s`` bytes
+        a request, with a window as without."""
 
         from .features import lookup_sequence
 

@@ -17,8 +17,9 @@ own (OneTrans NS tokens over their request's history), with an optional sliding
 window and always-visible first tokens. None of them has a gradient.
 
 CUDA: the kernels of ``csrc/kv_cache.cu`` (bf16, head widths 32 and 64); rows, pages
-and positions outside the cache are skipped and recorded in the device error word
-(``check_error_word``). CPU: the same contract in fp32 PyTorch.
+and positions outside the cache are skipped (attention: hidden) and recorded in the device
+error word (``check_error_word``). CPU: the same contract in fp32 PyTorch, which raises
+instead.
 """
 
 from __future__ import annotations
@@ -197,7 +198,8 @@ def kv_cache_write(cache: QuantizedKVCache, k: torch.Tensor, v: torch.Tensor, st
     """Quantises ``k, v [n, T, kv_heads * head_dim]`` into cache rows ``rows [n]`` (distinct;
     default all rows in order). Source row ``i``'s tokens ``kstart[i] ..`` (default 0: none is
     padding) go to positions ``start[i] ..`` (default: append), and the row's length becomes
-    the end of what was written."""
+    the end of what was written. A start past the row's length leaves a gap whose values are
+    not defined."""
 
     with trace_range("mdl.kv_cache.write"):
         if cache.err is not None:

@@ -8,7 +8,9 @@ will run has a kernel here, and describe which (reference ``_attention_runtime_d
   ``runtime.kernel_backend: torch``);
 * OneTrans with ``model.attention_window`` runs the tcgen05 windowed attention
   (``csrc/window_attn.cu``) and with ``model.request_cache_format: 4bit`` the 4-bit cache
-  kernels (``csrc/kv_cache.cu``), both for head_dim 32 and 64;
+  kernels (``csrc/kv_cache.cu``), both for head_dim 32 and 64. The request cache itself,
+  full or 4-bit, is built by the layers' fp32 PyTorch definition, whose scores grow with the
+  square of the history whatever the window;
 * MDL domain-aware attention and the task-query readout run the few-query kernel
   when both token counts are at most 64 (PyTorch SDPA beyond);
 * MixFormer / STCA single-query attention and the MDL-OneTrans sequence reader
